@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional, Sequence
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -51,6 +52,10 @@ EXPORTS = (
     "chitu_b200_scatter_rows",
     "chitu_b200_attn_q8_workspace_bytes",
     "chitu_b200_attn_fwd_q8",
+    "chitu_b200_rotary",
+    "chitu_b200_kv_append",
+    "chitu_b200_attn_cache_workspace_bytes",
+    "chitu_b200_attn_fwd_cache",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -96,6 +101,10 @@ class QPre(ctypes.Structure):
         ("n_t", ctypes.c_int), ("n_h", ctypes.c_int), ("pos_offset", ctypes.c_int64),
     ]
 
+
+# ``chitu_b200_kv_cache`` as bytes: a call packs it afresh, which takes a tenth of filling a ctypes structure field by field
+KV_CACHE = struct.Struct("4P" "3q3q2q2q" "3P" "q" "6i")
+CACHE_16BIT, CACHE_E4M3 = 0, 1
 
 SYNC_INTS = 64
 
@@ -240,6 +249,23 @@ def load() -> ctypes.CDLL:
         _i64p, _i64p, _i64p, ctypes.c_float, ctypes.c_int, ctypes.POINTER(QPre), ctypes.c_int, _vp, ctypes.c_int64,
         _vp, _vp,
     ]
+    lib.chitu_b200_rotary.restype = ctypes.c_int
+    lib.chitu_b200_rotary.argtypes = [
+        _vpp, _vpp, _i64p, _i64p, ctypes.POINTER(ctypes.c_int), ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
+        ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, _vp,
+    ]
+    lib.chitu_b200_kv_append.restype = ctypes.c_int
+    lib.chitu_b200_kv_append.argtypes = [
+        ctypes.c_char_p, _vp, _vp, _vp, _i64p, _i64p, _i64p, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
+        _vp, ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp,
+    ]
+    lib.chitu_b200_attn_cache_workspace_bytes.restype = ctypes.c_int64
+    lib.chitu_b200_attn_cache_workspace_bytes.argtypes = [ctypes.c_int, ctypes.c_int64] + [ctypes.c_int] * 5
+    lib.chitu_b200_attn_fwd_cache.restype = ctypes.c_int
+    lib.chitu_b200_attn_fwd_cache.argtypes = [
+        ctypes.c_char_p, _vp, _i64p, _vp, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_int,
+        ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int64, _vp, _vp,
+    ]
     lib.chitu_b200_peer_wait_outputs.restype = ctypes.c_int
     lib.chitu_b200_peer_wait_outputs.argtypes = [ctypes.POINTER(PeerSyncDesc), _vp, _vp]
     lib.chitu_b200_set_flag_wait_cycles.restype = ctypes.c_longlong
@@ -273,6 +299,7 @@ def ptr_array(ptrs: Sequence[int]):
     return (ctypes.c_void_p * len(ptrs))(*[int(p) for p in ptrs])
 
 
+_I64x2 = ctypes.c_int64 * 2
 _I64x4 = ctypes.c_int64 * 4
 
 

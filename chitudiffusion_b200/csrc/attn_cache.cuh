@@ -1,0 +1,611 @@
+// Attention of packed queries over a paged key/value cache, head_dim 128: what is common to its kernels, and the kernel
+// for few query rows per sequence and key head (single tokens, a few of them).
+//
+//   out_i = sum_j softmax_j(scale q_i . K_j) V_j,   j < lens[b], with `causal` j <= lens[b] - n_b + i
+//
+// Query row r of sequence b and key head h is token r / group, query head h * group + r % group: the heads that share keys
+// are rows of one tile, so keys and values are read once for all of them.
+//
+// 8-bit pages hold e4m3 codes k8, v8 with scales ks, vs for each page and head.  Codes are exact in fp16, so they are
+// widened to fp16 and never rounded; scales enter in fp32:
+//   score  s = (scale ks) (q . k8);   p = 2^(s log2e + log2 vs - m);   o = sum p v8,   l = sum p / vs
+// The value scale sits in the exponent, so the running maximum m is that of p itself and the 16-bit probabilities use their
+// range whatever the scales are.  A bf16 query row is brought to fp16 by a power of two of its own (bf16 values of one row are
+// 2^-24 of its largest before fp16 drops any of their bits), which goes into the score's factor.
+#pragma once
+
+#include "attn_fwd.cuh"
+#include "kv_cache.cuh"
+
+namespace chitu {
+
+struct CacheAttnParams {
+  const void* q;  // [tokens, heads_q, 128], element strides
+  long long q_token, q_head;
+  void* out;      // [tokens, heads_q, 128] contiguous
+  float* lse;     // [heads_q, tokens] fp32 natural log, or nullptr
+  const uint8_t* cache[2];                     // k, v
+  long long c_page[2], c_token[2], c_head[2];  // strides, bytes
+  const float* scale[2];                       // 8-bit pages: one fp32 per page and head
+  long long s_page[2], s_head[2];              // strides, elements
+  const int* block_table;
+  long long table_stride;
+  const int* lens;
+  const int* cu;
+  int* status;
+  int batch, tokens, width, n_pages, heads_kv, group, page_shift, causal;
+  float scale_log2;  // softmax_scale * log2(e)
+  // work split over the grid (see each kernel) and scratch for pieces of a row's keys
+  int min_tiles;
+  int* count;
+  float* part;
+};
+
+// Lengths of one sequence, brought into what the table and the packed queries can hold.
+struct SeqInfo {
+  int tok0, n_new, len, first;  // first packed token, tokens, keys, position of the first token
+};
+__device__ __forceinline__ SeqInfo seq_info(const CacheAttnParams& p, int b) {
+  SeqInfo s;
+  s.tok0 = min(max(__ldg(p.cu + b), 0), p.tokens);
+  s.n_new = min(max(__ldg(p.cu + b + 1), s.tok0), p.tokens) - s.tok0;
+  const int raw = __ldg(p.lens + b);
+  s.len = static_cast<int>(min(static_cast<long long>(max(raw, 0)), static_cast<long long>(p.width) << p.page_shift));
+  s.first = raw - s.n_new;
+  return s;
+}
+
+// probabilities are kept at up to 2^(kProbShift + kRescaleThreshold) in fp16, whose range would otherwise end 2^-24 below
+// the row's maximum
+constexpr float kProbShift = 7.f;
+constexpr float kMinValueScale = 1e-30f;  // (a value scale of zero has no logarithm; its codes are zero)
+
+__device__ __forceinline__ void mma_16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_16816_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool kHalf>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kHalf)
+    mma_16816_f16(d, a, b0, b1);
+  else
+    mma_16816_bf16(d, a, b0, b1);
+}
+__device__ __forceinline__ uint32_t widen_e4m3x2(uint32_t two_codes) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two_codes)));
+  return h;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  const int n = take ? 16 : 0;  // (0: the destination is filled with zeros)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// ----------------------------------------------------------------------------
+// rows kernel: 16 query rows of one key head per unit, warp-level matrix instructions
+// ----------------------------------------------------------------------------
+//
+// Memory bound: a key and a value byte are read once for at most 16 rows.  The grid's CTAs share all (sequence, 16 rows, key
+// head, 64-key tile) steps evenly, in that order: CTA c takes the c-th of gridDim.x equal runs, whatever the lengths are.  A
+// run that ends inside an item (sequence, rows, head) leaves the item's fp32 piece in scratch, and the CTA that completes the
+// item's count merges its pieces in order; nobody waits.
+//
+// A warp takes 16 of a tile's 64 keys and keeps its own softmax.  The matrix instructions' sum over channels and the output's
+// channels may be numbered as is convenient, so a lane's fragments are whole 16-byte pieces of cache rows: for q k^T, of key
+// lane / 4, the pieces lane % 4; for p v, of four keys, the piece lane / 4.  A lane copies exactly the bytes that it reads
+// itself (cp.async, kStages steps deep, over item borders), so the warps need no barrier inside a run; lanes 0 and 1 fetch the
+// scales of the warp's keys beside them.
+constexpr int kRowsWarps = 4;
+constexpr int kRowsThreads = kRowsWarps * 32;
+constexpr int kRowsTile = 16 * kRowsWarps;
+constexpr int kRowsMergeBytes = 2 * 16 * 32 * 16;  // two warps' accumulators
+template <bool kEightBit>
+struct RowsShape {
+  static constexpr int stages = kEightBit ? 5 : 4;
+  static constexpr int step_bytes = kEightBit ? 4096 : 8192;  // 16 keys and values
+  static constexpr int stage_bytes = step_bytes + 16;  // and the scales of the keys' page, and whether there is one
+  static constexpr int smem = kRowsWarps * stages * stage_bytes + kRowsMergeBytes + kRowsWarps * 16 * 8 + 16;
+};
+// scratch of one piece: 16 x 32 float4 of the accumulator's fragments, then (maximum, sum) of 16 rows
+constexpr int kRowsPieceFloats = 16 * 32 * 4 + 32;
+
+// Position in the order of steps.
+struct RowsCursor {
+  int b, rb, h, tile;   // sequence, 16-row block, key head, 64-key tile
+  int n_rb, n_tiles;    // of the sequence
+  SeqInfo seq;
+  __device__ __forceinline__ void measure(const CacheAttnParams& p) {
+    seq = seq_info(p, b);
+    n_rb = (seq.n_new * p.group + 15) >> 4;
+    n_tiles = max((seq.len + kRowsTile - 1) / kRowsTile, 1);
+  }
+  __device__ __forceinline__ void next_item(const CacheAttnParams& p) {
+    tile = 0;
+    if (++h < p.heads_kv) return;
+    h = 0;
+    if (++rb < n_rb) return;
+    rb = 0;
+    while (++b < p.batch) {
+      measure(p);
+      if (n_rb > 0) return;
+    }
+  }
+};
+__device__ __forceinline__ long long rows_steps(const CacheAttnParams& p, int b) {
+  const SeqInfo s = seq_info(p, b);
+  const long long n_rb = (static_cast<long long>(s.n_new) * p.group + 15) >> 4;
+  return n_rb * p.heads_kv * max((s.len + kRowsTile - 1) / kRowsTile, 1);
+}
+
+// Query rows g and g + 8 as matrix fragments: for 8-bit pages piece j (64 channels), step k (16 of them) is channels
+// 64 j + 16 c + 4 k + {0, 1, 2, 3} of lane c; for 16-bit pages 32 j + 8 c + 4 k + ....
+template <bool kFp16, bool kEightBit>
+__device__ __forceinline__ void rows_load_q(const CacheAttnParams& p, const RowsCursor& cur, int g, int c, uint32_t (&qf)[8][4], float (&factor)[2]) {
+  constexpr int kPieces = kEightBit ? 2 : 4, kSteps = kEightBit ? 4 : 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = cur.rb * 16 + g + 8 * i;
+    const int tok = r / p.group, hq = cur.h * p.group + r - tok * p.group;
+    const bool live = tok < cur.seq.n_new;
+    uint4 w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = make_uint4(0, 0, 0, 0);
+    if (live) {
+      const uint16_t* row = static_cast<const uint16_t*>(p.q) + (cur.seq.tok0 + tok) * p.q_token + hq * p.q_head;
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+        for (int k = 0; k < kSteps / 2; ++k) w[j * (kSteps / 2) + k] = __ldg(reinterpret_cast<const uint4*>(row + j * (128 / kPieces) + c * (32 / kPieces) + 8 * k));
+    }
+    factor[i] = p.scale_log2;
+    uint32_t v[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[4 * k] = w[k].x;
+      v[4 * k + 1] = w[k].y;
+      v[4 * k + 2] = w[k].z;
+      v[4 * k + 3] = w[k].w;
+    }
+    if constexpr (kEightBit && !kFp16) {
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(v[k] << 16)), fabsf(__uint_as_float(v[k] & 0xffff0000u))));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // row / 2^(exponent of its largest): below 2, exact in fp16 down to 2^-24
+      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253);
+      const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+      factor[i] *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = pack2<true>(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
+    }
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      qf[s][i] = v[2 * s];
+      qf[s][2 + i] = v[2 * s + 1];
+    }
+  }
+}
+
+// Accumulators of the CTA's warps for one item, brought to a common maximum and summed by warp 0 (others: undefined).
+__device__ __forceinline__ void rows_join(float (&o)[16][4], float (&m)[2], float (&l)[2], float4* buf, float2* stat, int warp, int lane) {
+  const int g = lane >> 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    if ((lane & 3) == 0) stat[warp * 16 + g + 8 * i] = make_float2(m[i], l[i]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, stat[w * 16 + g + 8 * i].x);
+#pragma unroll
+    for (int w = 0; w < kRowsWarps; ++w) {
+      const float2 s = stat[w * 16 + g + 8 * i];
+      sum += s.x == -INFINITY ? 0.f : s.y * fast_exp2(s.x - top);
+    }
+    const float f = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - top);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      o[t][2 * i] *= f;
+      o[t][2 * i + 1] *= f;
+    }
+    m[i] = top;
+    l[i] = sum;
+  }
+#pragma unroll
+  for (int half = kRowsWarps / 2; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t) buf[(warp - half) * 512 + t * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
+    }
+    __syncthreads();
+    if (warp < half) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        const float4 v = buf[warp * 512 + t * 32 + lane];
+        o[t][0] += v.x;
+        o[t][1] += v.y;
+        o[t][2] += v.z;
+        o[t][3] += v.w;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <bool kFp16, bool kEightBit>
+__global__ void __launch_bounds__(kRowsThreads)
+attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
+  using Shape = RowsShape<kEightBit>;
+  constexpr int kStages = Shape::stages;
+  constexpr bool kHalf = kEightBit || kFp16;  // fp16 products
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * Shape::stage_bytes;
+  float4* join_buf = reinterpret_cast<float4*>(smem + kRowsWarps * kStages * Shape::stage_bytes);
+  float2* join_stat = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(join_buf) + kRowsMergeBytes);
+  volatile int* last_flag = reinterpret_cast<volatile int*>(join_stat + kRowsWarps * 16);
+
+  // all steps, and where this CTA's run begins (each warp finds out by itself)
+  long long total = 0;
+  for (int b = lane; b < p.batch; b += 32) total += rows_steps(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(p.min_tiles));
+  const long long lo = blockIdx.x * per, hi = min(lo + per, total);
+  if (lo >= hi) return;
+  RowsCursor cur;
+  long long at = 0;  // steps before sequence cur.b
+  for (cur.b = 0;; cur.b += 32) {
+    const int b = cur.b + lane;
+    const long long mine = b < p.batch ? rows_steps(p, b) : 0;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, at + upto > lo);
+    if (past != 0) {
+      const int i = __ffs(past) - 1;
+      at += __shfl_sync(0xffffffffu, upto - mine, i);
+      cur.b += i;
+      break;
+    }
+    at += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  cur.measure(p);
+  long long item_start;  // first step of the item under the cursor
+  {
+    const long long item = (lo - at) / cur.n_tiles;
+    cur.rb = static_cast<int>(item / p.heads_kv);
+    cur.h = static_cast<int>(item - static_cast<long long>(cur.rb) * p.heads_kv);
+    item_start = at + item * cur.n_tiles;
+    cur.tile = static_cast<int>(lo - item_start);
+  }
+  RowsCursor ahead = cur;  // what is copied next
+  long long copied = lo;
+  auto page_of = [&](const RowsCursor& w) {  // page of this warp's 16 keys (they never cross a page), -1: none
+    const int key = w.tile * kRowsTile + warp * 16;
+    if (key >= w.seq.len) return -1;
+    const int id = __ldg(p.block_table + w.b * p.table_stride + (key >> p.page_shift));
+    return id >= 0 && id < p.n_pages ? id : -1;
+  };
+  int ahead_page = page_of(ahead);
+  auto copy_step = [&](int stage) {
+    const uint32_t meta = ring + stage * Shape::stage_bytes + Shape::step_bytes;
+    const uint32_t dst = ring + stage * Shape::stage_bytes + lane * 16;
+    if (kEightBit && lane < 2 && ahead_page >= 0) cp_async4(meta + 4 * lane, p.scale[lane] + ahead_page * p.s_page[lane] + ahead.h * p.s_head[lane]);
+    if (lane == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(meta + 8), "r"(ahead_page >= 0 ? 1 : 0) : "memory");
+    const int key0 = ahead.tile * kRowsTile + warp * 16;
+    const int in_page = key0 & ((1 << p.page_shift) - 1);
+    const int left = ahead_page < 0 ? 0 : ahead.seq.len - key0;  // keys of the 16 that exist
+    const long long id = max(ahead_page, 0);
+    const uint8_t* k = p.cache[0] + id * p.c_page[0] + ahead.h * p.c_head[0] + in_page * p.c_token[0] + c * 16;
+    const uint8_t* v = p.cache[1] + id * p.c_page[1] + ahead.h * p.c_head[1] + in_page * p.c_token[1] + g * (kEightBit ? 16 : 32);
+    constexpr int kPieces = kEightBit ? 2 : 4;
+    // (a row that does not exist: nothing is read, but the address stays inside the page)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const bool there = g + 8 * n < left;
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) cp_async16(dst + (n * kPieces + j) * 512, k + (there ? (g + 8 * n) * p.c_token[0] : 0) + j * 64, there);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int key = 2 * c + (n & 1) + (n >> 1) * 8;
+      const bool there = key < left;
+#pragma unroll
+      for (int j = 0; j < kPieces / 2; ++j)
+        cp_async16(dst + (2 * kPieces + n * (kPieces / 2) + j) * 512, v + (there ? key * p.c_token[1] : 0) + j * 16, there);
+    }
+  };
+  auto advance_copy = [&] {
+    if (++ahead.tile == ahead.n_tiles) ahead.next_item(p);
+    ++copied;
+    if (copied < hi) ahead_page = page_of(ahead);
+  };
+#pragma unroll 1
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (copied < hi) {
+      copy_step(s);
+      advance_copy();
+    }
+    cp_async_commit();
+  }
+
+  uint32_t qf[8][4];
+  float factor[2], o[16][4], m[2], l[2];
+  int limit[2];
+  int stage = 0;
+  bool fresh = true;
+#pragma unroll 1
+  for (long long step = lo; step < hi; ++step) {
+    if (fresh) {
+      rows_load_q<kFp16, kEightBit>(p, cur, g, c, qf, factor);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = cur.rb * 16 + g + 8 * i;
+        limit[i] = p.causal ? min(cur.seq.first + r / p.group + 1, cur.seq.len) : cur.seq.len;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+      }
+#pragma unroll
+      for (int t = 0; t < 16; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+      fresh = false;
+    }
+    const int key0 = cur.tile * kRowsTile + warp * 16;
+    cp_async_wait<kStages - 2>();
+    __syncwarp();  // (the scales are lanes 0's and 1's copies)
+    const uint32_t src = ring + stage * Shape::stage_bytes + lane * 16;
+    const uint4 meta = ld_shared16(ring + stage * Shape::stage_bytes + Shape::step_bytes);
+    const bool paged = meta.z != 0;
+    float k_scale = 1.f, v_log2 = 0.f, v_inv = 1.f;
+    if (kEightBit && paged) {
+      k_scale = __uint_as_float(meta.x);
+      const float vs = fmaxf(__uint_as_float(meta.y), kMinValueScale);
+      v_log2 = __log2f(vs);
+      v_inv = __fdividef(1.f, vs);
+    }
+    float s[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      if constexpr (kEightBit) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 w = ld_shared16(src + (n * 2 + j) * 512);
+          const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_16816_f16(s[n], qf[j * 4 + k], widen_e4m3x2(w4[k]), widen_e4m3x2(w4[k] >> 16));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 w = ld_shared16(src + (n * 4 + j) * 512);
+          mma_16816<kHalf>(s[n], qf[j * 2], w.x, w.y);
+          mma_16816<kHalf>(s[n], qf[j * 2 + 1], w.z, w.w);
+        }
+      }
+    }
+    // scores of rows g (e = 0, 1) and g + 8 (e = 2, 3), keys key0 + 8 n + 2 c + (e & 1), in units of log2
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float f = factor[i] * k_scale;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[n][2 * i + e];
+          x = fmaf(x, f, v_log2);
+          if (!paged || key0 + 8 * n + 2 * c + e >= limit[i]) x = -INFINITY;
+          top[i] = fmaxf(top[i], x);
+        }
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] + kRescaleThreshold || top[1] > m[1] + kRescaleThreshold)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float t = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        if (t > m[i] + kRescaleThreshold) {
+          const float f = fast_exp2(m[i] - t);  // (no maximum yet: 0)
+          m[i] = t;
+          l[i] *= f;
+#pragma unroll
+          for (int tt = 0; tt < 16; ++tt) {
+            o[tt][2 * i] *= f;
+            o[tt][2 * i + 1] *= f;
+          }
+        }
+      }
+    }
+    uint32_t pf[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float shift = m[i] == -INFINITY ? 0.f : kProbShift - m[i];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float a = fast_exp2(s[n][2 * i] + shift), b = fast_exp2(s[n][2 * i + 1] + shift);
+        l[i] = fmaf(a + b, v_inv, l[i]);
+        pf[n * 2 + i] = pack2<kHalf>(a, b);
+      }
+    }
+    // o += p v: lane's channels 16 g + t, t = 0 .. 15
+    if constexpr (kEightBit) {
+      uint4 w[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) w[n] = ld_shared16(src + (4 + n) * 512);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t r0 = q == 0 ? w[0].x : q == 1 ? w[0].y : q == 2 ? w[0].z : w[0].w;
+        const uint32_t r1 = q == 0 ? w[1].x : q == 1 ? w[1].y : q == 2 ? w[1].z : w[1].w;
+        const uint32_t r2 = q == 0 ? w[2].x : q == 1 ? w[2].y : q == 2 ? w[2].z : w[2].w;
+        const uint32_t r3 = q == 0 ? w[3].x : q == 1 ? w[3].y : q == 2 ? w[3].z : w[3].w;
+        const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
+        const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
+        mma_16816_f16(o[4 * q], pf, widen_e4m3x2(lo01), widen_e4m3x2(lo23));
+        mma_16816_f16(o[4 * q + 1], pf, widen_e4m3x2(lo01 >> 16), widen_e4m3x2(lo23 >> 16));
+        mma_16816_f16(o[4 * q + 2], pf, widen_e4m3x2(hi01), widen_e4m3x2(hi23));
+        mma_16816_f16(o[4 * q + 3], pf, widen_e4m3x2(hi01 >> 16), widen_e4m3x2(hi23 >> 16));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint4 w[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) w[n] = ld_shared16(src + (8 + n * 2 + j) * 512);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t r0 = q == 0 ? w[0].x : q == 1 ? w[0].y : q == 2 ? w[0].z : w[0].w;
+          const uint32_t r1 = q == 0 ? w[1].x : q == 1 ? w[1].y : q == 2 ? w[1].z : w[1].w;
+          const uint32_t r2 = q == 0 ? w[2].x : q == 1 ? w[2].y : q == 2 ? w[2].z : w[2].w;
+          const uint32_t r3 = q == 0 ? w[3].x : q == 1 ? w[3].y : q == 2 ? w[3].z : w[3].w;
+          mma_16816<kHalf>(o[8 * j + 2 * q], pf, __byte_perm(r0, r1, 0x5410), __byte_perm(r2, r3, 0x5410));
+          mma_16816<kHalf>(o[8 * j + 2 * q + 1], pf, __byte_perm(r0, r1, 0x7632), __byte_perm(r2, r3, 0x7632));
+        }
+      }
+    }
+    // the stage read in the step before this one is free: every lane has been through this step's __syncwarp since
+    const int refill = stage == 0 ? kStages - 1 : stage - 1;
+    if (copied < hi) {
+      copy_step(refill);
+      advance_copy();
+    }
+    cp_async_commit();
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+
+    const bool item_done = cur.tile + 1 == cur.n_tiles;
+    if (!item_done && step + 1 < hi) {
+      ++cur.tile;
+      continue;
+    }
+    // ---- the run leaves this item
+    rows_join(o, m, l, join_buf, join_stat, warp, lane);
+    const long long item_end = item_start + cur.n_tiles;
+    const long long c_first = item_start / per, c_last = (item_end - 1) / per;
+    bool write = warp == 0;
+    if (c_first != c_last) {
+      auto piece = [&](long long cta) {  // an item starts a CTA's run, or is the last of it
+        return p.part + (2 * cta + (item_start > cta * per ? 1 : 0)) * kRowsPieceFloats;
+      };
+      if (warp == 0) {
+        float4* mine = reinterpret_cast<float4*>(piece(blockIdx.x));
+#pragma unroll
+        for (int t = 0; t < 16; ++t) mine[t * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
+        if (c == 0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) reinterpret_cast<float2*>(mine + 512)[g + 8 * i] = make_float2(m[i], l[i]);
+        }
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+          const int before = atomicAdd(p.count + c_first, 1);
+          const int last = before == c_last - c_first;
+          if (last) p.count[c_first] = 0;
+          __threadfence();
+          *last_flag = last;
+        }
+      }
+      __syncthreads();
+      write = *last_flag != 0;
+      if (write) {
+        // the warps share the pieces; each keeps its own maximum, and they join as after a run
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          m[i] = -INFINITY;
+          l[i] = 0.f;
+        }
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
+        for (long long i = c_first + warp; i <= c_last; i += kRowsWarps) {
+          const float4* from = reinterpret_cast<const float4*>(piece(i));
+          float2 st[2];
+          float mine[2], theirs[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            st[r] = __ldcg(reinterpret_cast<const float2*>(from + 512) + g + 8 * r);
+            const float t = fmaxf(m[r], st[r].x);
+            mine[r] = m[r] == -INFINITY ? 0.f : fast_exp2(m[r] - t);
+            theirs[r] = st[r].x == -INFINITY ? 0.f : fast_exp2(st[r].x - t);
+            m[r] = t;
+            // (summed over the four lanes of a row when the warps join)
+            l[r] = l[r] * mine[r] + (c == 0 ? st[r].y * theirs[r] : 0.f);
+          }
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            const float4 v = __ldcg(from + t * 32 + lane);
+            o[t][0] = o[t][0] * mine[0] + v.x * theirs[0];
+            o[t][1] = o[t][1] * mine[0] + v.y * theirs[0];
+            o[t][2] = o[t][2] * mine[1] + v.z * theirs[1];
+            o[t][3] = o[t][3] * mine[1] + v.w * theirs[1];
+          }
+        }
+        rows_join(o, m, l, join_buf, join_stat, warp, lane);
+        write = warp == 0;
+      } else {
+        __syncthreads();  // (the flag has been read before a later item sets it)
+      }
+    }
+    if (write) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = cur.rb * 16 + g + 8 * i;
+        const int tok = r / p.group, hq = cur.h * p.group + r - tok * p.group;
+        if (tok < cur.seq.n_new) {
+          const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+          const size_t row = static_cast<size_t>(cur.seq.tok0 + tok);
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            // (accumulator t, column 2 c + e: channel 16 (2 c + e) + t)
+            uint32_t w[8];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) w[t] = pack2<kFp16>(o[2 * t][2 * i + e] * inv, o[2 * t + 1][2 * i + e] * inv);
+            uint4* d = reinterpret_cast<uint4*>(dst + 16 * (2 * c + e));
+            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+          if (p.lse != nullptr && c == 0)
+            p.lse[static_cast<size_t>(hq) * p.tokens + row] = l[i] > 0.f ? (m[i] - kProbShift + log2f(l[i])) * 0.6931471805599453f : -INFINITY;
+        }
+      }
+    }
+    if (step + 1 < hi) {
+      item_start = item_end;
+      cur.next_item(p);
+      fresh = true;
+    }
+  }
+  cp_async_wait<0>();
+}
+
+}  // namespace chitu

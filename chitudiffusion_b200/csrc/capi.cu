@@ -14,6 +14,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "capi_common.cuh"
 #include "attn_fwd.cuh"
 #include "attn_persist.cuh"
 #include "elementwise.cuh"
@@ -21,11 +22,9 @@
 #include "quant.cuh"
 #include "attn_q8.cuh"
 
-namespace {
+static thread_local char g_err[512] = "";
 
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
+int chitu::fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -33,9 +32,14 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-int cuda_fail(cudaError_t e, const char* what) {
+int chitu::cuda_fail(cudaError_t e, const char* what) {
   return fail(CHITU_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
+
+namespace {
+
+using chitu::cuda_fail;
+using chitu::fail;
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -136,7 +140,7 @@ int chitu_b200_version(void) { return 100; }
 
 unsigned chitu_b200_caps(void) {
   return CHITU_CAP_ATTN_BF16 | CHITU_CAP_ATTN_FP16 | CHITU_CAP_NORM_ROPE | CHITU_CAP_LSE_COMBINE | CHITU_CAP_A2A_LAYOUT |
-         CHITU_CAP_PEER_EXCHANGE | CHITU_CAP_ATTN_Q8;
+         CHITU_CAP_PEER_EXCHANGE | CHITU_CAP_ATTN_Q8 | CHITU_CAP_KV_CACHE;
 }
 
 const char* chitu_b200_last_error(void) { return g_err; }

@@ -1,0 +1,301 @@
+// extern "C" boundary of the paged key/value cache: argument checks and launches.  As in capi.cu nothing here allocates device
+// memory, synchronises the device or throws.
+#include "capi_common.cuh"
+
+#include <algorithm>
+#include <mutex>
+
+#include "attn_cache.cuh"
+
+namespace {
+
+using chitu::cuda_fail;
+using chitu::fail;
+
+constexpr int64_t kHeaderBytes = CHITU_SPLITKV_HEADER_BYTES;
+constexpr int kMaxDevices = 64;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int page_shift_of(int page) {
+  for (int s = 4; s <= 8; ++s)
+    if (page == 1 << s) return s;
+  return -1;
+}
+
+// Element strides of a [tokens, heads, D] tensor: multiples of 16 bytes, positive where the extent is above one.
+bool strides_fit(const int64_t* st, int64_t extent0, int64_t extent1, int bytes) {
+  return (extent0 <= 1 || (st[0] > 0 && (st[0] * bytes) % 16 == 0)) && (extent1 <= 1 || (st[1] > 0 && (st[1] * bytes) % 16 == 0));
+}
+
+int check_cache(const chitu_b200_kv_cache* c, const char* what) {
+  if (!c) return fail(CHITU_E_INVALID, "%s: null cache descriptor", what);
+  if (!c->k || !c->v || !c->block_table || !c->lens || !c->cu_seqlens) return fail(CHITU_E_INVALID, "%s: null pointer in the cache descriptor", what);
+  if (c->format != CHITU_CACHE_16BIT && c->format != CHITU_CACHE_E4M3) return fail(CHITU_E_UNSUPPORTED, "%s: pages must be 16-bit or e4m3", what);
+  if (c->format == CHITU_CACHE_E4M3 && (!c->k_scale || !c->v_scale)) return fail(CHITU_E_INVALID, "%s: 8-bit pages need k_scale and v_scale", what);
+  if (page_shift_of(c->page_size) < 0) return fail(CHITU_E_UNSUPPORTED, "%s: page_size must be 16, 32, 64, 128 or 256 (got %d)", what, c->page_size);
+  if (c->batch < 0 || c->table_width < 1 || c->n_pages < 1 || c->heads < 1 || c->table_stride < 0)
+    return fail(CHITU_E_INVALID, "%s: bad batch, table or page count", what);
+  const int es = c->format == CHITU_CACHE_E4M3 ? 1 : 2;
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(CHITU_E_INVALID, "%s: pages must be 16-byte aligned", what);
+  for (const int64_t* st : {c->k_strides, c->v_strides}) {
+    const int64_t extents[3] = {c->n_pages, c->page_size, c->heads};
+    for (int i = 0; i < 3; ++i)
+      if (extents[i] > 1 && (st[i] <= 0 || (st[i] * es) % 16 != 0))
+        return fail(CHITU_E_INVALID, "%s: cache stride[%d] = %lld must be positive and a multiple of 16 bytes", what, i, static_cast<long long>(st[i]));
+  }
+  return CHITU_OK;
+}
+
+int check_table(const float* table, int64_t rows, int rot, const char* what) {
+  if (!aligned16(table)) return fail(CHITU_E_INVALID, "%s: the rotary table must be 16-byte aligned", what);
+  if (rot < 16 || (rot & 15) || rows < 0) return fail(CHITU_E_UNSUPPORTED, "%s: rotated channels must be a positive multiple of 16 (got %d)", what, rot);
+  return CHITU_OK;
+}
+
+// More than 48 KB of shared memory is granted once per device and kernel.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices]) {
+  static std::mutex mu;
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done[dev] = true;
+  }
+  return e;
+}
+
+constexpr int kSms = 148;
+
+// Grid of the rows kernel: all CTAs resident at once (two per SM).
+constexpr int kRowsGrid = kSms * 2;
+constexpr int kRowsMinTiles = 2;
+int64_t rows_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kRowsGrid) * 2 * chitu::kRowsPieceFloats * 4; }
+
+template <bool kFp16, bool kEightBit>
+cudaError_t launch_rows(const chitu::CacheAttnParams& p, cudaStream_t st) {
+  static bool done[kMaxDevices] = {};
+  constexpr int smem = chitu::RowsShape<kEightBit>::smem;
+  cudaError_t e = allow_smem(chitu::attn_cache_rows_kernel<kFp16, kEightBit>, smem, done);
+  if (e != cudaSuccess) return e;
+  chitu::attn_cache_rows_kernel<kFp16, kEightBit><<<kRowsGrid, chitu::kRowsThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+int chitu_b200_rotary(const void* const* x, void* const* out, const int64_t* x_strides, const int64_t* out_strides,
+                      const int* heads, int n, int64_t tokens, int head_dim, int rot, int dtype, const void* positions,
+                      int positions_are_int64, const float* table, int64_t table_rows, int interleaved, void* stream) {
+  if (!x || !out || !x_strides || !out_strides || !heads || !positions || !table) return fail(CHITU_E_INVALID, "rotary: null pointer");
+  if (n < 1 || n > 3) return fail(CHITU_E_UNSUPPORTED, "rotary: one to three tensors (got %d)", n);
+  if (dtype < 0 || dtype > 2) return fail(CHITU_E_UNSUPPORTED, "rotary: dtype must be bf16, fp16 or fp32");
+  if (head_dim < 16 || head_dim > 512 || (head_dim & 15)) return fail(CHITU_E_UNSUPPORTED, "rotary: head_dim must be a multiple of 16 up to 512 (got %d)", head_dim);
+  if (rot > head_dim) return fail(CHITU_E_INVALID, "rotary: %d rotated channels of %d", rot, head_dim);
+  if (int rc = check_table(table, table_rows, rot, "rotary")) return rc;
+  if (tokens < 0 || tokens > 0x7fffffff) return fail(CHITU_E_INVALID, "rotary: bad token count");
+  const int es = dtype == CHITU_DTYPE_FP32 ? 4 : 2;
+  chitu::RotaryParams p;
+  p.n_jobs = n;
+  p.heads_total = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!x[i] || !out[i] || !aligned16(x[i]) || !aligned16(out[i])) return fail(CHITU_E_INVALID, "rotary: tensor %d null or not 16-byte aligned", i);
+    if (heads[i] < 1) return fail(CHITU_E_INVALID, "rotary: tensor %d has no heads", i);
+    if (!strides_fit(x_strides + 2 * i, tokens, heads[i], es) || !strides_fit(out_strides + 2 * i, tokens, heads[i], es))
+      return fail(CHITU_E_INVALID, "rotary: strides of tensor %d must be positive multiples of 16 bytes", i);
+    p.job[i] = {x[i], out[i], x_strides[2 * i], x_strides[2 * i + 1], out_strides[2 * i], out_strides[2 * i + 1], heads[i]};
+    p.heads_total += heads[i];
+  }
+  if (tokens == 0) return CHITU_OK;
+  p.positions = positions;
+  p.wide_positions = positions_are_int64;
+  p.table = reinterpret_cast<const float2*>(table);
+  p.table_rows = table_rows;
+  p.tokens = static_cast<int>(tokens);
+  p.head_dim = head_dim;
+  p.rot = rot;
+  const int per_block = chitu::kRotaryThreads / (head_dim / 16);
+  const int64_t blocks = (tokens + per_block - 1) / per_block;
+  // heads of one thread: as many as leave every SM eight blocks
+  const int64_t chunks = std::min<int64_t>(p.heads_total, std::max<int64_t>(1, (kSms * 8 + blocks - 1) / blocks));
+  p.heads_each = static_cast<int>((p.heads_total + chunks - 1) / chunks);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((p.heads_total + p.heads_each - 1) / p.heads_each));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define CHITU_ROTARY(DT) \
+  (interleaved ? chitu::rotary_kernel<DT, true><<<grid, chitu::kRotaryThreads, 0, st>>>(p) \
+               : chitu::rotary_kernel<DT, false><<<grid, chitu::kRotaryThreads, 0, st>>>(p))
+  if (dtype == CHITU_DTYPE_BF16)
+    CHITU_ROTARY(chitu::kBF16);
+  else if (dtype == CHITU_DTYPE_FP16)
+    CHITU_ROTARY(chitu::kFP16);
+  else
+    CHITU_ROTARY(chitu::kFP32);
+#undef CHITU_ROTARY
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "rotary: launch");
+}
+
+int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const void* v, const void* q,
+                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides, void* q_out,
+                         int q_heads, int64_t tokens, int dtype, int max_new, const void* positions, int positions_are_int64,
+                         const float* table, int64_t table_rows, int rot, int interleaved, void* stream) {
+  if (int rc = check_cache(cache, "kv_append")) return rc;
+  if (!k || !v || !k_strides || !v_strides) return fail(CHITU_E_INVALID, "kv_append: null pointer");
+  if (dtype != CHITU_DTYPE_BF16 && dtype != CHITU_DTYPE_FP16) return fail(CHITU_E_UNSUPPORTED, "kv_append: inputs must be bf16 or fp16");
+  if (tokens < 0 || tokens > 0x7fffffff) return fail(CHITU_E_INVALID, "kv_append: bad token count");
+  if (!aligned16(k) || !aligned16(v) || !strides_fit(k_strides, tokens, cache->heads, 2) || !strides_fit(v_strides, tokens, cache->heads, 2))
+    return fail(CHITU_E_INVALID, "kv_append: k and v must be 16-byte aligned, strides positive multiples of 8 elements");
+  if (q != nullptr) {
+    if (!q_strides || !q_out || q_heads < 1) return fail(CHITU_E_INVALID, "kv_append: q needs strides, heads and q_out");
+    if (!aligned16(q) || !aligned16(q_out) || !strides_fit(q_strides, tokens, q_heads, 2))
+      return fail(CHITU_E_INVALID, "kv_append: q must be 16-byte aligned, strides positive multiples of 8 elements");
+  }
+  if (table != nullptr) {
+    if (int rc = check_table(table, table_rows, rot, "kv_append")) return rc;
+    if (rot > 128) return fail(CHITU_E_INVALID, "kv_append: %d rotated channels of 128", rot);
+  }
+  if (tokens == 0 || cache->batch == 0) return CHITU_OK;
+  chitu::AppendParams p = {};
+  const void* src[3] = {k, v, q};
+  const int64_t* st3[3] = {k_strides, v_strides, q != nullptr ? q_strides : k_strides};
+  for (int i = 0; i < 3; ++i) {
+    p.src[i] = src[i];
+    p.src_token[i] = st3[i][0];
+    p.src_head[i] = st3[i][1];
+  }
+  const int es = cache->format == CHITU_CACHE_E4M3 ? 1 : 2;
+  p.cache[0] = cache->k;
+  p.cache[1] = cache->v;
+  p.scale[0] = cache->k_scale;
+  p.scale[1] = cache->v_scale;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* cs = i == 0 ? cache->k_strides : cache->v_strides;
+    const int64_t* ss = i == 0 ? cache->k_scale_strides : cache->v_scale_strides;
+    p.c_page[i] = cs[0] * es;
+    p.c_token[i] = cs[1] * es;
+    p.c_head[i] = cs[2] * es;
+    p.s_page[i] = ss[0];
+    p.s_head[i] = ss[1];
+  }
+  p.q_out = q_out;
+  p.block_table = cache->block_table;
+  p.table_stride = cache->table_stride;
+  p.lens = cache->lens;
+  p.cu = cache->cu_seqlens;
+  p.positions = positions;
+  p.wide_positions = positions_are_int64;
+  p.rope = reinterpret_cast<const float2*>(table);
+  p.rope_rows = table_rows;
+  p.rot = table != nullptr ? rot : 0;
+  p.interleaved = interleaved;
+  p.batch = cache->batch;
+  p.tokens = static_cast<int>(tokens);
+  p.width = cache->table_width;
+  p.n_pages = cache->n_pages;
+  p.heads_kv = cache->heads;
+  p.heads_q = q != nullptr ? q_heads : 0;
+  p.page = cache->page_size;
+  p.page_shift = page_shift_of(cache->page_size);
+  const int group = 4 * p.page;
+  p.heads_each = std::max(1, 256 / group);
+  const int expected = std::max<int>(1, static_cast<int>(std::min<int64_t>(max_new, tokens)));
+  p.slots = (expected + p.page - 2) / p.page + 1;
+  const int planes = 2 * p.heads_kv + p.heads_q;
+  const int64_t blocks = static_cast<int64_t>(p.batch) * p.slots;
+  const int64_t rows = (planes + p.heads_each - 1) / p.heads_each;
+  if (blocks > 0x7fffffff || rows > 65535) return fail(CHITU_E_UNSUPPORTED, "kv_append: too many pages or heads for one call");
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(rows));
+  const int threads = group * p.heads_each;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool fp16 = dtype == CHITU_DTYPE_FP16, eight = es == 1;
+  if (fp16 && eight)
+    chitu::kv_append_kernel<true, true><<<grid, threads, 0, st>>>(p);
+  else if (fp16)
+    chitu::kv_append_kernel<true, false><<<grid, threads, 0, st>>>(p);
+  else if (eight)
+    chitu::kv_append_kernel<false, true><<<grid, threads, 0, st>>>(p);
+  else
+    chitu::kv_append_kernel<false, false><<<grid, threads, 0, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "kv_append: launch");
+}
+
+int64_t chitu_b200_attn_cache_workspace_bytes(int batch, int64_t tokens, int heads, int q_heads, int format, int max_q,
+                                              int max_kv) {
+  (void)batch;
+  (void)tokens;
+  (void)heads;
+  (void)q_heads;
+  (void)format;
+  (void)max_q;
+  (void)max_kv;
+  return rows_workspace_bytes();
+}
+
+int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, const int64_t* q_strides, void* out, float* lse,
+                              int q_heads, int64_t tokens, float softmax_scale, int causal, int dtype, int max_q, int max_kv,
+                              void* workspace, int64_t workspace_bytes, int* status, void* stream) {
+  if (int rc = check_cache(cache, "attn_fwd_cache")) return rc;
+  if (!q || !q_strides || !out) return fail(CHITU_E_INVALID, "attn_fwd_cache: null pointer");
+  if (dtype != CHITU_DTYPE_BF16 && dtype != CHITU_DTYPE_FP16) return fail(CHITU_E_UNSUPPORTED, "attn_fwd_cache: q must be bf16 or fp16");
+  if (q_heads < 1 || q_heads % cache->heads != 0)
+    return fail(CHITU_E_INVALID, "attn_fwd_cache: %d query heads over %d key heads", q_heads, cache->heads);
+  if (tokens < 0 || tokens > 0x7fffffff / q_heads) return fail(CHITU_E_INVALID, "attn_fwd_cache: bad token count");
+  if (!(softmax_scale > 0.f) || softmax_scale > 1e30f) return fail(CHITU_E_INVALID, "attn_fwd_cache: softmax_scale must be positive and finite");
+  if (!aligned16(q) || !aligned16(out) || !strides_fit(q_strides, tokens, q_heads, 2))
+    return fail(CHITU_E_INVALID, "attn_fwd_cache: q and out must be 16-byte aligned, strides positive multiples of 8 elements");
+  if (tokens == 0 || cache->batch == 0) return CHITU_OK;
+  const int64_t need = chitu_b200_attn_cache_workspace_bytes(cache->batch, tokens, cache->heads, q_heads, cache->format, max_q, max_kv);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(CHITU_E_INVALID, "attn_fwd_cache: workspace must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));
+  chitu::CacheAttnParams p = {};
+  const int es = cache->format == CHITU_CACHE_E4M3 ? 1 : 2;
+  p.q = q;
+  p.q_token = q_strides[0];
+  p.q_head = q_strides[1];
+  p.out = out;
+  p.lse = lse;
+  p.cache[0] = static_cast<const uint8_t*>(cache->k);
+  p.cache[1] = static_cast<const uint8_t*>(cache->v);
+  p.scale[0] = cache->k_scale;
+  p.scale[1] = cache->v_scale;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* cs = i == 0 ? cache->k_strides : cache->v_strides;
+    const int64_t* ss = i == 0 ? cache->k_scale_strides : cache->v_scale_strides;
+    p.c_page[i] = cs[0] * es;
+    p.c_token[i] = cs[1] * es;
+    p.c_head[i] = cs[2] * es;
+    p.s_page[i] = ss[0];
+    p.s_head[i] = ss[1];
+  }
+  p.block_table = cache->block_table;
+  p.table_stride = cache->table_stride;
+  p.lens = cache->lens;
+  p.cu = cache->cu_seqlens;
+  p.status = status;
+  p.batch = cache->batch;
+  p.tokens = static_cast<int>(tokens);
+  p.width = cache->table_width;
+  p.n_pages = cache->n_pages;
+  p.heads_kv = cache->heads;
+  p.group = q_heads / cache->heads;
+  p.page_shift = page_shift_of(cache->page_size);
+  p.causal = causal;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.min_tiles = kRowsMinTiles;
+  p.count = static_cast<int*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeaderBytes);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool fp16 = dtype == CHITU_DTYPE_FP16, eight = es == 1;
+  cudaError_t e = fp16 ? (eight ? launch_rows<true, true>(p, st) : launch_rows<true, false>(p, st))
+                       : (eight ? launch_rows<false, true>(p, st) : launch_rows<false, false>(p, st));
+  return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "attn_fwd_cache: launch");
+}
+
+}  // extern "C"

@@ -115,7 +115,7 @@ __device__ __forceinline__ void block_sums(float (&s)[kRows], float (*red)[32], 
 // ----------------------------------------------------------------------------
 // LSE combine: one warp per (b, s, h) row of D values.
 // ----------------------------------------------------------------------------
-__global__ void __launch_bounds__(256)
+static __global__ void __launch_bounds__(256)
 lse_combine_kernel(float* __restrict__ acc_out, float* __restrict__ acc_lse, const void* __restrict__ blk_out,
                    const float* __restrict__ blk_lse, int B, int S, int H, int D, int blk_dtype, int first,
                    void* __restrict__ final_out, int final_dtype) {
@@ -582,7 +582,7 @@ qk_norm_rope_wide_kernel(const __grid_constant__ NormRopeBatch batch) {
 // ----------------------------------------------------------------------------
 // strided copy of 16-byte vectors: dst contiguous [n0, n1, n2, n3, row_vecs]
 // ----------------------------------------------------------------------------
-__global__ void __launch_bounds__(256)
+static __global__ void __launch_bounds__(256)
 strided_copy_kernel(const uint8_t* __restrict__ src, uint4* __restrict__ dst, long long n1, long long n2, long long n3,
                     long long row_vecs, long long st0, long long st1, long long st2, long long st3, long long total) {
   const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
@@ -610,7 +610,7 @@ struct ScatterRowsParams {
   long long dst_batch_bytes, dst_row_bytes;
 };
 
-__global__ void __launch_bounds__(256)
+static __global__ void __launch_bounds__(256)
 scatter_rows_kernel(const uint4* __restrict__ src, const ScatterRowsParams p) {
   const long long total = p.B * p.n_dest * p.rows * p.row_vecs;
   const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
@@ -640,7 +640,7 @@ struct PeerBarrierParams {
 // The epoch lives on the device (slot `world` of the local flag array) and advances by one per
 // barrier on every rank, so the kernel takes no per-call argument and can be replayed from a
 // CUDA graph.
-__global__ void peer_barrier_kernel(const PeerBarrierParams p) {
+static __global__ void peer_barrier_kernel(const PeerBarrierParams p) {
   const int i = threadIdx.x;
   int* counter = p.flags[p.rank] + p.world;
   const int epoch = *counter + 1;

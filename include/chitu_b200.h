@@ -44,6 +44,7 @@ int chitu_b200_version(void);
 #define CHITU_CAP_A2A_LAYOUT 16u
 #define CHITU_CAP_PEER_EXCHANGE 32u
 #define CHITU_CAP_ATTN_Q8 64u
+#define CHITU_CAP_KV_CACHE 128u
 unsigned chitu_b200_caps(void);
 const char* chitu_b200_last_error(void);
 
@@ -474,6 +475,84 @@ int chitu_b200_set_cluster_merge(int enable);
  * where events cannot be read back - it gives the per-launch timeline that bench.py reports.
  */
 int chitu_b200_stamp(unsigned long long* slot, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Paged key/value cache.  (No counterpart in the reference, whose K/V cache between steps is a list of gathered
+ * tensors, modules/attention/image_cp_attention.py:131-205.)
+ *
+ * A cache is a pool of pages of `page_size` tokens (16, 32, 64, 128 or 256) for keys and one for values, with any 16-byte
+ * aligned strides and the channels contiguous; block_table[b][i] names the page of tokens i * page_size ... of sequence b,
+ * and lens[b] counts the tokens that sequence b holds, those of the current call included.  A pool holds the inputs' 16-bit
+ * type, or e4m3 codes (CHITU_CACHE_E4M3) with one fp32 scale per page and head: value = code * scale.  Tokens of several
+ * sequences are packed: sequence b's are rows cu_seqlens[b] ... cu_seqlens[b + 1] - 1.  Rows behind the last sequence are
+ * left as they are.  lens, cu_seqlens and block_table are device memory and are not looked at by the host: page numbers
+ * outside [0, n_pages) are neither read nor written, lengths are cut to what the table can hold.
+ */
+#define CHITU_CACHE_16BIT 0
+#define CHITU_CACHE_E4M3 1
+
+typedef struct {
+  void* k;                 /* [n_pages, page_size, heads, 128] */
+  void* v;
+  float* k_scale;          /* [n_pages, heads], NULL for 16-bit pages */
+  float* v_scale;
+  int64_t k_strides[3];    /* page, token, head; in elements */
+  int64_t v_strides[3];
+  int64_t k_scale_strides[2]; /* page, head */
+  int64_t v_scale_strides[2];
+  const int* block_table;  /* [batch, table_width] */
+  const int* lens;         /* [batch] */
+  const int* cu_seqlens;   /* [batch + 1] */
+  int64_t table_stride;    /* entries from one sequence's row to the next */
+  int batch, table_width, n_pages, page_size, heads, format;
+} chitu_b200_kv_cache;
+
+/*
+ * Rotary embedding of up to three tensors of the same tokens (the q and k of a layer): x[i] is [tokens, heads[i], head_dim]
+ * with element strides x_strides[2 i] (token) and x_strides[2 i + 1] (head), channels contiguous, everything 16-byte
+ * aligned; out[i] likewise (out[i] == x[i] with the same strides: in place).  The first `rot` channels of a head turn by the
+ * factors of row positions[t] of `table` (fp32 (cos, sin) pairs [table_rows, rot / 2]), pairs are channels (2j, 2j + 1) where
+ * `interleaved`, else (j, j + rot / 2); other channels, and tokens whose position is outside the table, pass.  head_dim and
+ * rot are multiples of 16, head_dim at most 512.  The adjacent-pair form over whole heads with a norm before it is
+ * chitu_b200_qk_norm_rope.
+ */
+int chitu_b200_rotary(const void* const* x, void* const* out, const int64_t* x_strides, const int64_t* out_strides,
+                      const int* heads, int n, int64_t tokens, int head_dim, int rot, int dtype, const void* positions,
+                      int positions_are_int64, const float* table, int64_t table_rows, int interleaved, void* stream);
+
+/*
+ * Append the packed tokens' keys and values to the cache, rotating the keys and, where q is given, the queries on the way.
+ * Token i of sequence b takes position lens[b] - (tokens of b) + i, which also is its row of the rotary table unless
+ * `positions` (one entry per packed token) says otherwise; a NULL table stores keys as they come.  k, v, q are
+ * [tokens, heads, 128] with element strides (token, head); q_out is [tokens, q_heads, 128] contiguous.  max_new is how many
+ * tokens the longest sequence is expected to bring (it sizes the launch; longer ones are appended all the same).
+ *
+ * 8-bit pages: a page's scale is the smallest power of two that brings its values to at most 448; it grows when later tokens
+ * need it to (the codes that are there are brought to the new scale), and starts anew with the page's first token.
+ * No two sequences of a call may write to one page.
+ */
+int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const void* v, const void* q,
+                         const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides, void* q_out,
+                         int q_heads, int64_t tokens, int dtype, int max_new, const void* positions, int positions_are_int64,
+                         const float* table, int64_t table_rows, int rot, int interleaved, void* stream);
+
+/*
+ * Attention of packed queries over the cache: query i of sequence b attends to keys j < lens[b], with `causal` to
+ * j <= lens[b] - (tokens of b) + i.  q is [tokens, q_heads, 128] with element strides (token, head), q_heads a multiple of the
+ * cache's heads (query heads h * group ... share key head h); out is [tokens, q_heads, 128] contiguous, lse [q_heads, tokens]
+ * fp32 (natural log, scale included) or NULL.  A query that no key is visible to gives zeros and -inf.  Keys and values
+ * behind a sequence's length are never read; those within it have to be finite.  softmax_scale must be positive.
+ *
+ * max_q and max_kv are how many queries and keys the longest sequence is expected to have: they choose the kernel and the
+ * grid, and results are right whatever the lengths turn out to be.  workspace: chitu_b200_attn_cache_workspace_bytes(...) bytes,
+ * 16-byte aligned, its first CHITU_SPLITKV_HEADER_BYTES zero before the first call and left zero by each (rules as for
+ * chitu_b200_attn_fwd_splitkv, with which it may be shared).
+ */
+int64_t chitu_b200_attn_cache_workspace_bytes(int batch, int64_t tokens, int heads, int q_heads, int format, int max_q,
+                                              int max_kv);
+int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, const int64_t* q_strides, void* out, float* lse,
+                              int q_heads, int64_t tokens, float softmax_scale, int causal, int dtype, int max_q, int max_kv,
+                              void* workspace, int64_t workspace_bytes, int* status, void* stream);
 
 #ifdef __cplusplus
 }
