@@ -260,7 +260,7 @@ def load() -> ctypes.CDLL:
         _vp, ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp,
     ]
     lib.chitu_b200_attn_cache_workspace_bytes.restype = ctypes.c_int64
-    lib.chitu_b200_attn_cache_workspace_bytes.argtypes = [ctypes.c_int, ctypes.c_int64] + [ctypes.c_int] * 5
+    lib.chitu_b200_attn_cache_workspace_bytes.argtypes = [ctypes.c_int] * 3
     lib.chitu_b200_attn_fwd_cache.restype = ctypes.c_int
     lib.chitu_b200_attn_fwd_cache.argtypes = [
         ctypes.c_char_p, _vp, _i64p, _vp, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_int,

@@ -14,7 +14,7 @@
 // 2^-24 of its largest before fp16 drops any of their bits), which goes into the score's factor.
 #pragma once
 
-#include "attn_fwd.cuh"
+#include "attn_persist.cuh"
 #include "kv_cache.cuh"
 
 namespace chitu {
@@ -37,6 +37,8 @@ struct CacheAttnParams {
   float scale_log2;  // softmax_scale * log2(e)
   // work split over the grid (see each kernel) and scratch for pieces of a row's keys
   int min_tiles;
+  int tok_blk;        // tokens of a 256-row block (tile kernel)
+  int out_aligned32;
   int* count;
   float* part;
 };

@@ -1,0 +1,776 @@
+// Attention over a paged key/value cache for chunks of queries: 256-row query blocks on the tensor core (tcgen05, accumulators
+// in tensor memory).
+//
+// Query block: two tiles of 128 rows, row r = token r / group, query head r % group of the key head, so that heads which share
+// keys share a block.  Tensor bound; the layout is that of attn_persist_kernel - S | P0 | P1 | O0 | O1, one set of score
+// columns that leaves for registers at once, three issuing warps - with what a paged 8-bit cache adds:
+//
+//   warps 0-3 / 4-7  softmax of tile 0 / 1 (a thread is a row); they also bring the block's query rows to shared memory
+//   warps 8-11       widen e4m3 codes to fp16 in the swizzled layout of the matrix operands (16-bit pages: only clear the rows of
+//                    values behind the sequence's end)
+//   warps 12-14      issue QK^T, PV of tile 0, PV of tile 1
+//   warp  15         tensor copies of pages (a box is a page, or 128 rows of one; page numbers are the outermost coordinate, and
+//                    one outside the pool reads zeros) and the scales of a tile's sixteen-key groups
+//
+// Widening costs the SM sub-partitions' issue slots (about 100 instructions per warp and tile) rather than a pass over
+// memory: read back from a 16-bit copy of the cache, three frames over 21 would move 200 MB more.
+//
+// Work.  A block's share of the work is the keys it sees, K = the last row's, at least one.  All blocks in the order (sequence,
+// key head, block) are a line of such keys; CTA c takes the c-th of gridDim.x equal runs of it, and of a block those
+// 128-key tiles whose first key lies in its run.  So ragged lengths, causal blocks and few long blocks alike finish together.
+// A block that a run's border cuts leaves fp32 pieces in scratch; attn_cache_join_kernel, launched behind, merges them with all
+// SMs (the CTA that comes last would have up to 148 pieces of 128 KB to itself).
+#pragma once
+
+#include "attn_cache.cuh"
+
+namespace chitu {
+
+constexpr int kTileThreads = 512;
+constexpr int kTileRows = 2 * kTileM;    // rows of a block
+constexpr int kCoefStages = 8;           // tiles whose scales are kept: the copies run at most five ahead of the softmax
+template <bool kEightBit>
+struct TileShape {
+  static constexpr int slots = kEightBit ? 3 : 5;       // 16-bit operand tiles, keys and values in turn
+  static constexpr int raw_slots = kEightBit ? 4 : 5;   // as copied (16-bit pages are copied into their operand slot)
+  static constexpr int raw_bytes = kEightBit ? kTileBytes / 2 : 0;
+  static constexpr int coef_at = 2 * kTileBytes + slots * kTileBytes + raw_slots * raw_bytes;
+  static constexpr int bar_at = coef_at + kCoefStages * 8 * 16;
+  static constexpr int smem = bar_at + 512 + 1024;
+};
+// scratch of one piece: per tile [32 column groups][128 rows] float4, then (maximum, sum) of 128 rows
+constexpr int kTilePieceFloats = 2 * (32 * kTileM * 4 + 2 * kTileM);
+
+struct TileBlock {
+  int b, h, blk;       // sequence, key head, block
+  int n_blk;           // blocks of the sequence
+  int keys, n_tiles;   // K of the block
+  long long start;     // first key on the line
+  SeqInfo seq;
+};
+struct TileLine {
+  long long total, per;
+};
+
+// Blocks of a sequence hold whole tokens: tok_blk = 256 / group each.  The blocks' K are first + tok_blk, first + 2 tok_blk, ...,
+// all of the sequence's keys for the last one; where nothing is masked by position, or lengths do not fit (more queries than keys,
+// more keys than the table holds), it is all keys for every block.
+__device__ __forceinline__ bool tile_steps_grow(const CacheAttnParams& p, const SeqInfo& s) { return p.causal && s.first >= 0 && s.len == s.first + s.n_new; }
+__device__ __forceinline__ int tile_blocks(const CacheAttnParams& p, const SeqInfo& s) { return (s.n_new + p.tok_blk - 1) / p.tok_blk; }
+__device__ __forceinline__ int tile_keys(const CacheAttnParams& p, const SeqInfo& s, int blk) {
+  return max(tile_steps_grow(p, s) ? min(s.first + p.tok_blk * (blk + 1), s.len) : s.len, 1);
+}
+// keys of blocks [0, blk) of one head
+__device__ __forceinline__ long long tile_keys_before(const CacheAttnParams& p, const SeqInfo& s, int blk, int n_blk) {
+  if (!tile_steps_grow(p, s)) return static_cast<long long>(blk) * max(s.len, 1);
+  if (n_blk == 0) return 0;
+  const long long n = min(blk, n_blk - 1);  // (the last block ends with the sequence)
+  const long long sum = n * s.first + p.tok_blk * (n * (n + 1) / 2);
+  return blk == n_blk ? sum + s.len : sum;
+}
+__device__ __forceinline__ long long tile_keys_of(const CacheAttnParams& p, int b) {
+  const SeqInfo s = seq_info(p, b);
+  const int n_blk = tile_blocks(p, s);
+  return tile_keys_before(p, s, n_blk, n_blk) * p.heads_kv;
+}
+
+__device__ __forceinline__ void tile_measure(const CacheAttnParams& p, TileBlock& w) {
+  w.keys = tile_keys(p, w.seq, w.blk);
+  w.n_tiles = (w.keys + kTileN - 1) / kTileN;
+}
+__device__ __forceinline__ void tile_next_block(const CacheAttnParams& p, TileBlock& w) {
+  w.start += w.keys;
+  if (++w.blk == w.n_blk) {
+    w.blk = 0;
+    if (++w.h == p.heads_kv) {
+      w.h = 0;
+      while (++w.b < p.batch) {
+        w.seq = seq_info(p, w.b);
+        w.n_blk = tile_blocks(p, w.seq);
+        if (w.n_blk > 0) break;
+      }
+      if (w.b >= p.batch) return;
+    }
+  }
+  tile_measure(p, w);
+}
+
+// The line's length, by a whole warp.
+__device__ __forceinline__ TileLine tile_line(const CacheAttnParams& p, int lane, int ctas) {
+  TileLine line;
+  line.total = 0;
+  for (int b = lane; b < p.batch; b += 32) line.total += tile_keys_of(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) line.total += __shfl_xor_sync(0xffffffffu, line.total, o);
+  line.per = max((line.total + ctas - 1) / ctas, static_cast<long long>(p.min_tiles) * kTileN);
+  return line;
+}
+// The block that key `pos` of the line (< total) belongs to, by a whole warp.
+__device__ __forceinline__ TileBlock tile_locate(const CacheAttnParams& p, int lane, long long pos) {
+  TileBlock w;
+  long long at = 0;
+  for (w.b = 0;; w.b += 32) {
+    const int b = w.b + lane;
+    const long long mine = b < p.batch ? tile_keys_of(p, b) : 0;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, at + upto > pos);
+    if (past != 0) {
+      const int i = __ffs(past) - 1;
+      at += __shfl_sync(0xffffffffu, upto - mine, i);
+      w.b += i;
+      break;
+    }
+    at += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  w.seq = seq_info(p, w.b);
+  w.n_blk = tile_blocks(p, w.seq);
+  const long long per_head = tile_keys_before(p, w.seq, w.n_blk, w.n_blk);
+  w.h = static_cast<int>((pos - at) / per_head);
+  const long long in_head = pos - at - w.h * per_head;
+  int lo = 0, hi = w.n_blk - 1;  // the last block that starts at or before in_head
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tile_keys_before(p, w.seq, mid, w.n_blk) <= in_head)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  w.blk = lo;
+  w.start = at + w.h * per_head + tile_keys_before(p, w.seq, lo, w.n_blk);
+  tile_measure(p, w);
+  return w;
+}
+
+// A run's blocks one after the other, each with its tiles [t0, t0 + n).
+struct TileWalk {
+  TileBlock w;
+  long long pos, end;
+  bool begun;
+  __device__ __forceinline__ bool next(const CacheAttnParams& p, int& t0, int& n) {
+    while (true) {
+      if (begun) {
+        pos = w.start + w.keys;
+        if (pos >= end) return false;
+        tile_next_block(p, w);
+      }
+      begun = true;
+      t0 = static_cast<int>((pos - w.start + kTileN - 1) / kTileN);
+      const long long upto = min(end - w.start, static_cast<long long>(w.keys));
+      n = (upto == w.keys ? w.n_tiles : static_cast<int>((upto + kTileN - 1) / kTileN)) - t0;
+      if (n > 0) return true;
+    }
+  }
+  __device__ __forceinline__ int rows(const CacheAttnParams& p) const { return min(p.tok_blk, w.seq.n_new - w.blk * p.tok_blk) * p.group; }
+};
+
+__device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// One softmax step (thread = one row, 128 scores): scores in, probabilities out.  As persist_softmax_step, with a factor and an
+// addend for each sixteen keys (coef: key scale, log2 of the value scale, its inverse) and `valid` keys visible to this row.
+// m is the largest (score factor + addend) so far in log2 units, moved only when it has grown by more than 2^8.
+template <bool kHalf>
+__device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, bool first, int valid, float row_factor, const float4* coef,
+                                                  float& m, float& l_sum, volatile int* abort_flag, int* status) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld32(r.t_s + c * 32, s[c]);
+  tmem_wait_ld();
+  tc_fence_before_sync();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(r.bar_s_empty);
+  if (__any_sync(0xffffffffu, valid < kTileN)) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+      if (i >= valid) s[i >> 5][i & 31] = 0xff800000u;  // -inf
+  }
+  float mx = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const uint32_t* x = &s[c >> 1][(c & 1) * 16];
+    float a = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+    float b = max3(__uint_as_float(x[3]), __uint_as_float(x[4]), __uint_as_float(x[5]));
+    a = max3(a, __uint_as_float(x[6]), __uint_as_float(x[7]));
+    b = max3(b, __uint_as_float(x[8]), __uint_as_float(x[9]));
+    a = max3(a, __uint_as_float(x[10]), __uint_as_float(x[11]));
+    b = max3(b, __uint_as_float(x[12]), __uint_as_float(x[13]));
+    a = max3(a, __uint_as_float(x[14]), __uint_as_float(x[15]));
+    const float4 k = coef[c];
+    mx = fmaxf(mx, fmaf(fmaxf(a, b), row_factor * k.x, k.y));
+  }
+  if (first) {
+    m = mx;
+  } else {
+    const bool need = mx > m + kRescaleThreshold;
+    if (__any_sync(0xffffffffu, need)) {
+      mbar_wait(r.bar_pv, (step - 1) & 1, abort_flag, status, kDevTimeoutSoftmax);
+      __syncwarp();
+      tc_fence_after_sync();
+      const float f = need ? fast_exp2(m - mx) : 1.0f;
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        uint32_t o[16];
+        tmem_ld16(r.t_o + c * 16, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tmem_st16(r.t_o + c * 16, o);
+      }
+      l_sum *= f;
+      if (need) m = mx;
+    }
+  }
+  // (looked at early, so that the answer is there when the first probabilities are stored)
+  const bool pv_done = step == 0 || mbar_try_wait(r.bar_pv, (step - 1) & 1);
+  const float shift = m == -INFINITY ? 0.f : kProbShift - m;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t pk[32];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = half * 4 + q;
+      const float4 k = coef[c];
+      const float f = row_factor * k.x, add = k.y + shift;
+      const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
+      const uint32_t* x = &s[c >> 1][(c & 1) * 16];
+      float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        float2 x0 = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), f2, add2);
+        float2 x1 = __ffma2_rn(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), f2, add2);
+        x0.x = fast_exp2(x0.x);
+        x0.y = fast_exp2(x0.y);
+        x1.x = fast_exp2(x1.x);
+        x1.y = fast_exp2(x1.y);
+        la = __fadd2_rn(la, x0);
+        lb = __fadd2_rn(lb, x1);
+        pk[q * 8 + (i >> 1)] = pack2<kHalf>(x0.x, x0.y);
+        pk[q * 8 + (i >> 1) + 1] = pack2<kHalf>(x1.x, x1.y);
+      }
+      la = __fadd2_rn(la, lb);
+      l_sum = fmaf(la.x + la.y, k.z, l_sum);
+    }
+    // 64 probabilities done: hand this half to the issuing warp
+    if (half == 0) {
+      if (!pv_done) mbar_wait(r.bar_pv, (step - 1) & 1, abort_flag, status, kDevTimeoutSoftmax);
+      __syncwarp();  // (lanes may have found out on their own; the store below is the warp's)
+      tc_fence_after_sync();
+    }
+    tmem_st32(r.t_p + half * 32, pk);
+    tmem_wait_st();
+    tc_fence_before_sync();
+    mbar_arrive(r.bar_p + 8 * half);
+  }
+}
+
+template <bool kFp16, bool kEightBit>
+__global__ void __launch_bounds__(kTileThreads, 1)
+attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CacheAttnParams p) {
+  using Shape = TileShape<kEightBit>;
+  constexpr int kSlots = Shape::slots, kRaw = Shape::raw_slots;
+  constexpr bool kHalf = kEightBit || kFp16;  // fp16 products
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t q_smem = smem_base;                      // 2 tiles
+  const uint32_t kv_smem = smem_base + 2 * kTileBytes;    // kSlots operand tiles
+  const uint32_t raw_smem = kv_smem + kSlots * kTileBytes;
+  float4* coef_ring = reinterpret_cast<float4*>(smem_gen + Shape::coef_at);
+  uint8_t* ctl = smem_gen + Shape::bar_at;
+  const uint32_t bars = smem_u32(ctl);
+  const uint32_t bar_raw_full = bars;                     // [kRaw] copies have landed
+  const uint32_t bar_raw_empty = bar_raw_full + 8 * 5;    // [kRaw] codes have been widened (8-bit pages)
+  const uint32_t bar_kv_full = bar_raw_empty + 8 * 5;     // [kSlots]
+  const uint32_t bar_kv_empty = bar_kv_full + 8 * 5;      // [kSlots]
+  const uint32_t bar_coef = bar_kv_empty + 8 * 5;         // [kCoefStages]
+  const uint32_t bar_q_ready = bar_coef + 8 * kCoefStages;  // [2]
+  const uint32_t bar_s_full = bar_q_ready + 16;           // [2]
+  const uint32_t bar_p_full = bar_s_full + 16;            // [2][2]
+  const uint32_t bar_pv = bar_p_full + 32;                // [2]
+  const uint32_t bar_s_empty = bar_pv + 16;
+  const uint32_t bar_drain = bar_s_empty + 8;             // [3]
+  int* raw_rows = reinterpret_cast<int*>(ctl + 400);      // [kRaw] rows of the copy that exist, -1: no more
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 424);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctl + 428);
+  long long* run = reinterpret_cast<long long*>(ctl + 432);  // first key, end, block start, b | h, blk
+  static_assert(8 * (20 + kCoefStages) + 16 + 16 + 32 + 16 + 8 + 24 <= 400 && kRaw <= 5 && kSlots <= 5, "control block");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    const TileLine line = tile_line(p, lane, gridDim.x);
+    const long long lo = blockIdx.x * line.per, hi = min(lo + line.per, line.total);
+    TileBlock w = {};
+    if (lo < hi) w = tile_locate(p, lane, lo);
+    if (lane == 0) {
+      run[0] = lo;
+      run[1] = hi;
+      run[2] = w.start;
+      run[3] = w.b;
+      run[4] = w.h;
+      run[5] = w.blk;
+    }
+  } else if (threadIdx.x == 32) {
+    *abort_flag = 0;
+    for (int s = 0; s < kRaw; ++s) {
+      mbar_init(bar_raw_full + 8 * s, 1);
+      mbar_init(bar_raw_empty + 8 * s, 4);
+    }
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(bar_kv_full + 8 * s, 4);
+      mbar_init(bar_kv_empty + 8 * s, 2);
+    }
+    for (int s = 0; s < kCoefStages; ++s) mbar_init(bar_coef + 8 * s, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar_q_ready + 8 * t, kTileM);
+      mbar_init(bar_s_full + 8 * t, 1);
+      mbar_init(bar_p_full + 16 * t, kTileM);
+      mbar_init(bar_p_full + 16 * t + 8, kTileM);
+      mbar_init(bar_pv + 8 * t, 1);
+    }
+    mbar_init(bar_s_empty, 4);
+    for (int i = 0; i < 3; ++i) mbar_init(bar_drain + 8 * i, 1);
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  if (warp == 15 && lane == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  TileWalk walk;
+  walk.pos = run[0];
+  walk.end = run[1];
+  const bool busy = walk.pos < walk.end;  // (else the line is shorter than the grid)
+  walk.begun = false;
+  walk.w.start = run[2];
+  walk.w.b = static_cast<int>(run[3]);
+  walk.w.h = static_cast<int>(run[4]);
+  walk.w.blk = static_cast<int>(run[5]);
+  if (busy) {
+    walk.w.seq = seq_info(p, walk.w.b);
+    walk.w.n_blk = tile_blocks(p, walk.w.seq);
+    tile_measure(p, walk.w);
+  }
+
+  int t0, n;
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 15) {
+      // ---------------------------------------------------------------- copies of pages, scales
+      const int box_shift = min(p.page_shift, 7);
+      const int boxes = kTileN >> box_shift;
+      int slot = 0, phase = 0, tiles = 0;  // ring position, tiles so far
+      bool given_up = false;
+      auto page_of = [&](int tile) {  // lane l < boxes: the page of the tile's l-th box, -1 where there is none
+        const int key = tile * kTileN + (lane << box_shift);
+        if (lane >= boxes || key >= walk.w.seq.len) return -1;
+        const int id = __ldg(p.block_table + walk.w.b * p.table_stride + (key >> p.page_shift));
+        return id >= 0 && id < p.n_pages ? id : -1;
+      };
+      while (busy && !given_up && walk.next(p, t0, n)) {
+        int page = page_of(t0);
+        for (int j = 0; j < n && !given_up; ++j, ++tiles) {
+          const int tile = t0 + j;
+          const int next_page = j + 1 < n ? page_of(tile + 1) : -1;
+          // scales of the tile's sixteen-key groups (the entry's last reader is eight tiles back)
+          {
+            const int from = __shfl_sync(0xffffffffu, page, (lane * 16 >> box_shift) & 31);
+            if (lane < 8) {
+              float4 k = make_float4(1.f, from < 0 ? -INFINITY : 0.f, 1.f, 0.f);
+              if (kEightBit && from >= 0) {
+                const float ks = __ldg(p.scale[0] + from * p.s_page[0] + walk.w.h * p.s_head[0]);
+                const float vs = fmaxf(__ldg(p.scale[1] + from * p.s_page[1] + walk.w.h * p.s_head[1]), kMinValueScale);
+                k = make_float4(fmaxf(ks, 1e-30f), __log2f(vs), __fdividef(1.f, vs), 0.f);
+              }
+              coef_ring[(tiles % kCoefStages) * 8 + lane] = k;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_coef + 8 * (tiles % kCoefStages));
+          }
+          for (int kv = 0; kv < 2; ++kv) {
+            const bool ok = mbar_wait((kEightBit ? bar_raw_empty : bar_kv_empty) + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutLoad);
+            given_up = given_up || !__all_sync(0xffffffffu, ok);
+            const uint32_t bar = bar_raw_full + 8 * slot;
+            if (lane == 0) {
+              raw_rows[slot] = min(walk.w.seq.len - tile * kTileN, kTileN);
+              mbar_arrive_expect_tx(bar, kEightBit ? kTileBytes / 2 : kTileBytes);
+            }
+            __syncwarp();
+            if (lane < boxes) {
+              const CUtensorMap* tm = kv ? &tm_v : &tm_k;
+              const int token = (tile * kTileN + (lane << box_shift)) & ((1 << p.page_shift) - 1);
+              const uint32_t at = (lane << box_shift) * 128;
+              if constexpr (kEightBit) {
+                tma_load_4d(raw_smem + slot * Shape::raw_bytes + at, tm, bar, 0, walk.w.h, token, page);
+              } else {
+                tma_load_4d(kv_smem + slot * kTileBytes + at, tm, bar, 0, walk.w.h, token, page);
+                tma_load_4d(kv_smem + slot * kTileBytes + kHalfTileBytes + at, tm, bar, 64, walk.w.h, token, page);
+              }
+            }
+            __syncwarp();
+            if (++slot == kRaw) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
+          page = next_page;
+        }
+      }
+      // no more: the widening warps go home
+      mbar_wait((kEightBit ? bar_raw_empty : bar_kv_empty) + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutLoad);
+      if (lane == 0) {
+        raw_rows[slot] = -1;
+        mbar_arrive(bar_raw_full + 8 * slot);
+        // Should a role have given up, nothing of ours may still be landing when the CTA retires (bounded polls on the last
+        // copy into every slot, this one's arrival among them; a slot that was never filled counts as complete in its phase before the first).
+        for (int i = 0; i < kRaw; ++i)
+          for (int spin = 0; spin < (1 << 20) && !mbar_try_wait(bar_raw_full + 8 * i, i <= slot ? phase : phase ^ 1); ++spin) {
+          }
+      }
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------------------- matrix issuers
+      const bool leader = elect_one();
+      const int role = warp - 12;  // 0 scores; 1, 2 PV of tile 0, 1
+      int slot = 0, phase = 0;     // the next key (role 0) or value tile
+      auto advance = [&] {
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      if (role > 0) advance();
+      if (role == 0) {
+        constexpr uint32_t kIdescQK = umma_idesc(1, kHalf ? 0 : 1, kHalf ? 0 : 1, 0, kTileM, kTileN);
+        const uint64_t q_desc0 = umma_smem_desc_sw128(q_smem, 16, 1024);
+        const uint64_t k_desc0 = umma_smem_desc_sw128(kv_smem, 16, 1024);
+        int q_uses[2] = {0, 0}, scores = 0;
+        while (busy && walk.next(p, t0, n)) {
+          const int n_qt = walk.rows(p) > kTileM ? 2 : 1;
+          for (int j = 0; j < n; ++j) {
+            mbar_wait(bar_kv_full + 8 * slot, phase, abort_flag, p.status, kDevTimeoutMma);
+            for (int t = 0; t < n_qt; ++t) {
+              if (j == 0) {
+                mbar_wait(bar_q_ready + 8 * t, q_uses[t] & 1, abort_flag, p.status, kDevTimeoutMma);
+                ++q_uses[t];
+              }
+              // the columns of the scores are free once the softmax warps have the previous ones in registers
+              if (scores > 0) mbar_wait(bar_s_empty, (scores - 1) & 1, abort_flag, p.status, kDevTimeoutMma);
+              ++scores;
+              __syncwarp();
+              tc_fence_after_sync();
+              if (leader) {
+                const uint64_t a0 = q_desc0 + static_cast<uint64_t>((t * kTileBytes) >> 4);
+                const uint64_t b0 = k_desc0 + static_cast<uint64_t>((slot * kTileBytes) >> 4);
+#pragma unroll
+                for (int k = 0; k < kHeadDim / 16; ++k) {
+                  const uint64_t off = static_cast<uint64_t>(((k >> 2) * kHalfTileBytes + (k & 3) * 32) >> 4);
+                  umma_ss_f16(tmem_base, a0 + off, b0 + off, kIdescQK, k > 0);
+                }
+                umma_commit(bar_s_full + 8 * t);
+              }
+              __syncwarp();
+            }
+            if (leader) {  // (a slot is released by two arrivals: values have two readers)
+              umma_commit(bar_kv_empty + 8 * slot);
+              umma_commit(bar_kv_empty + 8 * slot);
+            }
+            __syncwarp();
+            advance();
+            advance();
+          }
+        }
+      } else {
+        constexpr uint32_t kIdescPV = umma_idesc(1, kHalf ? 0 : 1, kHalf ? 0 : 1, 1, kTileM, kHeadDim);
+        const int t = role - 1;
+        const uint64_t v_desc0 = umma_smem_desc_sw128(kv_smem, kHalfTileBytes, 1024);
+        const uint32_t t_p = tmem_base + kTileN + t * 64;
+        const uint32_t t_o = tmem_base + 2 * kTileN + t * kHeadDim;
+        int steps = 0;  // the tile's steps so far
+        while (busy && walk.next(p, t0, n)) {
+          const int n_qt = walk.rows(p) > kTileM ? 2 : 1;
+          for (int j = 0; j < n; ++j) {
+            mbar_wait(bar_kv_full + 8 * slot, phase, abort_flag, p.status, kDevTimeoutMma);
+            if (t < n_qt) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                mbar_wait(bar_p_full + 16 * t + 8 * h, steps & 1, abort_flag, p.status, kDevTimeoutMma);
+                __syncwarp();
+                tc_fence_after_sync();
+                if (leader) {
+                  const uint64_t b0 = v_desc0 + static_cast<uint64_t>((slot * kTileBytes + h * 8192) >> 4);
+#pragma unroll
+                  for (int k = 0; k < 4; ++k)
+                    umma_ts_f16(t_o, t_p + h * 32 + k * 8, b0 + static_cast<uint64_t>((k * 2048) >> 4), kIdescPV, (h > 0 || k > 0 || j > 0) ? 1u : 0u);
+                  if (h == 1) umma_commit(bar_pv + 8 * t);
+                }
+                __syncwarp();
+              }
+              ++steps;
+            }
+            if (leader) umma_commit(bar_kv_empty + 8 * slot);
+            __syncwarp();
+            advance();
+            advance();
+          }
+        }
+      }
+      // One more commit and a bounded poll on it: every arrival of this warp's commits has landed, and nothing writes tensor
+      // memory after it has been freed below.
+      if (leader) umma_commit(bar_drain + 8 * role);
+      __syncwarp();
+      for (int spin = 0; spin < (1 << 20) && !mbar_try_wait(bar_drain + 8 * role, 0); ++spin) {
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------------ codes to operands
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const int tid = threadIdx.x - 256;
+    int slot = 0, phase = 0, raw = 0, raw_phase = 0;
+    bool values = false;
+    while (true) {
+      bool ok = mbar_wait(bar_raw_full + 8 * raw, raw_phase, abort_flag, p.status, kDevTimeoutMma);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int rows = reinterpret_cast<volatile int*>(raw_rows)[raw];
+      if (rows < 0) break;
+      if constexpr (kEightBit) {
+        ok = mbar_wait(bar_kv_empty + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutMma);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        // thread: channels 16 c .. 16 c + 15 of rows r, r + 16, ...; two 16-byte pieces of a swizzled row, the second panel's
+        // threads in the other order (a quarter warp then covers all banks)
+        const int c = tid & 7, r = tid >> 3;
+        const uint32_t from = raw_smem + raw * Shape::raw_bytes + r * 128 + c * 16;
+        const uint32_t to = kv_smem + slot * kTileBytes + (c >> 2) * kHalfTileBytes + r * 128;
+        const int sw = r & 7, first = c >> 2;
+        const uint32_t at0 = to + ((((c & 3) * 2 + first) ^ sw) << 4), at1 = to + ((((c & 3) * 2 + 1 - first) ^ sw) << 4);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint4 w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = ld_shared16(from + (half * 4 + i) * 2048);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (values && r + (half * 4 + i) * 16 >= rows) w[i] = make_uint4(0, 0, 0, 0);
+            const uint32_t a0 = first ? w[i].z : w[i].x, a1 = first ? w[i].w : w[i].y;
+            const uint32_t b0 = first ? w[i].x : w[i].z, b1 = first ? w[i].y : w[i].w;
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at0 + (half * 4 + i) * 2048), "r"(widen_e4m3x2(a0)),
+                         "r"(widen_e4m3x2(a0 >> 16)), "r"(widen_e4m3x2(a1)), "r"(widen_e4m3x2(a1 >> 16))
+                         : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at1 + (half * 4 + i) * 2048), "r"(widen_e4m3x2(b0)),
+                         "r"(widen_e4m3x2(b0 >> 16)), "r"(widen_e4m3x2(b1)), "r"(widen_e4m3x2(b1 >> 16))
+                         : "memory");
+          }
+        }
+      } else if (values && rows < kTileN) {
+        // what the page holds behind the sequence's end may be anything: no weight is not enough
+        const uint32_t to = kv_smem + raw * kTileBytes + tid * 128;
+        if (tid >= rows) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(to + i * 16), "r"(0) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(to + kHalfTileBytes + i * 16), "r"(0) : "memory");
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (kEightBit) mbar_arrive(bar_raw_empty + 8 * raw);
+        mbar_arrive(bar_kv_full + 8 * (kEightBit ? slot : raw));
+      }
+      values = !values;
+      if (++slot == kSlots) {
+        slot = 0;
+        phase ^= 1;
+      }
+      if (++raw == kRaw) {
+        raw = 0;
+        raw_phase ^= 1;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax, queries in, results out
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    const int t = warp >> 2, quad = warp & 3;
+    const int row_in_tile = quad * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t t_o = tmem_base + lane_base + 2 * kTileN + t * kHeadDim;
+    const TileRefs refs{tmem_base + lane_base, tmem_base + lane_base + kTileN + t * 64, t_o, bar_s_empty, bar_p_full + 16 * t, bar_pv + 8 * t};
+    uint8_t* q_row = smem_gen + t * kTileBytes + row_in_tile * 128;
+    int steps = 0, tiles = 0;  // this tile's steps, the CTA's key tiles so far
+    while (busy && walk.next(p, t0, n)) {
+      const TileBlock& w = walk.w;
+      if (t * kTileM >= walk.rows(p)) {
+        tiles += n;
+        continue;
+      }
+      const int r = t * kTileM + row_in_tile;
+      const int in_blk = r / p.group;
+      const int tok = w.blk * p.tok_blk + in_blk, hq = w.h * p.group + r - in_blk * p.group;
+      const bool live = in_blk < p.tok_blk && tok < w.seq.n_new;
+      // the row to shared memory: the last QK^T that read this tile's rows is complete (its scores have been waited for)
+      float row_factor = p.scale_log2;
+      {
+        uint4 v[16];
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (w.seq.tok0 + tok) * p.q_token + hq * p.q_head);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+        if constexpr (kEightBit && !kFp16) {
+          uint32_t* x = reinterpret_cast<uint32_t*>(v);
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[i] << 16)), fabsf(__uint_as_float(x[i] & 0xffff0000u))));
+          const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253);
+          const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          row_factor *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) x[i] = pack2<true>(__uint_as_float(x[i] << 16) * down, __uint_as_float(x[i] & 0xffff0000u) * down);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(q_row + (i >> 3) * kHalfTileBytes + (((i & 7) ^ (row_in_tile & 7)) << 4)) = v[i];
+        fence_proxy_async_smem();
+        mbar_arrive(bar_q_ready + 8 * t);
+      }
+      const int limit = live && p.causal ? min(w.seq.first + tok + 1, w.seq.len) : w.seq.len;
+      float m = -INFINITY, l_sum = 0.f;
+      for (int j = 0; j < n; ++j, ++steps, ++tiles) {
+        mbar_wait(bar_s_full + 8 * t, steps & 1, abort_flag, p.status, kDevTimeoutSoftmax);
+        // (complete by now, and only now its own phase: warps without rows in a block run ahead of the copies)
+        mbar_wait(bar_coef + 8 * (tiles % kCoefStages), (tiles / kCoefStages) & 1, abort_flag, p.status, kDevTimeoutSoftmax);
+        __syncwarp();
+        tc_fence_after_sync();
+        tile_softmax_step<kHalf>(refs, steps, j == 0, limit - (t0 + j) * kTileN, row_factor, coef_ring + (tiles % kCoefStages) * 8, m, l_sum,
+                                 abort_flag, p.status);
+      }
+      mbar_wait(bar_pv + 8 * t, (steps - 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
+      __syncwarp();
+      tc_fence_after_sync();
+      if (n == w.n_tiles) {
+        const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+        const size_t row = static_cast<size_t>(w.seq.tok0 + tok);
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t v[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = pack2<kFp16>(__uint_as_float(o[16 * h + 2 * i]) * inv, __uint_as_float(o[16 * h + 2 * i + 1]) * inv);
+              if (p.out_aligned32) {
+                st_global32(dst + c * 32 + h * 16, v);
+              } else {
+                uint4* d = reinterpret_cast<uint4*>(dst + c * 32 + h * 16);
+                d[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                d[1] = make_uint4(v[4], v[5], v[6], v[7]);
+              }
+            }
+          }
+          __syncwarp();
+        }
+        if (live && p.lse != nullptr)
+          p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_sum > 0.f ? (m - kProbShift + log2f(l_sum)) * 0.6931471805599453f : -INFINITY;
+      } else {
+        // a piece: rows as they are, the maximum and the sum with them
+        float* piece = p.part + (2 * static_cast<long long>(blockIdx.x) + (w.start > run[0] ? 1 : 0)) * kTilePieceFloats + t * (kTilePieceFloats / 2);
+        float4* mine = reinterpret_cast<float4*>(piece) + row_in_tile;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            mine[(c * 8 + (i >> 2)) * kTileM] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+        }
+        reinterpret_cast<float2*>(piece + 32 * kTileM * 4)[row_in_tile] = make_float2(m, l_sum);
+      }
+      tc_fence_before_sync();
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Merges the pieces of the blocks that runs' borders have cut: blockIdx.x is the run in which a block begins (at most one block
+// begins in a run and ends behind it), blockIdx.y a group of 32 rows.  Eight warps, 16 channels each; a lane is a row.
+template <bool kFp16>
+__global__ void __launch_bounds__(256)
+attn_cache_join_kernel(const __grid_constant__ CacheAttnParams p, int ctas) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TileLine line = tile_line(p, lane, ctas);
+  const long long lo = blockIdx.x * line.per, border = lo + line.per;
+  if (border >= line.total) return;
+  const TileBlock w = tile_locate(p, lane, border - 1);
+  const long long last_tile = w.start + static_cast<long long>(w.n_tiles - 1) * kTileN;
+  if (w.start < lo || last_tile < border) return;
+  const int n_pieces = static_cast<int>(last_tile / line.per - blockIdx.x) + 1;
+  const int r = blockIdx.y * 32 + lane;
+  const int in_blk = r / p.group;
+  const int tok = w.blk * p.tok_blk + in_blk, hq = w.h * p.group + r - in_blk * p.group;
+  const bool live = in_blk < p.tok_blk && tok < w.seq.n_new;
+  if (!__any_sync(0xffffffffu, live)) return;
+  const int t = r >> 7, row_in_tile = r & 127;
+  auto piece = [&](int i) {  // the first may begin inside its run, the others begin theirs
+    return p.part + (2 * static_cast<long long>(blockIdx.x + i) + (i == 0 && w.start > lo ? 1 : 0)) * kTilePieceFloats + t * (kTilePieceFloats / 2);
+  };
+  float m = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+  for (int i = 0; i < n_pieces; ++i) {
+    const float* from = piece(i);
+    const float2 st = __ldcg(reinterpret_cast<const float2*>(from + 32 * kTileM * 4) + row_in_tile);
+    const float4* src = reinterpret_cast<const float4*>(from) + warp * 4 * kTileM + row_in_tile;
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __ldcg(src + j * kTileM);
+    const float top = fmaxf(m, st.x);
+    const float mine = m == -INFINITY ? 0.f : fast_exp2(m - top), theirs = st.x == -INFINITY ? 0.f : fast_exp2(st.x - top);
+    m = top;
+    l = l * mine + st.y * theirs;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[4 * j] = o[4 * j] * mine + v[j].x * theirs;
+      o[4 * j + 1] = o[4 * j + 1] * mine + v[j].y * theirs;
+      o[4 * j + 2] = o[4 * j + 2] * mine + v[j].z * theirs;
+      o[4 * j + 3] = o[4 * j + 3] * mine + v[j].w * theirs;
+    }
+  }
+  if (!live) return;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const size_t row = static_cast<size_t>(w.seq.tok0 + tok);
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128 + warp * 16;
+  uint32_t v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = pack2<kFp16>(o[2 * i] * inv, o[2 * i + 1] * inv);
+  uint4* d = reinterpret_cast<uint4*>(dst);
+  d[0] = make_uint4(v[0], v[1], v[2], v[3]);
+  d[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  if (warp == 0 && p.lse != nullptr)
+    p.lse[static_cast<size_t>(hq) * p.tokens + row] = l > 0.f ? (m - kProbShift + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+}  // namespace chitu

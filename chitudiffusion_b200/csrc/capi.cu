@@ -36,12 +36,7 @@ int chitu::cuda_fail(cudaError_t e, const char* what) {
   return fail(CHITU_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-namespace {
-
-using chitu::cuda_fail;
-using chitu::fail;
-
-PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 chitu::get_encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -54,6 +49,12 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
   });
   return fn;
 }
+
+namespace {
+
+using chitu::cuda_fail;
+using chitu::fail;
+using chitu::get_encode_fn;
 
 // Tensor map over a [B, S, H, 128] 16-bit tensor with element strides {b, s, h, 1}:
 // dims (innermost first) d, h, s, b; box = 64 x 1 x 128 x 1 with 128-byte swizzle,

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "attn_cache.cuh"
+#include "attn_cache_tile.cuh"
 
 namespace {
 
@@ -71,18 +72,60 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices]) {
 
 constexpr int kSms = 148;
 
-// Grid of the rows kernel: all CTAs resident at once (two per SM).
+// Grid of the rows kernel: all CTAs resident at once (two per SM), or as many as there can be runs of kRowsMinTiles tiles.
 constexpr int kRowsGrid = kSms * 2;
 constexpr int kRowsMinTiles = 2;
 int64_t rows_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kRowsGrid) * 2 * chitu::kRowsPieceFloats * 4; }
 
 template <bool kFp16, bool kEightBit>
-cudaError_t launch_rows(const chitu::CacheAttnParams& p, cudaStream_t st) {
+cudaError_t launch_rows(const chitu::CacheAttnParams& p, int max_q, int max_kv, cudaStream_t st) {
   static bool done[kMaxDevices] = {};
   constexpr int smem = chitu::RowsShape<kEightBit>::smem;
   cudaError_t e = allow_smem(chitu::attn_cache_rows_kernel<kFp16, kEightBit>, smem, done);
   if (e != cudaSuccess) return e;
-  chitu::attn_cache_rows_kernel<kFp16, kEightBit><<<kRowsGrid, chitu::kRowsThreads, smem, st>>>(p);
+  const int64_t items = static_cast<int64_t>(p.batch) * p.heads_kv * ((static_cast<int64_t>(max_q) * p.group + 15) / 16);
+  const int64_t runs = (items * ((max_kv + chitu::kRowsTile - 1) / chitu::kRowsTile) + kRowsMinTiles - 1) / kRowsMinTiles;
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowsGrid, runs)));
+  chitu::attn_cache_rows_kernel<kFp16, kEightBit><<<grid, chitu::kRowsThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+// Tensor map over a pool: channels, heads, tokens of a page, pages; a box is 128 bytes of the channels by a page's tokens, 128 of
+// them at most.  16-bit pages land in the swizzled layout of the matrix operands, codes as they are.
+int make_cache_map(CUtensorMap* map, const chitu_b200_kv_cache* c, const void* base, const int64_t* st, const char* name) {
+  auto encode = chitu::get_encode_fn();
+  if (!encode) return fail(CHITU_E_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  const bool eight = c->format == CHITU_CACHE_E4M3;
+  const int es = eight ? 1 : 2;
+  // (a dimension of extent 1 never advances; give it any legal stride)
+  auto bytes = [&](int i, int64_t extent) { return extent == 1 ? cuuint64_t{256} : static_cast<cuuint64_t>(st[i]) * es; };
+  cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(c->heads), static_cast<cuuint64_t>(c->page_size), static_cast<cuuint64_t>(c->n_pages)};
+  cuuint64_t strides[3] = {bytes(2, c->heads), bytes(1, c->page_size), bytes(0, c->n_pages)};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), 1, static_cast<cuuint32_t>(std::min(c->page_size, 128)), 1};
+  cuuint32_t elem[4] = {1, 1, 1, 1};
+  CUresult r = encode(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+                      elem, CU_TENSOR_MAP_INTERLEAVE_NONE, eight ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(CHITU_E_CUDA, "%s: cuTensorMapEncodeTiled failed with CUresult %d", name, static_cast<int>(r));
+  return CHITU_OK;
+}
+
+// Which kernel a call takes.  Up to 16 query rows of a key head (tokens x heads that share it) are one tile of the rows kernel;
+// more would have it read the cache once per 16 rows.
+bool takes_tile_kernel(int max_q, int group) { return static_cast<int64_t>(max_q) * group > 16 && group <= 128; }
+constexpr int kTileMinTiles = 2;
+int64_t tile_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kSms) * 2 * chitu::kTilePieceFloats * 4; }
+
+template <bool kFp16, bool kEightBit>
+cudaError_t launch_tile(const CUtensorMap& tk, const CUtensorMap& tv, const chitu::CacheAttnParams& p, cudaStream_t st) {
+  static bool done[kMaxDevices] = {};
+  constexpr int smem = chitu::TileShape<kEightBit>::smem;
+  cudaError_t e = allow_smem(chitu::attn_cache_tile_kernel<kFp16, kEightBit>, smem, done);
+  if (e != cudaSuccess) return e;
+  chitu::attn_cache_tile_kernel<kFp16, kEightBit><<<kSms, chitu::kTileThreads, smem, st>>>(tk, tv, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  chitu::attn_cache_join_kernel<kFp16><<<dim3(kSms - 1, chitu::kTileRows / 32), 256, 0, st>>>(p, kSms);
   return cudaGetLastError();
 }
 
@@ -226,16 +269,9 @@ int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const 
   return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "kv_append: launch");
 }
 
-int64_t chitu_b200_attn_cache_workspace_bytes(int batch, int64_t tokens, int heads, int q_heads, int format, int max_q,
-                                              int max_kv) {
-  (void)batch;
-  (void)tokens;
-  (void)heads;
-  (void)q_heads;
-  (void)format;
-  (void)max_q;
-  (void)max_kv;
-  return rows_workspace_bytes();
+int64_t chitu_b200_attn_cache_workspace_bytes(int heads, int q_heads, int max_q) {
+  if (heads < 1 || q_heads < heads) return 0;
+  return takes_tile_kernel(max_q, q_heads / heads) ? tile_workspace_bytes() : rows_workspace_bytes();
 }
 
 int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, const int64_t* q_strides, void* out, float* lse,
@@ -251,7 +287,9 @@ int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, c
   if (!aligned16(q) || !aligned16(out) || !strides_fit(q_strides, tokens, q_heads, 2))
     return fail(CHITU_E_INVALID, "attn_fwd_cache: q and out must be 16-byte aligned, strides positive multiples of 8 elements");
   if (tokens == 0 || cache->batch == 0) return CHITU_OK;
-  const int64_t need = chitu_b200_attn_cache_workspace_bytes(cache->batch, tokens, cache->heads, q_heads, cache->format, max_q, max_kv);
+  max_q = std::max(max_q, 1);
+  max_kv = std::max(max_kv, 1);
+  const int64_t need = chitu_b200_attn_cache_workspace_bytes(cache->heads, q_heads, max_q);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(CHITU_E_INVALID, "attn_fwd_cache: workspace must be 16-byte aligned and hold %lld bytes", static_cast<long long>(need));
   chitu::CacheAttnParams p = {};
@@ -288,13 +326,25 @@ int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, c
   p.page_shift = page_shift_of(cache->page_size);
   p.causal = causal;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  p.min_tiles = kRowsMinTiles;
+  p.tok_blk = p.group <= chitu::kTileRows ? chitu::kTileRows / p.group : 0;
+  p.out_aligned32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
   p.count = static_cast<int*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kHeaderBytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool fp16 = dtype == CHITU_DTYPE_FP16, eight = es == 1;
-  cudaError_t e = fp16 ? (eight ? launch_rows<true, true>(p, st) : launch_rows<true, false>(p, st))
-                       : (eight ? launch_rows<false, true>(p, st) : launch_rows<false, false>(p, st));
+  cudaError_t e;
+  if (takes_tile_kernel(max_q, p.group)) {
+    CUtensorMap tk, tv;
+    if (int rc = make_cache_map(&tk, cache, cache->k, cache->k_strides, "k_cache")) return rc;
+    if (int rc = make_cache_map(&tv, cache, cache->v, cache->v_strides, "v_cache")) return rc;
+    p.min_tiles = kTileMinTiles;
+    e = fp16 ? (eight ? launch_tile<true, true>(tk, tv, p, st) : launch_tile<true, false>(tk, tv, p, st))
+             : (eight ? launch_tile<false, true>(tk, tv, p, st) : launch_tile<false, false>(tk, tv, p, st));
+    return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "attn_fwd_cache: launch");
+  }
+  p.min_tiles = kRowsMinTiles;
+  e = fp16 ? (eight ? launch_rows<true, true>(p, max_q, max_kv, st) : launch_rows<true, false>(p, max_q, max_kv, st))
+           : (eight ? launch_rows<false, true>(p, max_q, max_kv, st) : launch_rows<false, false>(p, max_q, max_kv, st));
   return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "attn_fwd_cache: launch");
 }
 

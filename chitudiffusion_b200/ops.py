@@ -1174,7 +1174,7 @@ def attn_fwd_cache(
     max_kv = width * page if max_kv is None else max(1, min(int(max_kv), width * page))
     lib = _lib.load()
     with _on(device):
-        need = lib.chitu_b200_attn_cache_workspace_bytes(B, T, heads, Hq, _lib.CACHE_E4M3 if eight else _lib.CACHE_16BIT, max_q, max_kv)
+        need = lib.chitu_b200_attn_cache_workspace_bytes(heads, Hq, max_q)
         ws = _cache_scratch(device, need) if need else None
         rc = lib.chitu_b200_attn_fwd_cache(
             packed, q.data_ptr(), _lib._I64x2(*q.stride()[:2]), out.data_ptr(), lse.data_ptr() if lse is not None else None, Hq, T,

@@ -543,13 +543,12 @@ int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const 
  * fp32 (natural log, scale included) or NULL.  A query that no key is visible to gives zeros and -inf.  Keys and values
  * behind a sequence's length are never read; those within it have to be finite.  softmax_scale must be positive.
  *
- * max_q and max_kv are how many queries and keys the longest sequence is expected to have: they choose the kernel and the
- * grid, and results are right whatever the lengths turn out to be.  workspace: chitu_b200_attn_cache_workspace_bytes(...) bytes,
+ * max_q and max_kv are how many queries and keys the longest sequence is expected to have: they choose the kernel and its grid,
+ * and results are right whatever the lengths turn out to be (the work is shared out on the device).  workspace: chitu_b200_attn_cache_workspace_bytes(...) bytes,
  * 16-byte aligned, its first CHITU_SPLITKV_HEADER_BYTES zero before the first call and left zero by each (rules as for
  * chitu_b200_attn_fwd_splitkv, with which it may be shared).
  */
-int64_t chitu_b200_attn_cache_workspace_bytes(int batch, int64_t tokens, int heads, int q_heads, int format, int max_q,
-                                              int max_kv);
+int64_t chitu_b200_attn_cache_workspace_bytes(int heads, int q_heads, int max_q);
 int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, const int64_t* q_strides, void* out, float* lse,
                               int q_heads, int64_t tokens, float softmax_scale, int causal, int dtype, int max_q, int max_kv,
                               void* workspace, int64_t workspace_bytes, int* status, void* stream);
