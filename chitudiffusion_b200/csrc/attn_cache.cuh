@@ -84,17 +84,8 @@ __device__ __forceinline__ uint32_t widen_e4m3x2(uint32_t two_codes) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two_codes)));
   return h;
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-  const int n = take ? 16 : 0;  // (0: the destination is filled with zeros)
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int n>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
 }
 __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
   uint4 v;
@@ -113,19 +104,23 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
 //
 // A warp takes 16 of a tile's 64 keys and keeps its own softmax.  The matrix instructions' sum over channels and the output's
 // channels may be numbered as is convenient, so a lane's fragments are whole 16-byte pieces of cache rows: for q k^T, of key
-// lane / 4, the pieces lane % 4; for p v, of four keys, the piece lane / 4.  A lane copies exactly the bytes that it reads
-// itself (cp.async, kStages steps deep, over item borders), so the warps need no barrier inside a run; lanes 0 and 1 fetch the
-// scales of the warp's keys beside them.
+// lane / 4, the pieces lane % 4 (and every fourth further); for p v, of four keys, the piece lane / 4.  Each warp has a ring of its
+// own that one lane fills by tensor copies (a box is 16 tokens of a page, which 16 keys never leave; a page that does not exist
+// reads zeros), over item borders, so the warps need no barrier inside a run.
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kRowsTile = 16 * kRowsWarps;
-constexpr int kRowsMergeBytes = 2 * 16 * 32 * 16;  // two warps' accumulators
+constexpr int kRowsMergeBytes = 16 * 32 * 16;  // one warp's accumulators, or half of two warps'
 template <bool kEightBit>
 struct RowsShape {
-  static constexpr int stages = kEightBit ? 5 : 4;
+  static constexpr int ctas_per_sm = kEightBit ? 3 : 2;
+  static constexpr int stages = 3;
   static constexpr int step_bytes = kEightBit ? 4096 : 8192;  // 16 keys and values
-  static constexpr int stage_bytes = step_bytes + 16;  // and the scales of the keys' page, and whether there is one
-  static constexpr int smem = kRowsWarps * stages * stage_bytes + kRowsMergeBytes + kRowsWarps * 16 * 8 + 16;
+  static constexpr int ring = kRowsWarps * stages * step_bytes;
+  static constexpr int meta_at = ring + kRowsMergeBytes;      // per warp and stage: scales, whether there is a page
+  static constexpr int stat_at = meta_at + kRowsWarps * stages * 16;
+  static constexpr int bar_at = stat_at + kRowsWarps * 16 * 8;
+  static constexpr int smem = bar_at + kRowsWarps * stages * 8 + 16 + 1024;
 };
 // scratch of one piece: 16 x 32 float4 of the accumulator's fragments, then (maximum, sum) of 16 rows
 constexpr int kRowsPieceFloats = 16 * 32 * 4 + 32;
@@ -237,17 +232,20 @@ __device__ __forceinline__ void rows_join(float (&o)[16][4], float (&m)[2], floa
     m[i] = top;
     l[i] = sum;
   }
+  // warps 2 and 3 to 0 and 1, half of the accumulators at a time, then warp 1 to warp 0
+  static_assert(kRowsWarps == 4, "the order below");
+  auto move = [&](int from, int to, int n_warps, int t0, int n) {
+    if (warp >= from && warp < from + n_warps) {
 #pragma unroll
-  for (int half = kRowsWarps / 2; half > 0; half >>= 1) {
-    if (warp >= half && warp < 2 * half) {
-#pragma unroll
-      for (int t = 0; t < 16; ++t) buf[(warp - half) * 512 + t * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
+      for (int t = 0; t < 16; ++t)
+        if (t >= t0 && t < t0 + n) buf[((warp - from) * n + t - t0) * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
     }
     __syncthreads();
-    if (warp < half) {
+    if (warp >= to && warp < to + n_warps) {
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
-        const float4 v = buf[warp * 512 + t * 32 + lane];
+        if (t < t0 || t >= t0 + n) continue;
+        const float4 v = buf[((warp - to) * n + t - t0) * 32 + lane];
         o[t][0] += v.x;
         o[t][1] += v.y;
         o[t][2] += v.z;
@@ -255,21 +253,37 @@ __device__ __forceinline__ void rows_join(float (&o)[16][4], float (&m)[2], floa
       }
     }
     __syncthreads();
-  }
+  };
+  move(2, 0, 2, 0, 8);
+  move(2, 0, 2, 8, 8);
+  move(1, 0, 1, 0, 16);
 }
 
 template <bool kFp16, bool kEightBit>
-__global__ void __launch_bounds__(kRowsThreads)
-attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
+__global__ void __launch_bounds__(kRowsThreads, RowsShape<kEightBit>::ctas_per_sm)
+attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CacheAttnParams p) {
   using Shape = RowsShape<kEightBit>;
   constexpr int kStages = Shape::stages;
   constexpr bool kHalf = kEightBit || kFp16;  // fp16 products
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * Shape::stage_bytes;
-  float4* join_buf = reinterpret_cast<float4*>(smem + kRowsWarps * kStages * Shape::stage_bytes);
-  float2* join_stat = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(join_buf) + kRowsMergeBytes);
-  volatile int* last_flag = reinterpret_cast<volatile int*>(join_stat + kRowsWarps * 16);
+  const uint32_t ring = smem_base + warp * kStages * Shape::step_bytes;
+  const uint32_t meta_ring = smem_base + Shape::meta_at + warp * kStages * 16;
+  const uint32_t bars = smem_base + Shape::bar_at + warp * kStages * 8;
+  float4* join_buf = reinterpret_cast<float4*>(smem + Shape::ring);
+  float2* join_stat = reinterpret_cast<float2*>(smem + Shape::stat_at);
+  volatile int* last_flag = reinterpret_cast<volatile int*>(smem + Shape::bar_at + kRowsWarps * kStages * 8);
+  volatile int* abort_flag = last_flag + 1;
+  if (lane == 0) {
+    *abort_flag = 0;
+    // a step's copies, and lanes 0's and 1's of the scales
+    for (int s = 0; s < kStages; ++s) mbar_init(bars + 8 * s, kEightBit ? 3 : 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  __syncwarp();
 
   // all steps, and where this CTA's run begins (each warp finds out by itself)
   long long total = 0;
@@ -277,8 +291,9 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(p.min_tiles));
-  const long long lo = blockIdx.x * per, hi = min(lo + per, total);
-  if (lo >= hi) return;
+  const long long lo = blockIdx.x * per;
+  if (lo >= total) return;
+  const int n_steps = static_cast<int>(min(per, total - lo));
   RowsCursor cur;
   long long at = 0;  // steps before sequence cur.b
   for (cur.b = 0;; cur.b += 32) {
@@ -309,8 +324,8 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
     cur.tile = static_cast<int>(lo - item_start);
   }
   RowsCursor ahead = cur;  // what is copied next
-  long long copied = lo;
-  auto page_of = [&](const RowsCursor& w) {  // page of this warp's 16 keys (they never cross a page), -1: none
+  int copied = 0;
+  auto page_of = [&](const RowsCursor& w) {  // page of this warp's 16 keys, -1: none
     const int key = w.tile * kRowsTile + warp * 16;
     if (key >= w.seq.len) return -1;
     const int id = __ldg(p.block_table + w.b * p.table_stride + (key >> p.page_shift));
@@ -318,54 +333,41 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
   };
   int ahead_page = page_of(ahead);
   auto copy_step = [&](int stage) {
-    const uint32_t meta = ring + stage * Shape::stage_bytes + Shape::step_bytes;
-    const uint32_t dst = ring + stage * Shape::stage_bytes + lane * 16;
-    if (kEightBit && lane < 2 && ahead_page >= 0) cp_async4(meta + 4 * lane, p.scale[lane] + ahead_page * p.s_page[lane] + ahead.h * p.s_head[lane]);
-    if (lane == 2) asm volatile("st.shared.u32 [%0], %1;" ::"r"(meta + 8), "r"(ahead_page >= 0 ? 1 : 0) : "memory");
-    const int key0 = ahead.tile * kRowsTile + warp * 16;
-    const int in_page = key0 & ((1 << p.page_shift) - 1);
-    const int left = ahead_page < 0 ? 0 : ahead.seq.len - key0;  // keys of the 16 that exist
-    const long long id = max(ahead_page, 0);
-    const uint8_t* k = p.cache[0] + id * p.c_page[0] + ahead.h * p.c_head[0] + in_page * p.c_token[0] + c * 16;
-    const uint8_t* v = p.cache[1] + id * p.c_page[1] + ahead.h * p.c_head[1] + in_page * p.c_token[1] + g * (kEightBit ? 16 : 32);
-    constexpr int kPieces = kEightBit ? 2 : 4;
-    // (a row that does not exist: nothing is read, but the address stays inside the page)
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const bool there = g + 8 * n < left;
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j) cp_async16(dst + (n * kPieces + j) * 512, k + (there ? (g + 8 * n) * p.c_token[0] : 0) + j * 64, there);
+    const uint32_t bar = bars + 8 * stage;
+    const uint32_t meta = meta_ring + stage * 16;
+    if (lane == 0) {
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(meta + 8), "r"(ahead_page >= 0 ? 1 : 0) : "memory");
+      mbar_arrive_expect_tx(bar, Shape::step_bytes);
+      const uint32_t dst = ring + stage * Shape::step_bytes;
+      const int token = (ahead.tile * kRowsTile + warp * 16) & ((1 << p.page_shift) - 1);
+      if constexpr (kEightBit) {
+        tma_load_4d(dst, &tm_k, bar, 0, ahead.h, token, ahead_page);
+        tma_load_4d(dst + 2048, &tm_v, bar, 0, ahead.h, token, ahead_page);
+      } else {
+        tma_load_4d(dst, &tm_k, bar, 0, ahead.h, token, ahead_page);
+        tma_load_4d(dst + 2048, &tm_k, bar, 64, ahead.h, token, ahead_page);
+        tma_load_4d(dst + 4096, &tm_v, bar, 0, ahead.h, token, ahead_page);
+        tma_load_4d(dst + 6144, &tm_v, bar, 64, ahead.h, token, ahead_page);
+      }
     }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int key = 2 * c + (n & 1) + (n >> 1) * 8;
-      const bool there = key < left;
-#pragma unroll
-      for (int j = 0; j < kPieces / 2; ++j)
-        cp_async16(dst + (2 * kPieces + n * (kPieces / 2) + j) * 512, v + (there ? key * p.c_token[1] : 0) + j * 16, there);
+    if (kEightBit && lane < 2) {
+      if (ahead_page >= 0) cp_async4(meta + 4 * lane, p.scale[lane] + ahead_page * p.s_page[lane] + ahead.h * p.s_head[lane]);
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     }
-  };
-  auto advance_copy = [&] {
     if (++ahead.tile == ahead.n_tiles) ahead.next_item(p);
-    ++copied;
-    if (copied < hi) ahead_page = page_of(ahead);
+    if (++copied < n_steps) ahead_page = page_of(ahead);
   };
 #pragma unroll 1
-  for (int s = 0; s < kStages - 1; ++s) {
-    if (copied < hi) {
-      copy_step(s);
-      advance_copy();
-    }
-    cp_async_commit();
-  }
+  for (int s = 0; s < kStages; ++s)
+    if (copied < n_steps) copy_step(s);
 
   uint32_t qf[8][4];
   float factor[2], o[16][4], m[2], l[2];
-  int limit[2];
-  int stage = 0;
+  int limit[2], unmasked = 0;  // keys that all rows see
+  int stage = 0, phase = 0;
   bool fresh = true;
 #pragma unroll 1
-  for (long long step = lo; step < hi; ++step) {
+  for (int step = 0; step < n_steps; ++step) {
     if (fresh) {
       rows_load_q<kFp16, kEightBit>(p, cur, g, c, qf, factor);
 #pragma unroll
@@ -375,6 +377,7 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
         m[i] = -INFINITY;
         l[i] = 0.f;
       }
+      unmasked = p.causal ? min(cur.seq.first + cur.rb * 16 / p.group + 1, cur.seq.len) : cur.seq.len;
 #pragma unroll
       for (int t = 0; t < 16; ++t)
 #pragma unroll
@@ -382,27 +385,28 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
       fresh = false;
     }
     const int key0 = cur.tile * kRowsTile + warp * 16;
-    cp_async_wait<kStages - 2>();
-    __syncwarp();  // (the scales are lanes 0's and 1's copies)
-    const uint32_t src = ring + stage * Shape::stage_bytes + lane * 16;
-    const uint4 meta = ld_shared16(ring + stage * Shape::stage_bytes + Shape::step_bytes);
-    const bool paged = meta.z != 0;
+    mbar_wait(bars + 8 * stage, phase, abort_flag, p.status, kDevTimeoutSoftmax);
+    __syncwarp();
+    const uint32_t src = ring + stage * Shape::step_bytes;
+    const uint4 meta = ld_shared16(meta_ring + stage * 16);
     float k_scale = 1.f, v_log2 = 0.f, v_inv = 1.f;
-    if (kEightBit && paged) {
+    if (kEightBit && meta.z != 0) {
       k_scale = __uint_as_float(meta.x);
       const float vs = fmaxf(__uint_as_float(meta.y), kMinValueScale);
       v_log2 = __log2f(vs);
       v_inv = __fdividef(1.f, vs);
     }
+    // rows of 128 bytes, their 16-byte pieces exchanged by row & 7
     float s[2][4];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      const uint32_t row = src + (g + 8 * n) * 128;
       if constexpr (kEightBit) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint4 w = ld_shared16(src + (n * 2 + j) * 512);
+          const uint4 w = ld_shared16(row + (((j * 4 + c) ^ g) << 4));
           const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) mma_16816_f16(s[n], qf[j * 4 + k], widen_e4m3x2(w4[k]), widen_e4m3x2(w4[k] >> 16));
@@ -410,13 +414,14 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint4 w = ld_shared16(src + (n * 4 + j) * 512);
+          const uint4 w = ld_shared16(row + (j >> 1) * 2048 + ((((j & 1) * 4 + c) ^ g) << 4));
           mma_16816<kHalf>(s[n], qf[j * 2], w.x, w.y);
           mma_16816<kHalf>(s[n], qf[j * 2 + 1], w.z, w.w);
         }
       }
     }
     // scores of rows g (e = 0, 1) and g + 8 (e = 2, 3), keys key0 + 8 n + 2 c + (e & 1), in units of log2
+    const bool border = key0 + 16 > unmasked || meta.z == 0;  // (the same for the whole warp)
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -424,12 +429,15 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float& x = s[n][2 * i + e];
-          x = fmaf(x, f, v_log2);
-          if (!paged || key0 + 8 * n + 2 * c + e >= limit[i]) x = -INFINITY;
-          top[i] = fmaxf(top[i], x);
-        }
+        for (int e = 0; e < 2; ++e) s[n][2 * i + e] = fmaf(s[n][2 * i + e], f, v_log2);
+      if (border) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (meta.z == 0 || key0 + 8 * n + 2 * c + e >= limit[i]) s[n][2 * i + e] = -INFINITY;
+      }
+      top[i] = fmaxf(max3(s[0][2 * i], s[0][2 * i + 1], s[1][2 * i]), s[1][2 * i + 1]);
     }
     if (__any_sync(0xffffffffu, top[0] > m[0] + kRescaleThreshold || top[1] > m[1] + kRescaleThreshold)) {
 #pragma unroll
@@ -459,52 +467,48 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
         pf[n * 2 + i] = pack2<kHalf>(a, b);
       }
     }
-    // o += p v: lane's channels 16 g + t, t = 0 .. 15
-    if constexpr (kEightBit) {
+    // o += p v: lane's channels 16 g + t, t = 0 .. 15, of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+    const int left = cur.seq.len - key0;
+    constexpr int kPieces = kEightBit ? 1 : 2;
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
       uint4 w[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) w[n] = ld_shared16(src + (4 + n) * 512);
+      for (int n = 0; n < 4; ++n) {
+        const int key = 2 * c + (n & 1) + (n >> 1) * 8;
+        const uint32_t row = src + (kEightBit ? 2048 : 4096 + (g >> 2) * 2048) + key * 128;
+        w[n] = ld_shared16(row + (((kEightBit ? g : (g & 3) * 2 + j) ^ (key & 7)) << 4));
+        // what the page holds behind the sequence's end may be anything: no weight is not enough
+        if (border && key >= left) w[n] = make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint32_t r0 = q == 0 ? w[0].x : q == 1 ? w[0].y : q == 2 ? w[0].z : w[0].w;
         const uint32_t r1 = q == 0 ? w[1].x : q == 1 ? w[1].y : q == 2 ? w[1].z : w[1].w;
         const uint32_t r2 = q == 0 ? w[2].x : q == 1 ? w[2].y : q == 2 ? w[2].z : w[2].w;
         const uint32_t r3 = q == 0 ? w[3].x : q == 1 ? w[3].y : q == 2 ? w[3].z : w[3].w;
-        const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
-        const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
-        mma_16816_f16(o[4 * q], pf, widen_e4m3x2(lo01), widen_e4m3x2(lo23));
-        mma_16816_f16(o[4 * q + 1], pf, widen_e4m3x2(lo01 >> 16), widen_e4m3x2(lo23 >> 16));
-        mma_16816_f16(o[4 * q + 2], pf, widen_e4m3x2(hi01), widen_e4m3x2(hi23));
-        mma_16816_f16(o[4 * q + 3], pf, widen_e4m3x2(hi01 >> 16), widen_e4m3x2(hi23 >> 16));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint4 w[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) w[n] = ld_shared16(src + (8 + n * 2 + j) * 512);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t r0 = q == 0 ? w[0].x : q == 1 ? w[0].y : q == 2 ? w[0].z : w[0].w;
-          const uint32_t r1 = q == 0 ? w[1].x : q == 1 ? w[1].y : q == 2 ? w[1].z : w[1].w;
-          const uint32_t r2 = q == 0 ? w[2].x : q == 1 ? w[2].y : q == 2 ? w[2].z : w[2].w;
-          const uint32_t r3 = q == 0 ? w[3].x : q == 1 ? w[3].y : q == 2 ? w[3].z : w[3].w;
+        if constexpr (kEightBit) {
+          const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
+          const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
+          mma_16816_f16(o[4 * q], pf, widen_e4m3x2(lo01), widen_e4m3x2(lo23));
+          mma_16816_f16(o[4 * q + 1], pf, widen_e4m3x2(lo01 >> 16), widen_e4m3x2(lo23 >> 16));
+          mma_16816_f16(o[4 * q + 2], pf, widen_e4m3x2(hi01), widen_e4m3x2(hi23));
+          mma_16816_f16(o[4 * q + 3], pf, widen_e4m3x2(hi01 >> 16), widen_e4m3x2(hi23 >> 16));
+        } else {
           mma_16816<kHalf>(o[8 * j + 2 * q], pf, __byte_perm(r0, r1, 0x5410), __byte_perm(r2, r3, 0x5410));
           mma_16816<kHalf>(o[8 * j + 2 * q + 1], pf, __byte_perm(r0, r1, 0x7632), __byte_perm(r2, r3, 0x7632));
         }
       }
     }
-    // the stage read in the step before this one is free: every lane has been through this step's __syncwarp since
-    const int refill = stage == 0 ? kStages - 1 : stage - 1;
-    if (copied < hi) {
-      copy_step(refill);
-      advance_copy();
+    __syncwarp();  // every lane has read the stage
+    if (copied < n_steps) copy_step(stage);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
     }
-    cp_async_commit();
-    stage = stage + 1 == kStages ? 0 : stage + 1;
 
     const bool item_done = cur.tile + 1 == cur.n_tiles;
-    if (!item_done && step + 1 < hi) {
+    if (!item_done && step + 1 < n_steps) {
       ++cur.tile;
       continue;
     }
@@ -601,13 +605,18 @@ attn_cache_rows_kernel(const __grid_constant__ CacheAttnParams p) {
         }
       }
     }
-    if (step + 1 < hi) {
+    if (step + 1 < n_steps) {
       item_start = item_end;
       cur.next_item(p);
       fresh = true;
     }
   }
-  cp_async_wait<0>();
+  if (*abort_flag && lane == 0) {
+    // A wait has run out: nothing of ours may still be landing when the CTA retires (bounded polls on the last copies).
+    for (int i = max(0, n_steps - kStages); i < n_steps; ++i)
+      for (int spin = 0; spin < (1 << 20) && !mbar_try_wait(bars + 8 * (i % kStages), (i / kStages) & 1); ++spin) {
+      }
+  }
 }
 
 }  // namespace chitu

@@ -72,27 +72,10 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices]) {
 
 constexpr int kSms = 148;
 
-// Grid of the rows kernel: all CTAs resident at once (two per SM), or as many as there can be runs of kRowsMinTiles tiles.
-constexpr int kRowsGrid = kSms * 2;
-constexpr int kRowsMinTiles = 2;
-int64_t rows_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kRowsGrid) * 2 * chitu::kRowsPieceFloats * 4; }
-
-template <bool kFp16, bool kEightBit>
-cudaError_t launch_rows(const chitu::CacheAttnParams& p, int max_q, int max_kv, cudaStream_t st) {
-  static bool done[kMaxDevices] = {};
-  constexpr int smem = chitu::RowsShape<kEightBit>::smem;
-  cudaError_t e = allow_smem(chitu::attn_cache_rows_kernel<kFp16, kEightBit>, smem, done);
-  if (e != cudaSuccess) return e;
-  const int64_t items = static_cast<int64_t>(p.batch) * p.heads_kv * ((static_cast<int64_t>(max_q) * p.group + 15) / 16);
-  const int64_t runs = (items * ((max_kv + chitu::kRowsTile - 1) / chitu::kRowsTile) + kRowsMinTiles - 1) / kRowsMinTiles;
-  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowsGrid, runs)));
-  chitu::attn_cache_rows_kernel<kFp16, kEightBit><<<grid, chitu::kRowsThreads, smem, st>>>(p);
-  return cudaGetLastError();
-}
-
-// Tensor map over a pool: channels, heads, tokens of a page, pages; a box is 128 bytes of the channels by a page's tokens, 128 of
-// them at most.  16-bit pages land in the swizzled layout of the matrix operands, codes as they are.
-int make_cache_map(CUtensorMap* map, const chitu_b200_kv_cache* c, const void* base, const int64_t* st, const char* name) {
+// Tensor map over a pool: channels, heads, tokens of a page, pages; a box is 128 bytes of the channels by
+// box_tokens of a page, its rows swizzled (the layout of the matrix operands) or as they are.
+int make_cache_map(CUtensorMap* map, const chitu_b200_kv_cache* c, const void* base, const int64_t* st, int box_tokens, bool swizzled,
+                   const char* name) {
   auto encode = chitu::get_encode_fn();
   if (!encode) return fail(CHITU_E_CUDA, "cuTensorMapEncodeTiled entry point not available");
   const bool eight = c->format == CHITU_CACHE_E4M3;
@@ -101,13 +84,31 @@ int make_cache_map(CUtensorMap* map, const chitu_b200_kv_cache* c, const void* b
   auto bytes = [&](int i, int64_t extent) { return extent == 1 ? cuuint64_t{256} : static_cast<cuuint64_t>(st[i]) * es; };
   cuuint64_t dims[4] = {128, static_cast<cuuint64_t>(c->heads), static_cast<cuuint64_t>(c->page_size), static_cast<cuuint64_t>(c->n_pages)};
   cuuint64_t strides[3] = {bytes(2, c->heads), bytes(1, c->page_size), bytes(0, c->n_pages)};
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), 1, static_cast<cuuint32_t>(std::min(c->page_size, 128)), 1};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), 1, static_cast<cuuint32_t>(box_tokens), 1};
   cuuint32_t elem[4] = {1, 1, 1, 1};
   CUresult r = encode(map, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
-                      elem, CU_TENSOR_MAP_INTERLEAVE_NONE, eight ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                      elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(CHITU_E_CUDA, "%s: cuTensorMapEncodeTiled failed with CUresult %d", name, static_cast<int>(r));
   return CHITU_OK;
+}
+
+// Grid of the rows kernel: all CTAs resident at once, or as many as there can be runs of kRowsMinTiles tiles.
+constexpr int kRowsGrid = kSms * 3;
+constexpr int kRowsMinTiles = 2;
+int64_t rows_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kRowsGrid) * 2 * chitu::kRowsPieceFloats * 4; }
+
+template <bool kFp16, bool kEightBit>
+cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const chitu::CacheAttnParams& p, int max_q, int max_kv, cudaStream_t st) {
+  static bool done[kMaxDevices] = {};
+  constexpr int smem = chitu::RowsShape<kEightBit>::smem;
+  cudaError_t e = allow_smem(chitu::attn_cache_rows_kernel<kFp16, kEightBit>, smem, done);
+  if (e != cudaSuccess) return e;
+  const int64_t items = static_cast<int64_t>(p.batch) * p.heads_kv * ((static_cast<int64_t>(max_q) * p.group + 15) / 16);
+  const int64_t runs = (items * ((max_kv + chitu::kRowsTile - 1) / chitu::kRowsTile) + kRowsMinTiles - 1) / kRowsMinTiles;
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kSms * chitu::RowsShape<kEightBit>::ctas_per_sm, runs)));
+  chitu::attn_cache_rows_kernel<kFp16, kEightBit><<<grid, chitu::kRowsThreads, smem, st>>>(tk, tv, p);
+  return cudaGetLastError();
 }
 
 // Which kernel a call takes.  Up to 16 query rows of a key head (tokens x heads that share it) are one tile of the rows kernel;
@@ -333,18 +334,20 @@ int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, c
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool fp16 = dtype == CHITU_DTYPE_FP16, eight = es == 1;
   cudaError_t e;
-  if (takes_tile_kernel(max_q, p.group)) {
-    CUtensorMap tk, tv;
-    if (int rc = make_cache_map(&tk, cache, cache->k, cache->k_strides, "k_cache")) return rc;
-    if (int rc = make_cache_map(&tv, cache, cache->v, cache->v_strides, "v_cache")) return rc;
+  const bool tile = takes_tile_kernel(max_q, p.group);
+  const int box = tile ? std::min(cache->page_size, 128) : 16;
+  CUtensorMap tk, tv;
+  if (int rc = make_cache_map(&tk, cache, cache->k, cache->k_strides, box, !(tile && eight), "k_cache")) return rc;
+  if (int rc = make_cache_map(&tv, cache, cache->v, cache->v_strides, box, !(tile && eight), "v_cache")) return rc;
+  if (tile) {
     p.min_tiles = kTileMinTiles;
     e = fp16 ? (eight ? launch_tile<true, true>(tk, tv, p, st) : launch_tile<true, false>(tk, tv, p, st))
              : (eight ? launch_tile<false, true>(tk, tv, p, st) : launch_tile<false, false>(tk, tv, p, st));
     return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "attn_fwd_cache: launch");
   }
   p.min_tiles = kRowsMinTiles;
-  e = fp16 ? (eight ? launch_rows<true, true>(p, max_q, max_kv, st) : launch_rows<true, false>(p, max_q, max_kv, st))
-           : (eight ? launch_rows<false, true>(p, max_q, max_kv, st) : launch_rows<false, false>(p, max_q, max_kv, st));
+  e = fp16 ? (eight ? launch_rows<true, true>(tk, tv, p, max_q, max_kv, st) : launch_rows<true, false>(tk, tv, p, max_q, max_kv, st))
+           : (eight ? launch_rows<false, true>(tk, tv, p, max_q, max_kv, st) : launch_rows<false, false>(tk, tv, p, max_q, max_kv, st));
   return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "attn_fwd_cache: launch");
 }
 
