@@ -98,27 +98,28 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
 // ----------------------------------------------------------------------------
 //
 // Memory bound: a key and a value byte are read once for at most 16 rows.  The grid's CTAs share all (sequence, 16 rows, key
-// head, 64-key tile) steps evenly, in that order: CTA c takes the c-th of gridDim.x equal runs, whatever the lengths are.  A
+// head, tile of keys) steps evenly, in that order: CTA c takes the c-th of gridDim.x equal runs, whatever the lengths are.  A
 // run that ends inside an item (sequence, rows, head) leaves the item's fp32 piece in scratch, and the CTA that completes the
 // item's count merges its pieces in order; nobody waits.
 //
-// A warp takes 16 of a tile's 64 keys and keeps its own softmax.  The matrix instructions' sum over channels and the output's
-// channels may be numbered as is convenient, so a lane's fragments are whole 16-byte pieces of cache rows: for q k^T, of key
-// lane / 4, the pieces lane % 4 (and every fourth further); for p v, of four keys, the piece lane / 4.  Each warp has a ring of its
-// own that one lane fills by tensor copies (a box is 16 tokens of a page, which 16 keys never leave; a page that does not exist
-// reads zeros), over item borders, so the warps need no barrier inside a run.
+// A warp takes 32 (16-bit pages: 16) of a tile's keys and keeps its own softmax.  The matrix instructions' sum over channels and the
+// output's channels may be numbered as is convenient, so a lane's fragments are whole 16-byte pieces of cache rows: for q k^T, of
+// key lane / 4, the pieces lane % 4 (and every fourth further); for p v, of four keys, the piece lane / 4.  Each warp has a ring of
+// its own that one lane fills by tensor copies (a box is 16 or 32 tokens of a page; a page that does not exist reads zeros), over
+// item borders, so the warps need no barrier inside a run.
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
-constexpr int kRowsTile = 16 * kRowsWarps;
 constexpr int kRowsMergeBytes = 16 * 32 * 16;  // one warp's accumulators, or half of two warps'
 template <bool kEightBit>
 struct RowsShape {
   static constexpr int ctas_per_sm = kEightBit ? 3 : 2;
-  static constexpr int stages = 3;
-  static constexpr int step_bytes = kEightBit ? 4096 : 8192;  // 16 keys and values
+  static constexpr int stages = kEightBit ? 2 : 3;
+  static constexpr int keys = kEightBit ? 32 : 16;            // of a warp's step
+  static constexpr int tile = keys * kRowsWarps;
+  static constexpr int step_bytes = 8192;                     // keys, then values
   static constexpr int ring = kRowsWarps * stages * step_bytes;
-  static constexpr int meta_at = ring + kRowsMergeBytes;      // per warp and stage: scales, whether there is a page
-  static constexpr int stat_at = meta_at + kRowsWarps * stages * 16;
+  static constexpr int meta_at = ring + kRowsMergeBytes;      // per warp and stage: scales of both halves, whether they have a page
+  static constexpr int stat_at = meta_at + kRowsWarps * stages * 32;
   static constexpr int bar_at = stat_at + kRowsWarps * 16 * 8;
   static constexpr int smem = bar_at + kRowsWarps * stages * 8 + 16 + 1024;
 };
@@ -127,14 +128,16 @@ constexpr int kRowsPieceFloats = 16 * 32 * 4 + 32;
 
 // Position in the order of steps.
 struct RowsCursor {
-  int b, rb, h, tile;   // sequence, 16-row block, key head, 64-key tile
+  int b, rb, h, tile;   // sequence, 16-row block, key head, tile of keys
   int n_rb, n_tiles;    // of the sequence
   SeqInfo seq;
+  template <int kTile>
   __device__ __forceinline__ void measure(const CacheAttnParams& p) {
     seq = seq_info(p, b);
     n_rb = (seq.n_new * p.group + 15) >> 4;
-    n_tiles = max((seq.len + kRowsTile - 1) / kRowsTile, 1);
+    n_tiles = max((seq.len + kTile - 1) / kTile, 1);
   }
+  template <int kTile>
   __device__ __forceinline__ void next_item(const CacheAttnParams& p) {
     tile = 0;
     if (++h < p.heads_kv) return;
@@ -142,15 +145,16 @@ struct RowsCursor {
     if (++rb < n_rb) return;
     rb = 0;
     while (++b < p.batch) {
-      measure(p);
+      measure<kTile>(p);
       if (n_rb > 0) return;
     }
   }
 };
+template <int kTile>
 __device__ __forceinline__ long long rows_steps(const CacheAttnParams& p, int b) {
   const SeqInfo s = seq_info(p, b);
   const long long n_rb = (static_cast<long long>(s.n_new) * p.group + 15) >> 4;
-  return n_rb * p.heads_kv * max((s.len + kRowsTile - 1) / kRowsTile, 1);
+  return n_rb * p.heads_kv * max((s.len + kTile - 1) / kTile, 1);
 }
 
 // Query rows g and g + 8 as matrix fragments: for 8-bit pages piece j (64 channels), step k (16 of them) is channels
@@ -263,14 +267,15 @@ template <bool kFp16, bool kEightBit>
 __global__ void __launch_bounds__(kRowsThreads, RowsShape<kEightBit>::ctas_per_sm)
 attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CacheAttnParams p) {
   using Shape = RowsShape<kEightBit>;
-  constexpr int kStages = Shape::stages;
+  constexpr int kStages = Shape::stages, kKeys = Shape::keys, kTile = Shape::tile;
+  constexpr int kHalves = kKeys / 16;
   constexpr bool kHalf = kEightBit || kFp16;  // fp16 products
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_base + warp * kStages * Shape::step_bytes;
-  const uint32_t meta_ring = smem_base + Shape::meta_at + warp * kStages * 16;
+  const uint32_t meta_ring = smem_base + Shape::meta_at + warp * kStages * 32;
   const uint32_t bars = smem_base + Shape::bar_at + warp * kStages * 8;
   float4* join_buf = reinterpret_cast<float4*>(smem + Shape::ring);
   float2* join_stat = reinterpret_cast<float2*>(smem + Shape::stat_at);
@@ -278,8 +283,8 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   volatile int* abort_flag = last_flag + 1;
   if (lane == 0) {
     *abort_flag = 0;
-    // a step's copies, and lanes 0's and 1's of the scales
-    for (int s = 0; s < kStages; ++s) mbar_init(bars + 8 * s, kEightBit ? 3 : 1);
+    // a step's copies, and four lanes' of the scales
+    for (int s = 0; s < kStages; ++s) mbar_init(bars + 8 * s, kEightBit ? 5 : 1);
     mbar_fence_init();
     fence_proxy_async_smem();
   }
@@ -287,7 +292,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 
   // all steps, and where this CTA's run begins (each warp finds out by itself)
   long long total = 0;
-  for (int b = lane; b < p.batch; b += 32) total += rows_steps(p, b);
+  for (int b = lane; b < p.batch; b += 32) total += rows_steps<kTile>(p, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(p.min_tiles));
@@ -298,7 +303,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   long long at = 0;  // steps before sequence cur.b
   for (cur.b = 0;; cur.b += 32) {
     const int b = cur.b + lane;
-    const long long mine = b < p.batch ? rows_steps(p, b) : 0;
+    const long long mine = b < p.batch ? rows_steps<kTile>(p, b) : 0;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -314,7 +319,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     }
     at += __shfl_sync(0xffffffffu, upto, 31);
   }
-  cur.measure(p);
+  cur.measure<kTile>(p);
   long long item_start;  // first step of the item under the cursor
   {
     const long long item = (lo - at) / cur.n_tiles;
@@ -325,45 +330,65 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   }
   RowsCursor ahead = cur;  // what is copied next
   int copied = 0;
-  auto page_of = [&](const RowsCursor& w) {  // page of this warp's 16 keys, -1: none
-    const int key = w.tile * kRowsTile + warp * 16;
-    if (key >= w.seq.len) return -1;
-    const int id = __ldg(p.block_table + w.b * p.table_stride + (key >> p.page_shift));
-    return id >= 0 && id < p.n_pages ? id : -1;
+  // Table entries of the keys that are copied next, loaded a step before they are looked at: entry(0) and, where pages are
+  // smaller than a step, entry(1).
+  const int* table = p.block_table + ahead.b * p.table_stride;
+  auto entry = [&](int half) {
+    const int key = ahead.tile * kTile + warp * kKeys + half * 16;
+    int id = -1;
+    if (key < ahead.seq.len) id = __ldg(table + (key >> p.page_shift));
+    return id;
   };
-  int ahead_page = page_of(ahead);
+  const bool small_pages = kHalves == 2 && p.page_shift == 4;
+  int entry0 = entry(0), entry1 = small_pages ? entry(1) : 0;
   auto copy_step = [&](int stage) {
     const uint32_t bar = bars + 8 * stage;
-    const uint32_t meta = meta_ring + stage * 16;
+    const uint32_t meta = meta_ring + stage * 32;
+    const int page0 = static_cast<unsigned>(entry0) < static_cast<unsigned>(p.n_pages) ? entry0 : -1;
+    const int page1 = small_pages ? (static_cast<unsigned>(entry1) < static_cast<unsigned>(p.n_pages) ? entry1 : -1) : page0;
     if (lane == 0) {
-      asm volatile("st.shared.u32 [%0], %1;" ::"r"(meta + 8), "r"(ahead_page >= 0 ? 1 : 0) : "memory");
+      asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(meta + 16), "r"(page0 >= 0 ? 1 : 0), "r"(page1 >= 0 ? 1 : 0) : "memory");
       mbar_arrive_expect_tx(bar, Shape::step_bytes);
       const uint32_t dst = ring + stage * Shape::step_bytes;
-      const int token = (ahead.tile * kRowsTile + warp * 16) & ((1 << p.page_shift) - 1);
+      const int token = (ahead.tile * kTile + warp * kKeys) & ((1 << p.page_shift) - 1);
       if constexpr (kEightBit) {
-        tma_load_4d(dst, &tm_k, bar, 0, ahead.h, token, ahead_page);
-        tma_load_4d(dst + 2048, &tm_v, bar, 0, ahead.h, token, ahead_page);
+        tma_load_4d(dst, &tm_k, bar, 0, ahead.h, token, page0);
+        tma_load_4d(dst + 4096, &tm_v, bar, 0, ahead.h, token, page0);
+        if (small_pages) {
+          tma_load_4d(dst + 2048, &tm_k, bar, 0, ahead.h, token, page1);
+          tma_load_4d(dst + 6144, &tm_v, bar, 0, ahead.h, token, page1);
+        }
       } else {
-        tma_load_4d(dst, &tm_k, bar, 0, ahead.h, token, ahead_page);
-        tma_load_4d(dst + 2048, &tm_k, bar, 64, ahead.h, token, ahead_page);
-        tma_load_4d(dst + 4096, &tm_v, bar, 0, ahead.h, token, ahead_page);
-        tma_load_4d(dst + 6144, &tm_v, bar, 64, ahead.h, token, ahead_page);
+        tma_load_4d(dst, &tm_k, bar, 0, ahead.h, token, page0);
+        tma_load_4d(dst + 2048, &tm_k, bar, 64, ahead.h, token, page0);
+        tma_load_4d(dst + 4096, &tm_v, bar, 0, ahead.h, token, page0);
+        tma_load_4d(dst + 6144, &tm_v, bar, 64, ahead.h, token, page0);
       }
     }
-    if (kEightBit && lane < 2) {
-      if (ahead_page >= 0) cp_async4(meta + 4 * lane, p.scale[lane] + ahead_page * p.s_page[lane] + ahead.h * p.s_head[lane]);
+    if (kEightBit && lane < 4) {
+      const int page = lane < 2 ? page0 : page1, kv = lane & 1;
+      if (page >= 0) cp_async4(meta + 4 * lane, p.scale[kv] + page * p.s_page[kv] + ahead.h * p.s_head[kv]);
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
     }
-    if (++ahead.tile == ahead.n_tiles) ahead.next_item(p);
-    if (++copied < n_steps) ahead_page = page_of(ahead);
+    if (++ahead.tile == ahead.n_tiles) {
+      ahead.next_item<kTile>(p);
+      table = p.block_table + ahead.b * p.table_stride;
+    }
+    if (++copied < n_steps) {
+      entry0 = entry(0);
+      if (small_pages) entry1 = entry(1);
+    }
   };
 #pragma unroll 1
   for (int s = 0; s < kStages; ++s)
     if (copied < n_steps) copy_step(s);
 
+  // A row's probabilities are 2^(score + shift), shift = kProbShift - m; the largest score so far may pass m by kRescaleThreshold
+  // before the shift moves.  A row that has seen no key has no limit to pass.
+  constexpr float kTop = kProbShift + kRescaleThreshold;
   uint32_t qf[8][4];
-  float factor[2], o[16][4], m[2], l[2];
-  int limit[2], unmasked = 0;  // keys that all rows see
+  float factor[2], o[16][4], shift[2], l[2], ceiling[2];
+  int limit[2], unmasked = 0;  // keys that a row, that all rows see
   int stage = 0, phase = 0;
   bool fresh = true;
 #pragma unroll 1
@@ -374,7 +399,8 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       for (int i = 0; i < 2; ++i) {
         const int r = cur.rb * 16 + g + 8 * i;
         limit[i] = p.causal ? min(cur.seq.first + r / p.group + 1, cur.seq.len) : cur.seq.len;
-        m[i] = -INFINITY;
+        shift[i] = 0.f;
+        ceiling[i] = -INFINITY;
         l[i] = 0.f;
       }
       unmasked = p.causal ? min(cur.seq.first + cur.rb * 16 / p.group + 1, cur.seq.len) : cur.seq.len;
@@ -384,122 +410,157 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
       fresh = false;
     }
-    const int key0 = cur.tile * kRowsTile + warp * 16;
+    const int key0 = cur.tile * kTile + warp * kKeys;
     mbar_wait(bars + 8 * stage, phase, abort_flag, p.status, kDevTimeoutSoftmax);
     __syncwarp();
     const uint32_t src = ring + stage * Shape::step_bytes;
-    const uint4 meta = ld_shared16(meta_ring + stage * 16);
-    float k_scale = 1.f, v_log2 = 0.f, v_inv = 1.f;
-    if (kEightBit && meta.z != 0) {
-      k_scale = __uint_as_float(meta.x);
-      const float vs = fmaxf(__uint_as_float(meta.y), kMinValueScale);
-      v_log2 = __log2f(vs);
-      v_inv = __fdividef(1.f, vs);
+    const uint4 scales = ld_shared16(meta_ring + stage * 32);
+    const uint4 there = ld_shared16(meta_ring + stage * 32 + 16);
+    const bool border = key0 + kKeys > unmasked || there.x == 0 || there.y == 0;  // (the same for the whole warp)
+    if (border) {
+      // what a page holds behind the sequence's end may be anything: no weight is not enough
+      const int left = cur.seq.len - key0;
+      if constexpr (kEightBit) {
+        if (lane >= left) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(src + 4096 + lane * 128 + i * 16), "r"(0) : "memory");
+        }
+      } else {
+        if ((lane & 15) >= left) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(src + 4096 + lane * 128 + i * 16), "r"(0) : "memory");
+        }
+      }
+      fence_proxy_async_smem();  // (before the next copy into this stage)
+      __syncwarp();
     }
     // rows of 128 bytes, their 16-byte pieces exchanged by row & 7
-    float s[2][4];
+    float s[kKeys / 8][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-      const uint32_t row = src + (g + 8 * n) * 128;
-      if constexpr (kEightBit) {
+    const uint32_t k_row = src + g * 128;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 w = ld_shared16(row + (((j * 4 + c) ^ g) << 4));
+    for (int j = 0; j < (kEightBit ? 2 : 4); ++j) {
+      const uint32_t at = k_row + (kEightBit ? 0 : (j >> 1) * 2048) + ((((j & 1) * 4 + c) ^ g) << 4);
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n) {
+        const uint4 w = ld_shared16(at + n * 1024);
+        if constexpr (kEightBit) {
           const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) mma_16816_f16(s[n], qf[j * 4 + k], widen_e4m3x2(w4[k]), widen_e4m3x2(w4[k] >> 16));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 w = ld_shared16(row + (j >> 1) * 2048 + ((((j & 1) * 4 + c) ^ g) << 4));
+        } else {
           mma_16816<kHalf>(s[n], qf[j * 2], w.x, w.y);
           mma_16816<kHalf>(s[n], qf[j * 2 + 1], w.z, w.w);
         }
       }
     }
-    // scores of rows g (e = 0, 1) and g + 8 (e = 2, 3), keys key0 + 8 n + 2 c + (e & 1), in units of log2
-    const bool border = key0 + 16 > unmasked || meta.z == 0;  // (the same for the whole warp)
+    // scores of rows g (e = 0, 1) and g + 8 (e = 2, 3), keys key0 + 8 n + 2 c + (e & 1), in units of log2 and shifted
+    float v_inv[kHalves];
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float f = factor[i] * k_scale;
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) s[n][2 * i + e] = fmaf(s[n][2 * i + e], f, v_log2);
-      if (border) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (meta.z == 0 || key0 + 8 * n + 2 * c + e >= limit[i]) s[n][2 * i + e] = -INFINITY;
+    for (int half = 0; half < kHalves; ++half) {
+      float k_scale = 1.f, v_log2 = 0.f;
+      v_inv[half] = 1.f;
+      if constexpr (kEightBit) {
+        k_scale = __uint_as_float(half ? scales.z : scales.x);
+        const float vs = fmaxf(__uint_as_float(half ? scales.w : scales.y), kMinValueScale);
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(v_log2) : "f"(vs));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(v_inv[half]) : "f"(vs));
+        if (border && (half ? there.y : there.x) == 0) {  // (no scales either)
+          k_scale = v_inv[half] = 1.f;
+          v_log2 = 0.f;
+        }
       }
-      top[i] = fmaxf(max3(s[0][2 * i], s[0][2 * i + 1], s[1][2 * i]), s[1][2 * i + 1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float f = factor[i] * k_scale, add = v_log2 + shift[i];
+#pragma unroll
+        for (int n = 2 * half; n < 2 * half + 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[n][2 * i + e] = fmaf(s[n][2 * i + e], f, add);
+        if (border) {
+          asm volatile("" ::: "memory");  // (a branch that is rarely taken, not selections that always are)
+#pragma unroll
+          for (int n = 2 * half; n < 2 * half + 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if ((half ? there.y : there.x) == 0 || key0 + 8 * n + 2 * c + e >= limit[i]) s[n][2 * i + e] = -INFINITY;
+        }
+        top[i] = max3(top[i], max3(s[2 * half][2 * i], s[2 * half][2 * i + 1], s[2 * half + 1][2 * i]), s[2 * half + 1][2 * i + 1]);
+      }
     }
-    if (__any_sync(0xffffffffu, top[0] > m[0] + kRescaleThreshold || top[1] > m[1] + kRescaleThreshold)) {
+    if (__any_sync(0xffffffffu, top[0] > ceiling[0] || top[1] > ceiling[1])) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float t = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-        if (t > m[i] + kRescaleThreshold) {
-          const float f = fast_exp2(m[i] - t);  // (no maximum yet: 0)
-          m[i] = t;
+        if (t > ceiling[i]) {
+          const float down = kProbShift - t;  // the new shift, from the old one
+          const float f = ceiling[i] == -INFINITY ? 0.f : fast_exp2(down);
+          shift[i] += down;
+          ceiling[i] = kTop;
           l[i] *= f;
 #pragma unroll
           for (int tt = 0; tt < 16; ++tt) {
             o[tt][2 * i] *= f;
             o[tt][2 * i + 1] *= f;
           }
+#pragma unroll
+          for (int n = 0; n < kKeys / 8; ++n) {
+            s[n][2 * i] += down;
+            s[n][2 * i + 1] += down;
+          }
         }
       }
     }
-    uint32_t pf[4];
+    uint32_t pf[kHalves][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float shift = m[i] == -INFINITY ? 0.f : kProbShift - m[i];
+    for (int half = 0; half < kHalves; ++half)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float a = fast_exp2(s[n][2 * i] + shift), b = fast_exp2(s[n][2 * i + 1] + shift);
-        l[i] = fmaf(a + b, v_inv, l[i]);
-        pf[n * 2 + i] = pack2<kHalf>(a, b);
+      for (int i = 0; i < 2; ++i) {
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float a = fast_exp2(s[2 * half + n][2 * i]), b = fast_exp2(s[2 * half + n][2 * i + 1]);
+          sum = n == 0 ? a + b : sum + (a + b);
+          pf[half][n * 2 + i] = pack2<kHalf>(a, b);
+        }
+        l[i] = fmaf(sum, v_inv[half], l[i]);
       }
-    }
-    // o += p v: lane's channels 16 g + t, t = 0 .. 15, of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-    const int left = cur.seq.len - key0;
-    constexpr int kPieces = kEightBit ? 1 : 2;
+    // o += p v: lane's channels 16 g + t, t = 0 .. 15, of keys 16 half + 2 c, + 1, + 8, + 9
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      uint4 w[4];
+    for (int half = 0; half < kHalves; ++half)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int key = 2 * c + (n & 1) + (n >> 1) * 8;
-        const uint32_t row = src + (kEightBit ? 2048 : 4096 + (g >> 2) * 2048) + key * 128;
-        w[n] = ld_shared16(row + (((kEightBit ? g : (g & 3) * 2 + j) ^ (key & 7)) << 4));
-        // what the page holds behind the sequence's end may be anything: no weight is not enough
-        if (border && key >= left) w[n] = make_uint4(0, 0, 0, 0);
-      }
+      for (int j = 0; j < (kEightBit ? 1 : 2); ++j) {
+        uint4 w[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t r0 = q == 0 ? w[0].x : q == 1 ? w[0].y : q == 2 ? w[0].z : w[0].w;
-        const uint32_t r1 = q == 0 ? w[1].x : q == 1 ? w[1].y : q == 2 ? w[1].z : w[1].w;
-        const uint32_t r2 = q == 0 ? w[2].x : q == 1 ? w[2].y : q == 2 ? w[2].z : w[2].w;
-        const uint32_t r3 = q == 0 ? w[3].x : q == 1 ? w[3].y : q == 2 ? w[3].z : w[3].w;
-        if constexpr (kEightBit) {
-          const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
-          const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
-          mma_16816_f16(o[4 * q], pf, widen_e4m3x2(lo01), widen_e4m3x2(lo23));
-          mma_16816_f16(o[4 * q + 1], pf, widen_e4m3x2(lo01 >> 16), widen_e4m3x2(lo23 >> 16));
-          mma_16816_f16(o[4 * q + 2], pf, widen_e4m3x2(hi01), widen_e4m3x2(hi23));
-          mma_16816_f16(o[4 * q + 3], pf, widen_e4m3x2(hi01 >> 16), widen_e4m3x2(hi23 >> 16));
-        } else {
-          mma_16816<kHalf>(o[8 * j + 2 * q], pf, __byte_perm(r0, r1, 0x5410), __byte_perm(r2, r3, 0x5410));
-          mma_16816<kHalf>(o[8 * j + 2 * q + 1], pf, __byte_perm(r0, r1, 0x7632), __byte_perm(r2, r3, 0x7632));
+        for (int n = 0; n < 4; ++n) {
+          const int key = 2 * c + (n & 1);  // (+ 8 does not change key & 7)
+          const uint32_t row = src + 4096 + (kEightBit ? 0 : (g >> 2) * 2048) + key * 128 + half * 2048 + (n >> 1) * 1024;
+          w[n] = ld_shared16(row + (((kEightBit ? g : (g & 3) * 2 + j) ^ (key & 7)) << 4));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t r0 = q == 0 ? w[0].x : q == 1 ? w[0].y : q == 2 ? w[0].z : w[0].w;
+          const uint32_t r1 = q == 0 ? w[1].x : q == 1 ? w[1].y : q == 2 ? w[1].z : w[1].w;
+          const uint32_t r2 = q == 0 ? w[2].x : q == 1 ? w[2].y : q == 2 ? w[2].z : w[2].w;
+          const uint32_t r3 = q == 0 ? w[3].x : q == 1 ? w[3].y : q == 2 ? w[3].z : w[3].w;
+          if constexpr (kEightBit) {
+            const uint32_t lo01 = __byte_perm(r0, r1, 0x5140), hi01 = __byte_perm(r0, r1, 0x7362);
+            const uint32_t lo23 = __byte_perm(r2, r3, 0x5140), hi23 = __byte_perm(r2, r3, 0x7362);
+            mma_16816_f16(o[4 * q], pf[half], widen_e4m3x2(lo01), widen_e4m3x2(lo23));
+            mma_16816_f16(o[4 * q + 1], pf[half], widen_e4m3x2(lo01 >> 16), widen_e4m3x2(lo23 >> 16));
+            mma_16816_f16(o[4 * q + 2], pf[half], widen_e4m3x2(hi01), widen_e4m3x2(hi23));
+            mma_16816_f16(o[4 * q + 3], pf[half], widen_e4m3x2(hi01 >> 16), widen_e4m3x2(hi23 >> 16));
+          } else {
+            mma_16816<kHalf>(o[8 * j + 2 * q], pf[half], __byte_perm(r0, r1, 0x5410), __byte_perm(r2, r3, 0x5410));
+            mma_16816<kHalf>(o[8 * j + 2 * q + 1], pf[half], __byte_perm(r0, r1, 0x7632), __byte_perm(r2, r3, 0x7632));
+          }
         }
       }
-    }
     __syncwarp();  // every lane has read the stage
     if (copied < n_steps) copy_step(stage);
     if (++stage == kStages) {
@@ -513,6 +574,9 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       continue;
     }
     // ---- the run leaves this item
+    float m[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) m[i] = ceiling[i] == -INFINITY ? -INFINITY : kProbShift - shift[i];
     rows_join(o, m, l, join_buf, join_stat, warp, lane);
     const long long item_end = item_start + cur.n_tiles;
     const long long c_first = item_start / per, c_last = (item_end - 1) / per;
@@ -607,7 +671,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     }
     if (step + 1 < n_steps) {
       item_start = item_end;
-      cur.next_item(p);
+      cur.next_item<kTile>(p);
       fresh = true;
     }
   }

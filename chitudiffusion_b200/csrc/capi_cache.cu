@@ -105,7 +105,7 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const chit
   cudaError_t e = allow_smem(chitu::attn_cache_rows_kernel<kFp16, kEightBit>, smem, done);
   if (e != cudaSuccess) return e;
   const int64_t items = static_cast<int64_t>(p.batch) * p.heads_kv * ((static_cast<int64_t>(max_q) * p.group + 15) / 16);
-  const int64_t runs = (items * ((max_kv + chitu::kRowsTile - 1) / chitu::kRowsTile) + kRowsMinTiles - 1) / kRowsMinTiles;
+  const int64_t runs = (items * ((max_kv + chitu::RowsShape<kEightBit>::tile - 1) / chitu::RowsShape<kEightBit>::tile) + kRowsMinTiles - 1) / kRowsMinTiles;
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kSms * chitu::RowsShape<kEightBit>::ctas_per_sm, runs)));
   chitu::attn_cache_rows_kernel<kFp16, kEightBit><<<grid, chitu::kRowsThreads, smem, st>>>(tk, tv, p);
   return cudaGetLastError();
@@ -335,7 +335,7 @@ int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, c
   const bool fp16 = dtype == CHITU_DTYPE_FP16, eight = es == 1;
   cudaError_t e;
   const bool tile = takes_tile_kernel(max_q, p.group);
-  const int box = tile ? std::min(cache->page_size, 128) : 16;
+  const int box = std::min(cache->page_size, tile ? 128 : eight ? chitu::RowsShape<true>::keys : chitu::RowsShape<false>::keys);
   CUtensorMap tk, tv;
   if (int rc = make_cache_map(&tk, cache, cache->k, cache->k_strides, box, !(tile && eight), "k_cache")) return rc;
   if (int rc = make_cache_map(&tv, cache, cache->v, cache->v_strides, box, !(tile && eight), "v_cache")) return rc;
