@@ -109,22 +109,22 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
 // item borders, so the warps need no barrier inside a run.
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
-constexpr int kRowsMergeBytes = 16 * 32 * 16;  // one warp's accumulators, or half of two warps'
 template <bool kEightBit>
 struct RowsShape {
   static constexpr int ctas_per_sm = kEightBit ? 3 : 2;
   static constexpr int stages = kEightBit ? 2 : 3;
   static constexpr int keys = kEightBit ? 32 : 16;            // of a warp's step
   static constexpr int tile = keys * kRowsWarps;
-  static constexpr int step_bytes = 8192;                     // keys, then values
+  static constexpr int step_bytes = 8192;                     // keys, then values; also a warp's accumulators
   static constexpr int ring = kRowsWarps * stages * step_bytes;
-  static constexpr int meta_at = ring + kRowsMergeBytes;      // per warp and stage: scales of both halves, whether they have a page
-  static constexpr int stat_at = meta_at + kRowsWarps * stages * 32;
+  static constexpr int meta_at = ring;                        // per warp and stage: scales of both halves, whether they have a page
+  static constexpr int q_at = meta_at + kRowsWarps * stages * 32;  // query fragments: 8 steps of 16 channels, 32 lanes
+  static constexpr int stat_at = q_at + 8 * 32 * 16;
   static constexpr int bar_at = stat_at + kRowsWarps * 16 * 8;
   static constexpr int smem = bar_at + kRowsWarps * stages * 8 + 16 + 1024;
 };
-// scratch of one piece: 16 x 32 float4 of the accumulator's fragments, then (maximum, sum) of 16 rows
-constexpr int kRowsPieceFloats = 16 * 32 * 4 + 32;
+// scratch of one piece: [rows g, rows g + 8][16 accumulators][32 lanes] float2, then (maximum, sum) of 16 rows
+constexpr int kRowsPieceFloats = 2 * 16 * 32 * 2 + 32;
 
 // Position in the order of steps.
 struct RowsCursor {
@@ -207,62 +207,6 @@ __device__ __forceinline__ void rows_load_q(const CacheAttnParams& p, const Rows
   }
 }
 
-// Accumulators of the CTA's warps for one item, brought to a common maximum and summed by warp 0 (others: undefined).
-__device__ __forceinline__ void rows_join(float (&o)[16][4], float (&m)[2], float (&l)[2], float4* buf, float2* stat, int warp, int lane) {
-  const int g = lane >> 2;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if ((lane & 3) == 0) stat[warp * 16 + g + 8 * i] = make_float2(m[i], l[i]);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, stat[w * 16 + g + 8 * i].x);
-#pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) {
-      const float2 s = stat[w * 16 + g + 8 * i];
-      sum += s.x == -INFINITY ? 0.f : s.y * fast_exp2(s.x - top);
-    }
-    const float f = m[i] == -INFINITY ? 0.f : fast_exp2(m[i] - top);
-#pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      o[t][2 * i] *= f;
-      o[t][2 * i + 1] *= f;
-    }
-    m[i] = top;
-    l[i] = sum;
-  }
-  // warps 2 and 3 to 0 and 1, half of the accumulators at a time, then warp 1 to warp 0
-  static_assert(kRowsWarps == 4, "the order below");
-  auto move = [&](int from, int to, int n_warps, int t0, int n) {
-    if (warp >= from && warp < from + n_warps) {
-#pragma unroll
-      for (int t = 0; t < 16; ++t)
-        if (t >= t0 && t < t0 + n) buf[((warp - from) * n + t - t0) * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
-    }
-    __syncthreads();
-    if (warp >= to && warp < to + n_warps) {
-#pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        if (t < t0 || t >= t0 + n) continue;
-        const float4 v = buf[((warp - to) * n + t - t0) * 32 + lane];
-        o[t][0] += v.x;
-        o[t][1] += v.y;
-        o[t][2] += v.z;
-        o[t][3] += v.w;
-      }
-    }
-    __syncthreads();
-  };
-  move(2, 0, 2, 0, 8);
-  move(2, 0, 2, 8, 8);
-  move(1, 0, 1, 0, 16);
-}
-
 template <bool kFp16, bool kEightBit>
 __global__ void __launch_bounds__(kRowsThreads, RowsShape<kEightBit>::ctas_per_sm)
 attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CacheAttnParams p) {
@@ -277,7 +221,6 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   const uint32_t ring = smem_base + warp * kStages * Shape::step_bytes;
   const uint32_t meta_ring = smem_base + Shape::meta_at + warp * kStages * 32;
   const uint32_t bars = smem_base + Shape::bar_at + warp * kStages * 8;
-  float4* join_buf = reinterpret_cast<float4*>(smem + Shape::ring);
   float2* join_stat = reinterpret_cast<float2*>(smem + Shape::stat_at);
   volatile int* last_flag = reinterpret_cast<volatile int*>(smem + Shape::bar_at + kRowsWarps * kStages * 8);
   volatile int* abort_flag = last_flag + 1;
@@ -386,7 +329,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   // A row's probabilities are 2^(score + shift), shift = kProbShift - m; the largest score so far may pass m by kRescaleThreshold
   // before the shift moves.  A row that has seen no key has no limit to pass.
   constexpr float kTop = kProbShift + kRescaleThreshold;
-  uint32_t qf[8][4];
+  const uint32_t q_frag = smem_base + Shape::q_at + lane * 16;
   float factor[2], o[16][4], shift[2], l[2], ceiling[2];
   int limit[2], unmasked = 0;  // keys that a row, that all rows see
   int stage = 0, phase = 0;
@@ -394,7 +337,14 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll 1
   for (int step = 0; step < n_steps; ++step) {
     if (fresh) {
-      rows_load_q<kFp16, kEightBit>(p, cur, g, c, qf, factor);
+      {
+        uint32_t qf[8][4];
+        rows_load_q<kFp16, kEightBit>(p, cur, g, c, qf, factor);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k >> 1 == warp) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(q_frag + k * 512), "r"(qf[k][0]), "r"(qf[k][1]), "r"(qf[k][2]), "r"(qf[k][3]) : "memory");
+        __syncthreads();  // (each warp has written a quarter of the fragments that all of them read)
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = cur.rb * 16 + g + 8 * i;
@@ -444,16 +394,21 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll
     for (int j = 0; j < (kEightBit ? 2 : 4); ++j) {
       const uint32_t at = k_row + (kEightBit ? 0 : (j >> 1) * 2048) + ((((j & 1) * 4 + c) ^ g) << 4);
+      uint4 w[kKeys / 8];
 #pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n) {
-        const uint4 w = ld_shared16(at + n * 1024);
-        if constexpr (kEightBit) {
-          const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
+      for (int n = 0; n < kKeys / 8; ++n) w[n] = ld_shared16(at + n * 1024);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816_f16(s[n], qf[j * 4 + k], widen_e4m3x2(w4[k]), widen_e4m3x2(w4[k] >> 16));
-        } else {
-          mma_16816<kHalf>(s[n], qf[j * 2], w.x, w.y);
-          mma_16816<kHalf>(s[n], qf[j * 2 + 1], w.z, w.w);
+      for (int k = 0; k < (kEightBit ? 4 : 2); ++k) {
+        const uint4 qv = ld_shared16(q_frag + (j * (kEightBit ? 4 : 2) + k) * 512);
+        const uint32_t qf[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+        for (int n = 0; n < kKeys / 8; ++n) {
+          if constexpr (kEightBit) {
+            const uint32_t codes = k == 0 ? w[n].x : k == 1 ? w[n].y : k == 2 ? w[n].z : w[n].w;
+            mma_16816_f16(s[n], qf, widen_e4m3x2(codes), widen_e4m3x2(codes >> 16));
+          } else {
+            mma_16816<kHalf>(s[n], qf, k == 0 ? w[n].x : w[n].z, k == 0 ? w[n].y : w[n].w);
+          }
         }
       }
     }
@@ -562,117 +517,132 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         }
       }
     __syncwarp();  // every lane has read the stage
-    if (copied < n_steps) copy_step(stage);
-    if (++stage == kStages) {
-      stage = 0;
-      phase ^= 1;
-    }
-
-    const bool item_done = cur.tile + 1 == cur.n_tiles;
-    if (!item_done && step + 1 < n_steps) {
-      ++cur.tile;
-      continue;
-    }
-    // ---- the run leaves this item
-    float m[2];
+    const bool leaves = cur.tile + 1 == cur.n_tiles || step + 1 == n_steps;
+    if (leaves) {
+      // The run leaves this item.  The warps' accumulators meet in the stages that the step has just read; warp w sums
+      // accumulators 4 w .. 4 w + 3 of all of them and takes these to the end.
+      const int n_halves = min(cur.seq.n_new * p.group - cur.rb * 16, 16) > 8 ? 2 : 1;  // rows g + 8 in use?
+      const uint32_t mine = src + lane * 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) m[i] = ceiling[i] == -INFINITY ? -INFINITY : kProbShift - shift[i];
-    rows_join(o, m, l, join_buf, join_stat, warp, lane);
-    const long long item_end = item_start + cur.n_tiles;
-    const long long c_first = item_start / per, c_last = (item_end - 1) / per;
-    bool write = warp == 0;
-    if (c_first != c_last) {
-      auto piece = [&](long long cta) {  // an item starts a CTA's run, or is the last of it
-        return p.part + (2 * cta + (item_start > cta * per ? 1 : 0)) * kRowsPieceFloats;
-      };
-      if (warp == 0) {
-        float4* mine = reinterpret_cast<float4*>(piece(blockIdx.x));
+      for (int i = 0; i < 2; ++i) {
+        if (i >= n_halves) break;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) mine[t * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
-        if (c == 0) {
+        for (int t = 0; t < 16; ++t) asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(mine + (i * 16 + t) * 256), "f"(o[t][2 * i]), "f"(o[t][2 * i + 1]) : "memory");
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (c == 0) join_stat[warp * 16 + g + 8 * i] = make_float2(ceiling[i] == -INFINITY ? -INFINITY : kProbShift - shift[i], l[i]);
+      }
+      __syncthreads();
+      float2 r[2][4];
+      float m_row[2] = {-INFINITY, -INFINITY}, l_row[2] = {0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 2; ++i) reinterpret_cast<float2*>(mine + 512)[g + 8 * i] = make_float2(m[i], l[i]);
+      for (int i = 0; i < 2; ++i) {
+        if (i >= n_halves) break;
+        float f[kRowsWarps];
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) m_row[i] = fmaxf(m_row[i], join_stat[w * 16 + g + 8 * i].x);
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) {
+          const float2 st = join_stat[w * 16 + g + 8 * i];
+          f[w] = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m_row[i]);
+          l_row[i] = fmaf(st.y, f[w], l_row[i]);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          r[i][t] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kRowsWarps; ++w) {
+            float x, y;
+            asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x), "=f"(y) : "r"(smem_base + (w * kStages + stage) * Shape::step_bytes + (i * 16 + 4 * warp + t) * 256 + lane * 8) : "memory");
+            r[i][t].x = fmaf(x, f[w], r[i][t].x);
+            r[i][t].y = fmaf(y, f[w], r[i][t].y);
+          }
+        }
+      }
+      fence_proxy_async_smem();  // (before the next copies into these stages)
+      const long long item_end = item_start + cur.n_tiles;
+      const long long c_first = item_start / per, c_last = (item_end - 1) / per;
+      bool write = true;
+      if (c_first == c_last) {
+        __syncthreads();
+      } else {
+        auto piece = [&](long long cta) {  // an item starts a CTA's run, or is the last of it
+          return p.part + (2 * cta + (item_start > cta * per ? 1 : 0)) * kRowsPieceFloats;
+        };
+        float* out_piece = piece(blockIdx.x);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i >= n_halves) break;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) reinterpret_cast<float2*>(out_piece)[(i * 16 + 4 * warp + t) * 32 + lane] = r[i][t];
+          if (warp == 0 && c == 0) reinterpret_cast<float2*>(out_piece + 2048)[g + 8 * i] = make_float2(m_row[i], l_row[i]);
         }
         __threadfence();
-        __syncwarp();
-        if (lane == 0) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
           const int before = atomicAdd(p.count + c_first, 1);
           const int last = before == c_last - c_first;
           if (last) p.count[c_first] = 0;
           __threadfence();
           *last_flag = last;
         }
+        __syncthreads();
+        write = *last_flag != 0;
+        if (write) {
+          const int n_pieces = static_cast<int>(c_last - c_first) + 1;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (i >= n_halves) break;
+            m_row[i] = -INFINITY;
+            l_row[i] = 0.f;
+            for (int k = 0; k < n_pieces; ++k) m_row[i] = fmaxf(m_row[i], __ldcg(reinterpret_cast<const float2*>(piece(c_first + k) + 2048) + g + 8 * i).x);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) r[i][t] = make_float2(0.f, 0.f);
+#pragma unroll 4
+            for (int k = 0; k < n_pieces; ++k) {
+              const float2* from = reinterpret_cast<const float2*>(piece(c_first + k));
+              const float2 st = __ldcg(from + 1024 + g + 8 * i);
+              const float f = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m_row[i]);
+              l_row[i] = fmaf(st.y, f, l_row[i]);
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                const float2 v = __ldcg(from + (i * 16 + 4 * warp + t) * 32 + lane);
+                r[i][t].x = fmaf(v.x, f, r[i][t].x);
+                r[i][t].y = fmaf(v.y, f, r[i][t].y);
+              }
+            }
+          }
+        }
       }
-      __syncthreads();
-      write = *last_flag != 0;
       if (write) {
-        // the warps share the pieces; each keeps its own maximum, and they join as after a run
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          m[i] = -INFINITY;
-          l[i] = 0.f;
-        }
-#pragma unroll
-        for (int t = 0; t < 16; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
-        for (long long i = c_first + warp; i <= c_last; i += kRowsWarps) {
-          const float4* from = reinterpret_cast<const float4*>(piece(i));
-          float2 st[2];
-          float mine[2], theirs[2];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            st[r] = __ldcg(reinterpret_cast<const float2*>(from + 512) + g + 8 * r);
-            const float t = fmaxf(m[r], st[r].x);
-            mine[r] = m[r] == -INFINITY ? 0.f : fast_exp2(m[r] - t);
-            theirs[r] = st[r].x == -INFINITY ? 0.f : fast_exp2(st[r].x - t);
-            m[r] = t;
-            // (summed over the four lanes of a row when the warps join)
-            l[r] = l[r] * mine[r] + (c == 0 ? st[r].y * theirs[r] : 0.f);
-          }
-#pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            const float4 v = __ldcg(from + t * 32 + lane);
-            o[t][0] = o[t][0] * mine[0] + v.x * theirs[0];
-            o[t][1] = o[t][1] * mine[0] + v.y * theirs[0];
-            o[t][2] = o[t][2] * mine[1] + v.z * theirs[1];
-            o[t][3] = o[t][3] * mine[1] + v.w * theirs[1];
-          }
-        }
-        rows_join(o, m, l, join_buf, join_stat, warp, lane);
-        write = warp == 0;
-      } else {
-        __syncthreads();  // (the flag has been read before a later item sets it)
-      }
-    }
-    if (write) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = cur.rb * 16 + g + 8 * i;
-        const int tok = r / p.group, hq = cur.h * p.group + r - tok * p.group;
-        if (tok < cur.seq.n_new) {
-          const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
-          const size_t row = static_cast<size_t>(cur.seq.tok0 + tok);
-          uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          const int row_i = cur.rb * 16 + g + 8 * i;
+          const int tok = row_i / p.group, hq = cur.h * p.group + row_i - tok * p.group;
+          if (i < n_halves && tok < cur.seq.n_new) {
+            const float inv = l_row[i] > 0.f ? 1.f / l_row[i] : 0.f;
+            const size_t row = static_cast<size_t>(cur.seq.tok0 + tok);
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128 + 4 * warp;
             // (accumulator t, column 2 c + e: channel 16 (2 c + e) + t)
-            uint32_t w[8];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) w[t] = pack2<kFp16>(o[2 * t][2 * i + e] * inv, o[2 * t + 1][2 * i + e] * inv);
-            uint4* d = reinterpret_cast<uint4*>(dst + 16 * (2 * c + e));
-            d[0] = make_uint4(w[0], w[1], w[2], w[3]);
-            d[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            *reinterpret_cast<uint2*>(dst + 32 * c) = make_uint2(pack2<kFp16>(r[i][0].x * inv, r[i][1].x * inv), pack2<kFp16>(r[i][2].x * inv, r[i][3].x * inv));
+            *reinterpret_cast<uint2*>(dst + 32 * c + 16) = make_uint2(pack2<kFp16>(r[i][0].y * inv, r[i][1].y * inv), pack2<kFp16>(r[i][2].y * inv, r[i][3].y * inv));
+            if (p.lse != nullptr && warp == 0 && c == 0)
+              p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_row[i] > 0.f ? (m_row[i] - kProbShift + log2f(l_row[i])) * 0.6931471805599453f : -INFINITY;
           }
-          if (p.lse != nullptr && c == 0)
-            p.lse[static_cast<size_t>(hq) * p.tokens + row] = l[i] > 0.f ? (m[i] - kProbShift + log2f(l[i])) * 0.6931471805599453f : -INFINITY;
         }
       }
+      if (step + 1 < n_steps) {
+        item_start = item_end;
+        cur.next_item<kTile>(p);
+        fresh = true;
+      }
+    } else {
+      ++cur.tile;
     }
-    if (step + 1 < n_steps) {
-      item_start = item_end;
-      cur.next_item<kTile>(p);
-      fresh = true;
+    if (copied < n_steps) copy_step(stage);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
     }
   }
   if (*abort_flag && lane == 0) {
