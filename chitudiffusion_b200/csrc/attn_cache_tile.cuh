@@ -9,8 +9,9 @@
 //   warps 8-11       widen e4m3 codes to fp16 in the swizzled layout of the matrix operands (16-bit pages: only clear the rows of
 //                    values behind the sequence's end)
 //   warps 12-14      issue QK^T, PV of tile 0, PV of tile 1
-//   warp  15         tensor copies of pages (a box is a page, or 128 rows of one; page numbers are the outermost coordinate, and
-//                    one outside the pool reads zeros) and the scales of a tile's sixteen-key groups
+//   warp  15         walks the CTA's share of the work and publishes it block by block (TileSeg); tensor copies of pages (a box is a
+//                    page, or 128 rows of one; page numbers are the outermost coordinate, and one outside the pool reads
+//                    zeros) and the scales of a tile's sixteen-key groups
 //
 // Widening costs the SM sub-partitions' issue slots (about 100 instructions per warp and tile) rather than a pass over
 // memory: read back from a 16-bit copy of the cache, three frames over 21 would move 200 MB more.
@@ -18,8 +19,9 @@
 // Work.  A block's share of the work is the keys it sees, K = the last row's, at least one.  All blocks in the order (sequence,
 // key head, block) are a line of such keys; CTA c takes the c-th of gridDim.x equal runs of it, and of a block those
 // 128-key tiles whose first key lies in its run.  So ragged lengths, causal blocks and few long blocks alike finish together.
-// A block that a run's border cuts leaves fp32 pieces in scratch; attn_cache_join_kernel, launched behind, merges them with all
-// SMs (the CTA that comes last would have up to 148 pieces of 128 KB to itself).
+// (Dealing out whole blocks first, so that CTAs walk the same keys at the same time, gained nothing: 790 us against 770 for
+// three frames over 21.)  A block that a run's border cuts leaves fp32 pieces in scratch; attn_cache_join_kernel, launched
+// behind, merges them with all SMs (the CTA that comes last would have up to 148 pieces of 128 KB to itself).
 #pragma once
 
 #include "attn_cache.cuh"
@@ -29,14 +31,23 @@ namespace chitu {
 constexpr int kTileThreads = 512;
 constexpr int kTileRows = 2 * kTileM;    // rows of a block
 constexpr int kCoefStages = 8;           // tiles whose scales are kept: the copies run at most five ahead of the softmax
+constexpr int kSegStages = 8;            // blocks whose description is kept (each has a tile at least)
 template <bool kEightBit>
 struct TileShape {
-  static constexpr int slots = kEightBit ? 3 : 5;       // 16-bit operand tiles, keys and values in turn
-  static constexpr int raw_slots = kEightBit ? 4 : 5;   // as copied (16-bit pages are copied into their operand slot)
+  static constexpr int slots = kEightBit ? 4 : 5;       // 16-bit operand tiles, keys and values in turn
+  static constexpr int raw_slots = kEightBit ? 2 : 5;   // as copied (16-bit pages are copied into their operand slot)
   static constexpr int raw_bytes = kEightBit ? kTileBytes / 2 : 0;
   static constexpr int coef_at = 2 * kTileBytes + slots * kTileBytes + raw_slots * raw_bytes;
   static constexpr int bar_at = coef_at + kCoefStages * 8 * 16;
-  static constexpr int smem = bar_at + 512 + 1024;
+  static constexpr int seg_at = bar_at + 496;
+  static constexpr int smem = seg_at + kSegStages * 48 + 1024;
+};
+// What the join kernel needs to know of a block that begins in a CTA's run and ends behind it.
+struct TileJoin {
+  int n_pieces;          // 0: there is no such block
+  int first;             // where the first piece is; the others are 2 (CTA + 1), 2 (CTA + 2), ...
+  int row, n_rows;       // first packed token, query rows
+  int h, unused[3];
 };
 // scratch of one piece: per tile [32 column groups][128 rows] float4, then (maximum, sum) of 128 rows
 constexpr int kTilePieceFloats = 2 * (32 * kTileM * 4 + 2 * kTileM);
@@ -48,8 +59,18 @@ struct TileBlock {
   long long start;     // first key on the line
   SeqInfo seq;
 };
+// What the warps of a CTA need to know of a block that they work on.
+struct TileSeg {
+  int n;                        // its key tiles t0 ... t0 + n - 1; 0: there is no more work
+  int t0;
+  int tok0, n_new, len, first;  // of the sequence
+  int h, blk, rows;             // key head, block, query rows
+  int piece;                    // where its fp32 piece goes, -1: the result itself
+  int unused[2];
+};
+static_assert(sizeof(TileSeg) == 48, "control block");
 struct TileLine {
-  long long total, per;
+  long long total, per;  // keys, keys of a run
 };
 
 // Blocks of a sequence hold whole tokens: tok_blk = 256 / group each.  The blocks' K are first + tok_blk, first + 2 tok_blk, ...,
@@ -95,7 +116,7 @@ __device__ __forceinline__ void tile_next_block(const CacheAttnParams& p, TileBl
   tile_measure(p, w);
 }
 
-// The line's length, by a whole warp.
+// The line, by a whole warp.
 __device__ __forceinline__ TileLine tile_line(const CacheAttnParams& p, int lane, int ctas) {
   TileLine line;
   line.total = 0;
@@ -146,12 +167,21 @@ __device__ __forceinline__ TileBlock tile_locate(const CacheAttnParams& p, int l
   return w;
 }
 
-// A run's blocks one after the other, each with its tiles [t0, t0 + n).
+// The blocks of a CTA's run one after the other, each with its tiles [t0, t0 + n).
 struct TileWalk {
   TileBlock w;
-  long long pos, end;
+  long long lo, end;  // the run
   bool begun;
+  __device__ __forceinline__ void begin(const CacheAttnParams& p, int lane, int cta, int ctas) {
+    const TileLine line = tile_line(p, lane, ctas);
+    lo = cta * line.per;
+    end = min(lo + line.per, line.total);
+    if (lo < end) w = tile_locate(p, lane, lo);
+    begun = false;
+  }
   __device__ __forceinline__ bool next(const CacheAttnParams& p, int& t0, int& n) {
+    if (lo >= end) return false;
+    long long pos = lo;
     while (true) {
       if (begun) {
         pos = w.start + w.keys;
@@ -165,7 +195,6 @@ struct TileWalk {
       if (n > 0) return true;
     }
   }
-  __device__ __forceinline__ int rows(const CacheAttnParams& p) const { return min(p.tok_blk, w.seq.n_new - w.blk * p.tok_blk) * p.group; }
 };
 
 __device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
@@ -175,9 +204,29 @@ __device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
 }
 
 // One softmax step (thread = one row, 128 scores): scores in, probabilities out.  As persist_softmax_step, with a factor and an
-// addend for each sixteen keys (coef: key scale, log2 of the value scale, its inverse) and `valid` keys visible to this row.
-// m is the largest (score factor + addend) so far in log2 units, moved only when it has grown by more than 2^8.
-template <bool kHalf>
+// addend for each sixteen keys (coef: key scale, log2 of the value scale, its inverse) and, in a form of its own that keeps the
+// other one short, `valid` keys visible to this row.  m is the largest (score factor + addend) so far in log2 units, moved only when it has grown by more than 2^8.
+// mbar_wait with its loop in a few instructions: the roles' hot loops share the instruction cache.  As there, a wait ends when
+// the barrier's phase is complete, when another role has given up, or after about a second (2^24 polls of at least 100 cycles).
+__device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n, a;\n\tmov.u32 n, 0;\n"
+      "POLL:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE;\n\t"
+      "ld.volatile.shared.u32 a, [%3];\n\tsetp.ne.u32 q, a, 0;\n\t@q bra DONE;\n\t"
+      "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 16777216;\n\t@q bra POLL;\n"
+      "DONE:\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(smem_u32(const_cast<const int*>(abort_flag)))
+      : "memory");
+  if (ok == 0 && *abort_flag == 0) {
+    *abort_flag = 1;
+    record_status(status, code);
+  }
+  return ok != 0;
+}
+
+template <bool kHalf, bool kMasked>
 __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, bool first, int valid, float row_factor, const float4* coef,
                                                   float& m, float& l_sum, volatile int* abort_flag, int* status) {
   uint32_t s[4][32];
@@ -187,7 +236,7 @@ __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, b
   tc_fence_before_sync();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(r.bar_s_empty);
-  if (__any_sync(0xffffffffu, valid < kTileN)) {
+  if constexpr (kMasked) {
 #pragma unroll
     for (int i = 0; i < 128; ++i)
       if (i >= valid) s[i >> 5][i & 31] = 0xff800000u;  // -inf
@@ -211,7 +260,7 @@ __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, b
   } else {
     const bool need = mx > m + kRescaleThreshold;
     if (__any_sync(0xffffffffu, need)) {
-      mbar_wait(r.bar_pv, (step - 1) & 1, abort_flag, status, kDevTimeoutSoftmax);
+      tile_wait(r.bar_pv, (step - 1) & 1, abort_flag, status, kDevTimeoutSoftmax);
       __syncwarp();
       tc_fence_after_sync();
       const float f = need ? fast_exp2(m - mx) : 1.0f;
@@ -260,7 +309,7 @@ __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, b
     }
     // 64 probabilities done: hand this half to the issuing warp
     if (half == 0) {
-      if (!pv_done) mbar_wait(r.bar_pv, (step - 1) & 1, abort_flag, status, kDevTimeoutSoftmax);
+      if (!pv_done) tile_wait(r.bar_pv, (step - 1) & 1, abort_flag, status, kDevTimeoutSoftmax);
       __syncwarp();  // (lanes may have found out on their own; the store below is the warp's)
       tc_fence_after_sync();
     }
@@ -297,27 +346,16 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   const uint32_t bar_pv = bar_p_full + 32;                // [2]
   const uint32_t bar_s_empty = bar_pv + 16;
   const uint32_t bar_drain = bar_s_empty + 8;             // [3]
-  int* raw_rows = reinterpret_cast<int*>(ctl + 400);      // [kRaw] rows of the copy that exist, -1: no more
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 424);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctl + 428);
-  long long* run = reinterpret_cast<long long*>(ctl + 432);  // first key, end, block start, b | h, blk
-  static_assert(8 * (20 + kCoefStages) + 16 + 16 + 32 + 16 + 8 + 24 <= 400 && kRaw <= 5 && kSlots <= 5, "control block");
+  const uint32_t bar_seg = bar_drain + 24;                // [kSegStages] a block is described
+  const uint32_t bar_seg_empty = bar_seg + 8 * kSegStages;  // [kSegStages] and has been read
+  int* raw_rows = reinterpret_cast<int*>(ctl + 464);       // [kRaw] rows of the copy that exist, -1: no more
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctl + 484);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctl + 488);
+  TileSeg* segs = reinterpret_cast<TileSeg*>(smem_gen + Shape::seg_at);
+  static_assert(8 * (20 + kCoefStages + 2 * kSegStages) + 16 + 16 + 32 + 16 + 8 + 24 <= 464 && kRaw <= 5 && kSlots <= 5, "control block");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    const TileLine line = tile_line(p, lane, gridDim.x);
-    const long long lo = blockIdx.x * line.per, hi = min(lo + line.per, line.total);
-    TileBlock w = {};
-    if (lo < hi) w = tile_locate(p, lane, lo);
-    if (lane == 0) {
-      run[0] = lo;
-      run[1] = hi;
-      run[2] = w.start;
-      run[3] = w.b;
-      run[4] = w.h;
-      run[5] = w.blk;
-    }
-  } else if (threadIdx.x == 32) {
+  if (threadIdx.x == 32) {
     *abort_flag = 0;
     for (int s = 0; s < kRaw; ++s) {
       mbar_init(bar_raw_full + 8 * s, 1);
@@ -328,6 +366,10 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       mbar_init(bar_kv_empty + 8 * s, 2);
     }
     for (int s = 0; s < kCoefStages; ++s) mbar_init(bar_coef + 8 * s, 1);
+    for (int s = 0; s < kSegStages; ++s) {
+      mbar_init(bar_seg + 8 * s, 1);
+      mbar_init(bar_seg_empty + 8 * s, 11);  // the issuing and the softmax warps
+    }
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar_q_ready + 8 * t, kTileM);
       mbar_init(bar_s_full + 8 * t, 1);
@@ -351,22 +393,19 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  TileWalk walk;
-  walk.pos = run[0];
-  walk.end = run[1];
-  const bool busy = walk.pos < walk.end;  // (else the line is shorter than the grid)
-  walk.begun = false;
-  walk.w.start = run[2];
-  walk.w.b = static_cast<int>(run[3]);
-  walk.w.h = static_cast<int>(run[4]);
-  walk.w.blk = static_cast<int>(run[5]);
-  if (busy) {
-    walk.w.seq = seq_info(p, walk.w.b);
-    walk.w.n_blk = tile_blocks(p, walk.w.seq);
-    tile_measure(p, walk.w);
-  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int n_segs = 0;  // blocks that this warp has taken up
+  // the next of them (n 0: there is none; the warp decides as one)
+  auto next_seg = [&](TileSeg& seg) {
+    const int e = n_segs % kSegStages;
+    if (!__all_sync(0xffffffffu, tile_wait(bar_seg + 8 * e, (n_segs / kSegStages) & 1, abort_flag, p.status, kDevTimeoutMma))) return false;
+    ++n_segs;
+    seg = segs[e];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_seg_empty + 8 * e);
+    return seg.n > 0;
+  };
 
-  int t0, n;
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 15) {
@@ -375,13 +414,39 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       const int boxes = kTileN >> box_shift;
       int slot = 0, phase = 0, tiles = 0;  // ring position, tiles so far
       bool given_up = false;
+      TileWalk walk;
+      TileJoin join = {};
+      walk.begin(p, lane, blockIdx.x, gridDim.x);
+      int t0, n;
       auto page_of = [&](int tile) {  // lane l < boxes: the page of the tile's l-th box, -1 where there is none
         const int key = tile * kTileN + (lane << box_shift);
         if (lane >= boxes || key >= walk.w.seq.len) return -1;
         const int id = __ldg(p.block_table + walk.w.b * p.table_stride + (key >> p.page_shift));
         return id >= 0 && id < p.n_pages ? id : -1;
       };
-      while (busy && !given_up && walk.next(p, t0, n)) {
+      while (!given_up && walk.next(p, t0, n)) {
+        tile_wait(bar_seg_empty + 8 * (n_segs % kSegStages), (n_segs / kSegStages & 1) ^ 1, abort_flag, p.status, kDevTimeoutLoad);
+        if (lane == 0) {
+          TileSeg& seg = segs[n_segs % kSegStages];
+          const TileBlock& w = walk.w;
+          seg.n = n;
+          seg.t0 = t0;
+          seg.tok0 = w.seq.tok0;
+          seg.n_new = w.seq.n_new;
+          seg.len = w.seq.len;
+          seg.first = w.seq.first;
+          seg.h = w.h;
+          seg.blk = w.blk;
+          seg.rows = min(p.tok_blk, w.seq.n_new - w.blk * p.tok_blk) * p.group;
+          seg.piece = n == w.n_tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (w.start > walk.lo ? 1 : 0);
+          if (w.start >= walk.lo && n < w.n_tiles) {
+            const long long last_tile = w.start + static_cast<long long>(w.n_tiles - 1) * kTileN;
+            const long long per = walk.end - walk.lo;  // (a run that a block outlasts is a whole one)
+            join = {static_cast<int>(last_tile / per) - static_cast<int>(blockIdx.x) + 1, seg.piece, seg.tok0 + w.blk * p.tok_blk, seg.rows, w.h, {}};
+          }
+          mbar_arrive(bar_seg + 8 * (n_segs % kSegStages));
+        }
+        ++n_segs;
         int page = page_of(t0);
         for (int j = 0; j < n && !given_up; ++j, ++tiles) {
           const int tile = t0 + j;
@@ -402,7 +467,7 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             if (lane == 0) mbar_arrive(bar_coef + 8 * (tiles % kCoefStages));
           }
           for (int kv = 0; kv < 2; ++kv) {
-            const bool ok = mbar_wait((kEightBit ? bar_raw_empty : bar_kv_empty) + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutLoad);
+            const bool ok = tile_wait((kEightBit ? bar_raw_empty : bar_kv_empty) + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutLoad);
             given_up = given_up || !__all_sync(0xffffffffu, ok);
             const uint32_t bar = bar_raw_full + 8 * slot;
             if (lane == 0) {
@@ -430,8 +495,14 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           page = next_page;
         }
       }
-      // no more: the widening warps go home
-      mbar_wait((kEightBit ? bar_raw_empty : bar_kv_empty) + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutLoad);
+      // no more: everybody goes home
+      tile_wait(bar_seg_empty + 8 * (n_segs % kSegStages), (n_segs / kSegStages & 1) ^ 1, abort_flag, p.status, kDevTimeoutLoad);
+      if (lane == 0) {
+        reinterpret_cast<TileJoin*>(p.part + 2ll * gridDim.x * kTilePieceFloats)[blockIdx.x] = join;
+        segs[n_segs % kSegStages].n = 0;
+        mbar_arrive(bar_seg + 8 * (n_segs % kSegStages));
+      }
+      tile_wait((kEightBit ? bar_raw_empty : bar_kv_empty) + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutLoad);
       if (lane == 0) {
         raw_rows[slot] = -1;
         mbar_arrive(bar_raw_full + 8 * slot);
@@ -459,17 +530,18 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         const uint64_t q_desc0 = umma_smem_desc_sw128(q_smem, 16, 1024);
         const uint64_t k_desc0 = umma_smem_desc_sw128(kv_smem, 16, 1024);
         int q_uses[2] = {0, 0}, scores = 0;
-        while (busy && walk.next(p, t0, n)) {
-          const int n_qt = walk.rows(p) > kTileM ? 2 : 1;
+        TileSeg seg;
+        while (next_seg(seg)) {
+          const int n = seg.n, n_qt = seg.rows > kTileM ? 2 : 1;
           for (int j = 0; j < n; ++j) {
-            mbar_wait(bar_kv_full + 8 * slot, phase, abort_flag, p.status, kDevTimeoutMma);
+            tile_wait(bar_kv_full + 8 * slot, phase, abort_flag, p.status, kDevTimeoutMma);
             for (int t = 0; t < n_qt; ++t) {
               if (j == 0) {
-                mbar_wait(bar_q_ready + 8 * t, q_uses[t] & 1, abort_flag, p.status, kDevTimeoutMma);
+                tile_wait(bar_q_ready + 8 * t, q_uses[t] & 1, abort_flag, p.status, kDevTimeoutMma);
                 ++q_uses[t];
               }
               // the columns of the scores are free once the softmax warps have the previous ones in registers
-              if (scores > 0) mbar_wait(bar_s_empty, (scores - 1) & 1, abort_flag, p.status, kDevTimeoutMma);
+              if (scores > 0) tile_wait(bar_s_empty, (scores - 1) & 1, abort_flag, p.status, kDevTimeoutMma);
               ++scores;
               __syncwarp();
               tc_fence_after_sync();
@@ -501,14 +573,15 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         const uint32_t t_p = tmem_base + kTileN + t * 64;
         const uint32_t t_o = tmem_base + 2 * kTileN + t * kHeadDim;
         int steps = 0;  // the tile's steps so far
-        while (busy && walk.next(p, t0, n)) {
-          const int n_qt = walk.rows(p) > kTileM ? 2 : 1;
+        TileSeg seg;
+        while (next_seg(seg)) {
+          const int n = seg.n, n_qt = seg.rows > kTileM ? 2 : 1;
           for (int j = 0; j < n; ++j) {
-            mbar_wait(bar_kv_full + 8 * slot, phase, abort_flag, p.status, kDevTimeoutMma);
+            tile_wait(bar_kv_full + 8 * slot, phase, abort_flag, p.status, kDevTimeoutMma);
             if (t < n_qt) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                mbar_wait(bar_p_full + 16 * t + 8 * h, steps & 1, abort_flag, p.status, kDevTimeoutMma);
+                tile_wait(bar_p_full + 16 * t + 8 * h, steps & 1, abort_flag, p.status, kDevTimeoutMma);
                 __syncwarp();
                 tc_fence_after_sync();
                 if (leader) {
@@ -544,12 +617,12 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     int slot = 0, phase = 0, raw = 0, raw_phase = 0;
     bool values = false;
     while (true) {
-      bool ok = mbar_wait(bar_raw_full + 8 * raw, raw_phase, abort_flag, p.status, kDevTimeoutMma);
+      bool ok = tile_wait(bar_raw_full + 8 * raw, raw_phase, abort_flag, p.status, kDevTimeoutMma);
       if (!__all_sync(0xffffffffu, ok)) break;
       const int rows = reinterpret_cast<volatile int*>(raw_rows)[raw];
       if (rows < 0) break;
       if constexpr (kEightBit) {
-        ok = mbar_wait(bar_kv_empty + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutMma);
+        ok = tile_wait(bar_kv_empty + 8 * slot, phase ^ 1, abort_flag, p.status, kDevTimeoutMma);
         if (!__all_sync(0xffffffffu, ok)) break;
         // thread: channels 16 c .. 16 c + 15 of rows r, r + 16, ...; two 16-byte pieces of a swizzled row, the second panel's
         // threads in the other order (a quarter warp then covers all banks)
@@ -558,14 +631,19 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         const uint32_t to = kv_smem + slot * kTileBytes + (c >> 2) * kHalfTileBytes + r * 128;
         const int sw = r & 7, first = c >> 2;
         const uint32_t at0 = to + ((((c & 3) * 2 + first) ^ sw) << 4), at1 = to + ((((c & 3) * 2 + 1 - first) ^ sw) << 4);
-#pragma unroll
+        if (values && rows < kTileN) {
+          // what the page holds behind the sequence's end may be anything: no weight is not enough
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i)
+            if (r + i * 16 >= rows) asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(from + i * 2048), "r"(0) : "memory");
+        }
+#pragma unroll 1  // (the hot loops of all roles together should stay in the instruction cache: unrolled, 3 % slower)
         for (int half = 0; half < 2; ++half) {
           uint4 w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = ld_shared16(from + (half * 4 + i) * 2048);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (values && r + (half * 4 + i) * 16 >= rows) w[i] = make_uint4(0, 0, 0, 0);
             const uint32_t a0 = first ? w[i].z : w[i].x, a1 = first ? w[i].w : w[i].y;
             const uint32_t b0 = first ? w[i].x : w[i].z, b1 = first ? w[i].y : w[i].w;
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at0 + (half * 4 + i) * 2048), "r"(widen_e4m3x2(a0)),
@@ -577,7 +655,6 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           }
         }
       } else if (values && rows < kTileN) {
-        // what the page holds behind the sequence's end may be anything: no weight is not enough
         const uint32_t to = kv_smem + raw * kTileBytes + tid * 128;
         if (tid >= rows) {
 #pragma unroll
@@ -613,23 +690,28 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     const TileRefs refs{tmem_base + lane_base, tmem_base + lane_base + kTileN + t * 64, t_o, bar_s_empty, bar_p_full + 16 * t, bar_pv + 8 * t};
     uint8_t* q_row = smem_gen + t * kTileBytes + row_in_tile * 128;
     int steps = 0, tiles = 0;  // this tile's steps, the CTA's key tiles so far
-    while (busy && walk.next(p, t0, n)) {
-      const TileBlock& w = walk.w;
-      if (t * kTileM >= walk.rows(p)) {
-        tiles += n;
-        continue;
-      }
+    // A block's queries are fetched before the previous block's result is written, so that its first scores are formed
+    // meanwhile.
+    bool held = false;  // a result waits in tensor memory: the row's
+    bool live = false;
+    int row = 0, hq = 0, piece = 0;
+    float m = -INFINITY, l_sum = 0.f;
+    while (true) {
+      TileSeg seg;
+      bool more;
+      while ((more = next_seg(seg)) && t * kTileM >= seg.rows) tiles += seg.n;
       const int r = t * kTileM + row_in_tile;
-      const int in_blk = r / p.group;
-      const int tok = w.blk * p.tok_blk + in_blk, hq = w.h * p.group + r - in_blk * p.group;
-      const bool live = in_blk < p.tok_blk && tok < w.seq.n_new;
-      // the row to shared memory: the last QK^T that read this tile's rows is complete (its scores have been waited for)
+      const int in_blk = more ? r / p.group : 0;
+      const int tok = seg.blk * p.tok_blk + in_blk;
+      const int next_row = seg.tok0 + tok, next_hq = seg.h * p.group + r - in_blk * p.group;
+      const bool next_live = more && r < seg.rows;
       float row_factor = p.scale_log2;
-      {
+      if (more) {
+        // the row to shared memory: the last QK^T that read this tile's rows is complete (its scores have been waited for)
         uint4 v[16];
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (w.seq.tok0 + tok) * p.q_token + hq * p.q_head);
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + next_row * p.q_token + next_hq * p.q_head);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 16; ++i) v[i] = next_live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
         if constexpr (kEightBit && !kFp16) {
           uint32_t* x = reinterpret_cast<uint32_t*>(v);
           float top = 0.f;
@@ -646,64 +728,76 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         fence_proxy_async_smem();
         mbar_arrive(bar_q_ready + 8 * t);
       }
-      const int limit = live && p.causal ? min(w.seq.first + tok + 1, w.seq.len) : w.seq.len;
-      float m = -INFINITY, l_sum = 0.f;
-      for (int j = 0; j < n; ++j, ++steps, ++tiles) {
-        mbar_wait(bar_s_full + 8 * t, steps & 1, abort_flag, p.status, kDevTimeoutSoftmax);
-        // (complete by now, and only now its own phase: warps without rows in a block run ahead of the copies)
-        mbar_wait(bar_coef + 8 * (tiles % kCoefStages), (tiles / kCoefStages) & 1, abort_flag, p.status, kDevTimeoutSoftmax);
+      if (held) {
+        tile_wait(bar_pv + 8 * t, (steps - 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
         __syncwarp();
         tc_fence_after_sync();
-        tile_softmax_step<kHalf>(refs, steps, j == 0, limit - (t0 + j) * kTileN, row_factor, coef_ring + (tiles % kCoefStages) * 8, m, l_sum,
-                                 abort_flag, p.status);
-      }
-      mbar_wait(bar_pv + 8 * t, (steps - 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue);
-      __syncwarp();
-      tc_fence_after_sync();
-      if (n == w.n_tiles) {
-        const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
-        const size_t row = static_cast<size_t>(w.seq.tok0 + tok);
-        uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128;
+        if (piece < 0) {
+          const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+          uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + c * 32, o);
-          tmem_wait_ld();
-          if (live) {
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o + c * 32, o);
+            tmem_wait_ld();
+            if (live) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t v[8];
+              for (int h = 0; h < 2; ++h) {
+                uint32_t v[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = pack2<kFp16>(__uint_as_float(o[16 * h + 2 * i]) * inv, __uint_as_float(o[16 * h + 2 * i + 1]) * inv);
-              if (p.out_aligned32) {
-                st_global32(dst + c * 32 + h * 16, v);
-              } else {
-                uint4* d = reinterpret_cast<uint4*>(dst + c * 32 + h * 16);
-                d[0] = make_uint4(v[0], v[1], v[2], v[3]);
-                d[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                for (int i = 0; i < 8; ++i) v[i] = pack2<kFp16>(__uint_as_float(o[16 * h + 2 * i]) * inv, __uint_as_float(o[16 * h + 2 * i + 1]) * inv);
+                if (p.out_aligned32) {
+                  st_global32(dst + c * 32 + h * 16, v);
+                } else {
+                  uint4* d = reinterpret_cast<uint4*>(dst + c * 32 + h * 16);
+                  d[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                  d[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                }
               }
             }
+            __syncwarp();
           }
-          __syncwarp();
-        }
-        if (live && p.lse != nullptr)
-          p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_sum > 0.f ? (m - kProbShift + log2f(l_sum)) * 0.6931471805599453f : -INFINITY;
-      } else {
-        // a piece: rows as they are, the maximum and the sum with them
-        float* piece = p.part + (2 * static_cast<long long>(blockIdx.x) + (w.start > run[0] ? 1 : 0)) * kTilePieceFloats + t * (kTilePieceFloats / 2);
-        float4* mine = reinterpret_cast<float4*>(piece) + row_in_tile;
+          if (live && p.lse != nullptr)
+            p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_sum > 0.f ? (m - kProbShift + log2f(l_sum)) * 0.6931471805599453f : -INFINITY;
+        } else {
+          // a piece: rows as they are, the maximum and the sum with them
+          float* to = p.part + static_cast<long long>(piece) * kTilePieceFloats + t * (kTilePieceFloats / 2);
+          float4* mine = reinterpret_cast<float4*>(to) + row_in_tile;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + c * 32, o);
-          tmem_wait_ld();
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o + c * 32, o);
+            tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            mine[(c * 8 + (i >> 2)) * kTileM] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+            for (int i = 0; i < 32; i += 4)
+              mine[(c * 8 + (i >> 2)) * kTileM] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+          }
+          reinterpret_cast<float2*>(to + 32 * kTileM * 4)[row_in_tile] = make_float2(m, l_sum);
         }
-        reinterpret_cast<float2*>(piece + 32 * kTileM * 4)[row_in_tile] = make_float2(m, l_sum);
+        tc_fence_before_sync();
       }
-      tc_fence_before_sync();
+      if (!more) break;
+      held = true;
+      live = next_live;
+      row = next_row;
+      hq = next_hq;
+      piece = seg.piece;
+      // keys visible to the row, from the block's first tile on
+      int left = (live && p.causal ? min(seg.first + tok + 1, seg.len) : seg.len) - seg.t0 * kTileN;
+      m = -INFINITY;
+      l_sum = 0.f;
+      for (int j = 0; j < seg.n; ++j, ++steps, ++tiles, left -= kTileN) {
+        tile_wait(bar_s_full + 8 * t, steps & 1, abort_flag, p.status, kDevTimeoutSoftmax);
+        // (complete by now, and only now its own phase: warps without rows in a block run ahead of the copies)
+        tile_wait(bar_coef + 8 * (tiles % kCoefStages), (tiles / kCoefStages) & 1, abort_flag, p.status, kDevTimeoutSoftmax);
+        __syncwarp();
+        tc_fence_after_sync();
+        const float4* coef = coef_ring + (tiles % kCoefStages) * 8;
+        if (__any_sync(0xffffffffu, left < kTileN))
+          tile_softmax_step<kHalf, true>(refs, steps, j == 0, left, row_factor, coef, m, l_sum, abort_flag, p.status);
+        else
+          tile_softmax_step<kHalf, false>(refs, steps, j == 0, left, row_factor, coef, m, l_sum, abort_flag, p.status);
+      }
     }
   }
 
@@ -716,32 +810,28 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 }
 
 // Merges the pieces of the blocks that runs' borders have cut: blockIdx.x is the run in which a block begins (at most one block
-// begins in a run and ends behind it), blockIdx.y a group of 32 rows.  Eight warps, 16 channels each; a lane is a row.
+// begins in a run and ends behind it), blockIdx.y a group of 32 rows.  Eight warps, 16 channels each; a lane is a row.  Launched
+// while attn_cache_tile_kernel still runs; its CTAs come to the SMs that have finished.
 template <bool kFp16>
 __global__ void __launch_bounds__(256)
 attn_cache_join_kernel(const __grid_constant__ CacheAttnParams p, int ctas) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TileLine line = tile_line(p, lane, ctas);
-  const long long lo = blockIdx.x * line.per, border = lo + line.per;
-  if (border >= line.total) return;
-  const TileBlock w = tile_locate(p, lane, border - 1);
-  const long long last_tile = w.start + static_cast<long long>(w.n_tiles - 1) * kTileN;
-  if (w.start < lo || last_tile < border) return;
-  const int n_pieces = static_cast<int>(last_tile / line.per - blockIdx.x) + 1;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4* at = reinterpret_cast<const int4*>(reinterpret_cast<const TileJoin*>(p.part + 2ll * ctas * kTilePieceFloats) + blockIdx.x);
+  const int4 d0 = __ldcg(at), d1 = __ldcg(at + 1);
+  const TileJoin join = {d0.x, d0.y, d0.z, d0.w, d1.x, {}};
   const int r = blockIdx.y * 32 + lane;
-  const int in_blk = r / p.group;
-  const int tok = w.blk * p.tok_blk + in_blk, hq = w.h * p.group + r - in_blk * p.group;
-  const bool live = in_blk < p.tok_blk && tok < w.seq.n_new;
-  if (!__any_sync(0xffffffffu, live)) return;
+  const bool live = r < join.n_rows;
+  if (join.n_pieces == 0 || !__any_sync(0xffffffffu, live)) return;
+  const int in_blk = r / p.group, hq = join.h * p.group + r - in_blk * p.group;
   const int t = r >> 7, row_in_tile = r & 127;
-  auto piece = [&](int i) {  // the first may begin inside its run, the others begin theirs
-    return p.part + (2 * static_cast<long long>(blockIdx.x + i) + (i == 0 && w.start > lo ? 1 : 0)) * kTilePieceFloats + t * (kTilePieceFloats / 2);
-  };
+  const float* part = p.part + t * (kTilePieceFloats / 2);
   float m = -INFINITY, l = 0.f, o[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = 0.f;
-  for (int i = 0; i < n_pieces; ++i) {
-    const float* from = piece(i);
+#pragma unroll 2
+  for (int i = 0; i < join.n_pieces; ++i) {
+    const float* from = part + static_cast<long long>(i == 0 ? join.first : 2 * (blockIdx.x + i)) * kTilePieceFloats;
     const float2 st = __ldcg(reinterpret_cast<const float2*>(from + 32 * kTileM * 4) + row_in_tile);
     const float4* src = reinterpret_cast<const float4*>(from) + warp * 4 * kTileM + row_in_tile;
     float4 v[4];
@@ -761,7 +851,7 @@ attn_cache_join_kernel(const __grid_constant__ CacheAttnParams p, int ctas) {
   }
   if (!live) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  const size_t row = static_cast<size_t>(w.seq.tok0 + tok);
+  const size_t row = static_cast<size_t>(join.row + in_blk);
   uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128 + warp * 16;
   uint32_t v[8];
 #pragma unroll

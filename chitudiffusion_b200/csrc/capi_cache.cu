@@ -115,7 +115,7 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const chit
 // more would have it read the cache once per 16 rows.
 bool takes_tile_kernel(int max_q, int group) { return static_cast<int64_t>(max_q) * group > 16 && group <= 128; }
 constexpr int kTileMinTiles = 2;
-int64_t tile_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kSms) * 2 * chitu::kTilePieceFloats * 4; }
+int64_t tile_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kSms) * (2 * chitu::kTilePieceFloats * 4 + sizeof(chitu::TileJoin)); }
 
 template <bool kFp16, bool kEightBit>
 cudaError_t launch_tile(const CUtensorMap& tk, const CUtensorMap& tv, const chitu::CacheAttnParams& p, cudaStream_t st) {
@@ -126,8 +126,16 @@ cudaError_t launch_tile(const CUtensorMap& tk, const CUtensorMap& tv, const chit
   chitu::attn_cache_tile_kernel<kFp16, kEightBit><<<kSms, chitu::kTileThreads, smem, st>>>(tk, tv, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  chitu::attn_cache_join_kernel<kFp16><<<dim3(kSms - 1, chitu::kTileRows / 32), 256, 0, st>>>(p, kSms);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSms - 1, chitu::kTileRows / 32);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, chitu::attn_cache_join_kernel<kFp16>, p, kSms);
 }
 
 }  // namespace

@@ -390,25 +390,27 @@ def test_two_streams_at_once(new):
             assert torch.equal(o[:T], got[0][:T])
 
 
-def test_two_captured_graphs_and_eager_calls_between():
-    """A captured step is replayed with lengths that grow in place, beside another graph and eager calls of the same stream."""
+@pytest.mark.parametrize("n", [1, 9])
+def test_two_captured_graphs_and_eager_calls_between(n):
+    """A captured step of n tokens is replayed with lengths that grow in place, beside another graph and eager calls of the
+    same stream."""
     ops = _ops()
     gen = torch.Generator().manual_seed(8)
     heads, group, page, B = 2, 4, 16, 3
     table = torch.randperm(B * 8, generator=gen).int().view(B, 8)
     rope = model.rope_table(128, 200)
-    cu = torch.arange(B + 1, dtype=torch.int32)
+    cu = n * torch.arange(B + 1, dtype=torch.int32)
     dev_table, dev_cu, dev_rope = table.cuda(), cu.cuda(), rope.cuda()
     graphs = []
     for i in range(2):
         caches = [model.make_cache(gen, B * 8, page, heads, BF16, True) for _ in range(2)]
         lens = torch.tensor([20, 37, 64], dtype=torch.int32)
-        s = dict(k=torch.zeros(B, heads, 128, dtype=BF16).cuda(), v=torch.zeros(B, heads, 128, dtype=BF16).cuda(),
-                 q=torch.zeros(B, heads * group, 128, dtype=BF16).cuda(), lens=lens.cuda(), caches=caches,
+        s = dict(k=torch.zeros(B * n, heads, 128, dtype=BF16).cuda(), v=torch.zeros(B * n, heads, 128, dtype=BF16).cuda(),
+                 q=torch.zeros(B * n, heads * group, 128, dtype=BF16).cuda(), lens=lens.cuda(), caches=caches,
                  dev=[(c.cuda(), sc.cuda()) for c, sc in caches], host_lens=lens)
 
         def step(s=s):
-            s["lens"] += 1
+            s["lens"] += n
             (kc, ks), (vc, vs) = s["dev"]
             qr = ops.kv_cache_append(s["k"], s["v"], kc, vc, dev_table, s["lens"], dev_cu, k_scale=ks, v_scale=vs, rope_table=dev_rope, q=s["q"])
             return ops.attn_fwd_cache(qr, kc, vc, dev_table, s["lens"], dev_cu, k_scale=ks, v_scale=vs, causal=True, return_lse=True)
@@ -419,8 +421,8 @@ def test_two_captured_graphs_and_eager_calls_between():
         graphs.append((graph, s, step))
     for turn in range(6):
         for i, (graph, s, step) in enumerate(graphs):
-            k, v = (torch.randn(B, heads, 128, generator=gen).to(BF16) for _ in range(2))
-            q = torch.randn(B, heads * group, 128, generator=gen).to(BF16)
+            k, v = (torch.randn(B * n, heads, 128, generator=gen).to(BF16) for _ in range(2))
+            q = torch.randn(B * n, heads * group, 128, generator=gen).to(BF16)
             for name, t in (("k", k), ("v", v), ("q", q)):
                 s[name].copy_(t)
             if (turn + i) % 3 == 2:
@@ -428,8 +430,8 @@ def test_two_captured_graphs_and_eager_calls_between():
             else:
                 graph.replay()
                 out, lse = s["out"], s["lse"]
-            s["host_lens"] = s["host_lens"] + 1
-            pos = s["host_lens"].long() - 1
+            s["host_lens"] = s["host_lens"] + n
+            pos = (s["host_lens"].long()[:, None] + torch.arange(-n, 0)).flatten()
             for (c, sc), x in zip(s["caches"], (model.rotate(k, pos, rope, True), v.float())):
                 model.append(x, c, sc, table, s["host_lens"], cu)
             for (c, sc), (gc, gs) in zip(s["caches"], s["dev"]):
