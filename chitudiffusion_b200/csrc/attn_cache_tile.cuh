@@ -16,9 +16,10 @@
 // Widening costs the SM sub-partitions' issue slots (about 100 instructions per warp and tile) rather than a pass over
 // memory: read back from a 16-bit copy of the cache, three frames over 21 would move 200 MB more.
 //
-// Work.  A block's share of the work is the keys it sees, K = the last row's, at least one.  All blocks in the order (sequence,
+// Work.  A block's share of the work is the keys it sees, K = the last row's, and kBlockKeys for what a block costs besides (its
+// queries, the first scores, its result).  All blocks in the order (sequence,
 // key head, block) are a line of such keys; CTA c takes the c-th of gridDim.x equal runs of it, and of a block those
-// 128-key tiles whose first key lies in its run.  So ragged lengths, causal blocks and few long blocks alike finish together.
+// 128-key tiles whose first key (behind the block's kBlockKeys) lies in its run.  So ragged lengths, causal blocks and few long blocks alike finish together.
 // (Dealing out whole blocks first, so that CTAs walk the same keys at the same time, gained nothing: 790 us against 770 for
 // three frames over 21.)  A block that a run's border cuts leaves fp32 pieces in scratch; attn_cache_join_kernel, launched
 // behind, merges them with all SMs (the CTA that comes last would have up to 148 pieces of 128 KB to itself).
@@ -42,7 +43,7 @@ struct TileShape {
   static constexpr int seg_at = bar_at + 496;
   static constexpr int smem = seg_at + kSegStages * 48 + 1024;
 };
-// What the join kernel needs to know of a block that begins in a CTA's run and ends behind it.
+// What the join kernel needs to know of a block whose first tile is in a CTA's run and whose last one is not.
 struct TileJoin {
   int n_pieces;          // 0: there is no such block
   int first;             // where the first piece is; the others are 2 (CTA + 1), 2 (CTA + 2), ...
@@ -55,10 +56,13 @@ constexpr int kTilePieceFloats = 2 * (32 * kTileM * 4 + 2 * kTileM);
 struct TileBlock {
   int b, h, blk;       // sequence, key head, block
   int n_blk;           // blocks of the sequence
-  int keys, n_tiles;   // K of the block
+  int keys, n_tiles;   // K of the block, kBlockKeys included; its tiles
   long long start;     // first key on the line
   SeqInfo seq;
 };
+// (four causal chunks, one to nine blocks a CTA: CTAs end between 125 and 185 us without it)
+constexpr int kBlockKeys = 512;
+
 // What the warps of a CTA need to know of a block that they work on.
 struct TileSeg {
   int n;                        // its key tiles t0 ... t0 + n - 1; 0: there is no more work
@@ -79,15 +83,15 @@ struct TileLine {
 __device__ __forceinline__ bool tile_steps_grow(const CacheAttnParams& p, const SeqInfo& s) { return p.causal && s.first >= 0 && s.len == s.first + s.n_new; }
 __device__ __forceinline__ int tile_blocks(const CacheAttnParams& p, const SeqInfo& s) { return (s.n_new + p.tok_blk - 1) / p.tok_blk; }
 __device__ __forceinline__ int tile_keys(const CacheAttnParams& p, const SeqInfo& s, int blk) {
-  return max(tile_steps_grow(p, s) ? min(s.first + p.tok_blk * (blk + 1), s.len) : s.len, 1);
+  return (tile_steps_grow(p, s) ? min(s.first + p.tok_blk * (blk + 1), s.len) : s.len) + kBlockKeys;
 }
 // keys of blocks [0, blk) of one head
 __device__ __forceinline__ long long tile_keys_before(const CacheAttnParams& p, const SeqInfo& s, int blk, int n_blk) {
-  if (!tile_steps_grow(p, s)) return static_cast<long long>(blk) * max(s.len, 1);
+  if (!tile_steps_grow(p, s)) return static_cast<long long>(blk) * (s.len + kBlockKeys);
   if (n_blk == 0) return 0;
   const long long n = min(blk, n_blk - 1);  // (the last block ends with the sequence)
-  const long long sum = n * s.first + p.tok_blk * (n * (n + 1) / 2);
-  return blk == n_blk ? sum + s.len : sum;
+  const long long sum = n * (s.first + kBlockKeys) + p.tok_blk * (n * (n + 1) / 2);
+  return blk == n_blk ? sum + s.len + kBlockKeys : sum;
 }
 __device__ __forceinline__ long long tile_keys_of(const CacheAttnParams& p, int b) {
   const SeqInfo s = seq_info(p, b);
@@ -97,7 +101,7 @@ __device__ __forceinline__ long long tile_keys_of(const CacheAttnParams& p, int 
 
 __device__ __forceinline__ void tile_measure(const CacheAttnParams& p, TileBlock& w) {
   w.keys = tile_keys(p, w.seq, w.blk);
-  w.n_tiles = (w.keys + kTileN - 1) / kTileN;
+  w.n_tiles = max((w.keys - kBlockKeys + kTileN - 1) / kTileN, 1);
 }
 __device__ __forceinline__ void tile_next_block(const CacheAttnParams& p, TileBlock& w) {
   w.start += w.keys;
@@ -189,9 +193,10 @@ struct TileWalk {
         tile_next_block(p, w);
       }
       begun = true;
-      t0 = static_cast<int>((pos - w.start + kTileN - 1) / kTileN);
-      const long long upto = min(end - w.start, static_cast<long long>(w.keys));
-      n = (upto == w.keys ? w.n_tiles : static_cast<int>((upto + kTileN - 1) / kTileN)) - t0;
+      // (tile i's place on the line: kBlockKeys + 128 i)
+      auto first_at = [](long long at) { return static_cast<int>((max(at - kBlockKeys, 0ll) + kTileN - 1) / kTileN); };
+      t0 = first_at(pos - w.start);
+      n = (end - w.start >= w.keys ? w.n_tiles : end - w.start <= kBlockKeys ? 0 : first_at(end - w.start)) - t0;
       if (n > 0) return true;
     }
   }
@@ -418,11 +423,12 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       TileJoin join = {};
       walk.begin(p, lane, blockIdx.x, gridDim.x);
       int t0, n;
-      auto page_of = [&](int tile) {  // lane l < boxes: the page of the tile's l-th box, -1 where there is none
+      // lane l < boxes: the table's entry for the tile's l-th box, -1 where there is none
+      auto entry = [&](int tile) {
         const int key = tile * kTileN + (lane << box_shift);
-        if (lane >= boxes || key >= walk.w.seq.len) return -1;
-        const int id = __ldg(p.block_table + walk.w.b * p.table_stride + (key >> p.page_shift));
-        return id >= 0 && id < p.n_pages ? id : -1;
+        int id = -1;
+        if (lane < boxes && key < walk.w.seq.len) id = __ldg(p.block_table + walk.w.b * p.table_stride + (key >> p.page_shift));
+        return id;
       };
       while (!given_up && walk.next(p, t0, n)) {
         tile_wait(bar_seg_empty + 8 * (n_segs % kSegStages), (n_segs / kSegStages & 1) ^ 1, abort_flag, p.status, kDevTimeoutLoad);
@@ -439,18 +445,19 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           seg.blk = w.blk;
           seg.rows = min(p.tok_blk, w.seq.n_new - w.blk * p.tok_blk) * p.group;
           seg.piece = n == w.n_tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (w.start > walk.lo ? 1 : 0);
-          if (w.start >= walk.lo && n < w.n_tiles) {
-            const long long last_tile = w.start + static_cast<long long>(w.n_tiles - 1) * kTileN;
+          if (t0 == 0 && n < w.n_tiles) {
+            const long long last_tile = w.start + kBlockKeys + static_cast<long long>(w.n_tiles - 1) * kTileN;
             const long long per = walk.end - walk.lo;  // (a run that a block outlasts is a whole one)
             join = {static_cast<int>(last_tile / per) - static_cast<int>(blockIdx.x) + 1, seg.piece, seg.tok0 + w.blk * p.tok_blk, seg.rows, w.h, {}};
           }
           mbar_arrive(bar_seg + 8 * (n_segs % kSegStages));
         }
         ++n_segs;
-        int page = page_of(t0);
+        int next = entry(t0);
         for (int j = 0; j < n && !given_up; ++j, ++tiles) {
           const int tile = t0 + j;
-          const int next_page = j + 1 < n ? page_of(tile + 1) : -1;
+          const int page = static_cast<unsigned>(next) < static_cast<unsigned>(p.n_pages) ? next : -1;
+          if (j + 1 < n) next = entry(tile + 1);
           // scales of the tile's sixteen-key groups (the entry's last reader is eight tiles back)
           {
             const int from = __shfl_sync(0xffffffffu, page, (lane * 16 >> box_shift) & 31);
@@ -492,7 +499,6 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
               phase ^= 1;
             }
           }
-          page = next_page;
         }
       }
       // no more: everybody goes home
@@ -688,7 +694,6 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t t_o = tmem_base + lane_base + 2 * kTileN + t * kHeadDim;
     const TileRefs refs{tmem_base + lane_base, tmem_base + lane_base + kTileN + t * 64, t_o, bar_s_empty, bar_p_full + 16 * t, bar_pv + 8 * t};
-    uint8_t* q_row = smem_gen + t * kTileBytes + row_in_tile * 128;
     int steps = 0, tiles = 0;  // this tile's steps, the CTA's key tiles so far
     // A block's queries are fetched before the previous block's result is written, so that its first scores are formed
     // meanwhile.
@@ -707,24 +712,36 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       const bool next_live = more && r < seg.rows;
       float row_factor = p.scale_log2;
       if (more) {
-        // the row to shared memory: the last QK^T that read this tile's rows is complete (its scores have been waited for)
+        // The warp's 32 rows to shared memory, two at a time in whole lines (a row per thread was 4096 L1 accesses, 2 us): the last
+        // QK^T that read this tile's rows is complete, its scores have been waited for.
+        const unsigned long long src = next_live ? reinterpret_cast<unsigned long long>(static_cast<const uint16_t*>(p.q) + next_row * p.q_token + next_hq * p.q_head) : 0ull;
+        const int half = lane >> 4, piece16 = lane & 15;
         uint4 v[16];
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + next_row * p.q_token + next_hq * p.q_head);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = next_live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-        if constexpr (kEightBit && !kFp16) {
-          uint32_t* x = reinterpret_cast<uint32_t*>(v);
-          float top = 0.f;
-#pragma unroll
-          for (int i = 0; i < 64; ++i) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(x[i] << 16)), fabsf(__uint_as_float(x[i] & 0xffff0000u))));
-          const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253);
-          const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-          row_factor *= __uint_as_float(static_cast<uint32_t>(e) << 23);
-#pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] = pack2<true>(__uint_as_float(x[i] << 16) * down, __uint_as_float(x[i] & 0xffff0000u) * down);
+        for (int i = 0; i < 16; ++i) {
+          const unsigned long long from = __shfl_sync(0xffffffffu, src, 2 * i + half);
+          v[i] = from != 0ull ? __ldg(reinterpret_cast<const uint4*>(from) + piece16) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) *reinterpret_cast<uint4*>(q_row + (i >> 3) * kHalfTileBytes + (((i & 7) ^ (row_in_tile & 7)) << 4)) = v[i];
+        for (int i = 0; i < 16; ++i) {
+          const int r = quad * 32 + 2 * i + half;
+          if constexpr (kEightBit && !kFp16) {
+            uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            uint32_t top = 0;  // largest magnitude of the row, as bits (they order like the values)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = max(top, max((x[k] << 16) & 0x7fff0000u, x[k] & 0x7fff0000u));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = min(max(static_cast<int>(top >> 23), 1), 253);
+            const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = pack2<true>(__uint_as_float(x[k] << 16) * down, __uint_as_float(x[k] & 0xffff0000u) * down);
+            v[i] = make_uint4(x[0], x[1], x[2], x[3]);
+            const int mine = __shfl_sync(0xffffffffu, e, (lane & 1) * 16);
+            if (lane >> 1 == i) row_factor *= __uint_as_float(static_cast<uint32_t>(mine) << 23);
+          }
+          *reinterpret_cast<uint4*>(smem_gen + t * kTileBytes + (piece16 >> 3) * kHalfTileBytes + r * 128 + (((piece16 & 7) ^ (r & 7)) << 4)) = v[i];
+        }
         fence_proxy_async_smem();
         mbar_arrive(bar_q_ready + 8 * t);
       }
@@ -735,7 +752,7 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         if (piece < 0) {
           const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
           uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t o[32];
             tmem_ld32(t_o + c * 32, o);
@@ -763,7 +780,7 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           // a piece: rows as they are, the maximum and the sum with them
           float* to = p.part + static_cast<long long>(piece) * kTilePieceFloats + t * (kTilePieceFloats / 2);
           float4* mine = reinterpret_cast<float4*>(to) + row_in_tile;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t o[32];
             tmem_ld32(t_o + c * 32, o);
@@ -809,8 +826,8 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   }
 }
 
-// Merges the pieces of the blocks that runs' borders have cut: blockIdx.x is the run in which a block begins (at most one block
-// begins in a run and ends behind it), blockIdx.y a group of 32 rows.  Eight warps, 16 channels each; a lane is a row.  Launched
+// Merges the pieces of the blocks that runs' borders have cut: blockIdx.x is the run that has a block's first tile (of at most one
+// block that ends behind it), blockIdx.y a group of 32 rows.  Eight warps, 16 channels each; a lane is a row.  Launched
 // while attn_cache_tile_kernel still runs; its CTAs come to the SMs that have finished.
 template <bool kFp16>
 __global__ void __launch_bounds__(256)
