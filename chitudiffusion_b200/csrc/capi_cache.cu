@@ -72,6 +72,9 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices]) {
 
 constexpr int kSms = 148;
 
+// Appended tokens per sequence up to which eight threads take all of them (kv_append_few_kernel).
+constexpr int kAppendFew = 4;
+
 // Tensor map over a pool: channels, heads, tokens of a page, pages; a box is 128 bytes of the channels by
 // box_tokens of a page, its rows swizzled (the layout of the matrix operands) or as they are.
 int make_cache_map(CUtensorMap* map, const chitu_b200_kv_cache* c, const void* base, const int64_t* st, int box_tokens, bool swizzled,
@@ -138,6 +141,24 @@ cudaError_t launch_tile(const CUtensorMap& tk, const CUtensorMap& tv, const chit
   return cudaLaunchKernelEx(&cfg, chitu::attn_cache_join_kernel<kFp16>, p, kSms);
 }
 
+template <bool kFp16, bool kEightBit, int kThreads>
+cudaError_t launch_append_of(const chitu::AppendParams& p, dim3 grid, cudaStream_t st) {
+  static bool done[kMaxDevices] = {};
+  constexpr int smem = chitu::AppendShape<kThreads>::smem;
+  cudaError_t e = allow_smem(chitu::kv_append_kernel<kFp16, kEightBit, kThreads>, smem, done);
+  if (e != cudaSuccess) return e;
+  chitu::kv_append_kernel<kFp16, kEightBit, kThreads><<<grid, kThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+template <bool kFp16, bool kEightBit>
+cudaError_t launch_append(const chitu::AppendParams& p, int threads, dim3 grid, cudaStream_t st) {
+  if constexpr (kEightBit) {
+    if (threads == 512) return launch_append_of<kFp16, kEightBit, 512>(p, grid, st);
+    if (threads == 1024) return launch_append_of<kFp16, kEightBit, 1024>(p, grid, st);
+  }
+  return launch_append_of<kFp16, kEightBit, 256>(p, grid, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -154,15 +175,14 @@ int chitu_b200_rotary(const void* const* x, void* const* out, const int64_t* x_s
   if (tokens < 0 || tokens > 0x7fffffff) return fail(CHITU_E_INVALID, "rotary: bad token count");
   const int es = dtype == CHITU_DTYPE_FP32 ? 4 : 2;
   chitu::RotaryParams p;
-  p.n_jobs = n;
-  p.heads_total = 0;
+  int64_t heads_total = 0;
   for (int i = 0; i < n; ++i) {
     if (!x[i] || !out[i] || !aligned16(x[i]) || !aligned16(out[i])) return fail(CHITU_E_INVALID, "rotary: tensor %d null or not 16-byte aligned", i);
-    if (heads[i] < 1) return fail(CHITU_E_INVALID, "rotary: tensor %d has no heads", i);
+    if (heads[i] < 1 || heads[i] > 65535) return fail(CHITU_E_INVALID, "rotary: tensor %d has no heads, or too many", i);
     if (!strides_fit(x_strides + 2 * i, tokens, heads[i], es) || !strides_fit(out_strides + 2 * i, tokens, heads[i], es))
       return fail(CHITU_E_INVALID, "rotary: strides of tensor %d must be positive multiples of 16 bytes", i);
     p.job[i] = {x[i], out[i], x_strides[2 * i], x_strides[2 * i + 1], out_strides[2 * i], out_strides[2 * i + 1], heads[i]};
-    p.heads_total += heads[i];
+    heads_total += heads[i];
   }
   if (tokens == 0) return CHITU_OK;
   p.positions = positions;
@@ -174,10 +194,16 @@ int chitu_b200_rotary(const void* const* x, void* const* out, const int64_t* x_s
   p.rot = rot;
   const int per_block = chitu::kRotaryThreads / (head_dim / 16);
   const int64_t blocks = (tokens + per_block - 1) / per_block;
-  // heads of one thread: as many as leave every SM eight blocks
-  const int64_t chunks = std::min<int64_t>(p.heads_total, std::max<int64_t>(1, (kSms * 8 + blocks - 1) / blocks));
-  p.heads_each = static_cast<int>((p.heads_total + chunks - 1) / chunks);
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((p.heads_total + p.heads_each - 1) / p.heads_each));
+  // heads of one thread: one where that fits the machine at once (three blocks per SM), else as many as then do
+  const int64_t chunks = std::min<int64_t>(heads_total, std::max<int64_t>(1, kSms * 3 / blocks));
+  p.heads_each = static_cast<int>((heads_total + chunks - 1) / chunks);
+  int rows = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (i < n) rows += (heads[i] + p.heads_each - 1) / p.heads_each;
+    p.chunk_end[i] = rows;
+  }
+  if (rows > 65535) return fail(CHITU_E_UNSUPPORTED, "rotary: too many heads for one call");
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(rows));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define CHITU_ROTARY(DT) \
   (interleaved ? chitu::rotary_kernel<DT, true><<<grid, chitu::kRotaryThreads, 0, st>>>(p) \
@@ -254,26 +280,54 @@ int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const 
   p.heads_q = q != nullptr ? q_heads : 0;
   p.page = cache->page_size;
   p.page_shift = page_shift_of(cache->page_size);
-  const int group = 4 * p.page;
-  p.heads_each = std::max(1, 256 / group);
-  const int expected = std::max<int>(1, static_cast<int>(std::min<int64_t>(max_new, tokens)));
-  p.slots = (expected + p.page - 2) / p.page + 1;
-  const int planes = 2 * p.heads_kv + p.heads_q;
-  const int64_t blocks = static_cast<int64_t>(p.batch) * p.slots;
-  const int64_t rows = (planes + p.heads_each - 1) / p.heads_each;
-  if (blocks > 0x7fffffff || rows > 65535) return fail(CHITU_E_UNSUPPORTED, "kv_append: too many pages or heads for one call");
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(rows));
-  const int threads = group * p.heads_each;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool fp16 = dtype == CHITU_DTYPE_FP16, eight = es == 1;
-  if (fp16 && eight)
-    chitu::kv_append_kernel<true, true><<<grid, threads, 0, st>>>(p);
-  else if (fp16)
-    chitu::kv_append_kernel<true, false><<<grid, threads, 0, st>>>(p);
-  else if (eight)
-    chitu::kv_append_kernel<false, true><<<grid, threads, 0, st>>>(p);
-  else
-    chitu::kv_append_kernel<false, false><<<grid, threads, 0, st>>>(p);
+  const int expected = std::max<int>(1, static_cast<int>(std::min<int64_t>(max_new, tokens)));
+  const int planes = 2 * p.heads_kv + p.heads_q;
+  if (expected <= kAppendFew) {
+    const dim3 grid(static_cast<unsigned>(p.batch), static_cast<unsigned>((planes + 31) / 32));
+    if (grid.y > 65535) return fail(CHITU_E_UNSUPPORTED, "kv_append: too many heads for one call");
+    if (fp16 && eight)
+      chitu::kv_append_few_kernel<true, true><<<grid, 256, 0, st>>>(p);
+    else if (fp16)
+      chitu::kv_append_few_kernel<true, false><<<grid, 256, 0, st>>>(p);
+    else if (eight)
+      chitu::kv_append_few_kernel<false, true><<<grid, 256, 0, st>>>(p);
+    else
+      chitu::kv_append_few_kernel<false, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    // rows of a run, threads, heads of a block at a time (see kv_append_kernel)
+    const int q_rows = std::min(p.page, 64), kv_rows = eight ? p.page : q_rows;
+    const int threads = std::max(256, 4 * kv_rows);
+    const int kv_each = threads / (4 * kv_rows), q_each = threads / (4 * q_rows);
+    p.slots = (expected + q_rows - 2) / q_rows + 1;
+    const int64_t blocks = static_cast<int64_t>(p.batch) * p.slots;
+    const int kv_groups = (p.heads_kv + kv_each - 1) / kv_each, q_groups = (p.heads_q + q_each - 1) / q_each;
+    // groups of a block: as many as leave every SM six blocks
+    p.turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, blocks * (2 * kv_groups + q_groups) / (kSms * 6))));
+    p.kv_blocks = (kv_groups + p.turns - 1) / p.turns;
+    const int64_t rows = 2 * p.kv_blocks + (q_groups + p.turns - 1) / p.turns;
+    if (blocks > 0x7fffffff || rows > 65535) return fail(CHITU_E_UNSUPPORTED, "kv_append: too many pages or heads for one call");
+    auto launch = [&](int n_threads, int64_t y) {
+      const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(y));
+      if (fp16) return eight ? launch_append<true, true>(p, n_threads, grid, st) : launch_append<true, false>(p, n_threads, grid, st);
+      return eight ? launch_append<false, true>(p, n_threads, grid, st) : launch_append<false, false>(p, n_threads, grid, st);
+    };
+    cudaError_t e;
+    if (threads > 512 && q != nullptr) {
+      // Pages of 256 tokens want blocks without room for the factors, queries do not: 12 prompts 127 us in one launch, 108 in two
+      // (pages of 128: 80 and 84).
+      e = launch(threads, 2 * p.kv_blocks);
+      const int each = 256 / (4 * q_rows);
+      const int groups = (p.heads_q + each - 1) / each;
+      p.turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, blocks * groups / (kSms * 6))));
+      p.kv_blocks = 0;
+      if (e == cudaSuccess) e = launch(256, (groups + p.turns - 1) / p.turns);
+    } else {
+      e = launch(threads, rows);
+    }
+    if (e != cudaSuccess) return cuda_fail(e, "kv_append: launch");
+  }
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "kv_append: launch");
 }

@@ -110,26 +110,30 @@ def _append_case(page, new, old, heads, heads_q, dtype, eight, heads_first, rot,
     k, v, q = (t.to(dtype) for t in (k, v, q))
     caches = [model.make_cache(gen, pages, page, heads, dtype, eight, heads_first) for _ in range(2)]
     rope = model.rope_table(rot, 500)
+    hints = [max(new + [1]), 1, 1000, None]  # whatever the launch is sized for
     seq_pos = torch.cat([torch.arange(int(lens[b]) - n, int(lens[b])) for b, n in enumerate(new)] + [torch.zeros(behind, dtype=torch.long)])
     positions = torch.randint(-2, 505, (T + behind,), generator=gen) if explicit else None
     turn = seq_pos if positions is None else positions
-    dev = [(c.cuda(), None if s is None else s.cuda()) for c, s in caches]
-    dev = [(c.transpose(1, 2).contiguous().transpose(1, 2) if heads_first else c, s) for c, s in dev]
-    got_q = _ops().kv_cache_append(
+    put = lambda c: c.transpose(1, 2).contiguous().cuda().transpose(1, 2) if heads_first else c.contiguous().cuda()  # noqa: E731
+    devs = [[(put(c), None if s is None else s.cuda()) for c, s in caches] for _ in hints]
+    got_qs = [_ops().kv_cache_append(
         k.cuda(), v.cuda(), dev[0][0], dev[1][0], table.cuda(), lens.cuda(), cu.cuda(), k_scale=dev[0][1], v_scale=dev[1][1],
-        positions=None if positions is None else positions.cuda(), rope_table=rope.cuda(), interleaved=interleaved, q=q.cuda(), max_new=max(new + [1]))
+        positions=None if positions is None else positions.cuda(), rope_table=rope.cuda(), interleaved=interleaved, q=q.cuda(), max_new=hint)
+        for hint, dev in zip(hints, devs)]
     for (c, s), x in zip(caches, (model.rotate(k, turn, rope, interleaved), v.float())):
         model.append(x, c, s, table, lens, cu)
-    for (c, s), (gc, gs) in zip(caches, dev):
-        _equal(gc, c)
-        if s is not None:
-            _equal(gs, s)
-    _equal(got_q[:T], model.rotate(q, turn, rope, interleaved).to(dtype)[:T])
+    for dev, got_q in zip(devs, got_qs):
+        for (c, s), (gc, gs) in zip(caches, dev):
+            _equal(gc, c)
+            if s is not None:
+                _equal(gs, s)
+        _equal(got_q[:T], model.rotate(q, turn, rope, interleaved).to(dtype)[:T])
 
 
 @pytest.mark.parametrize("eight", [True, False])
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
-@pytest.mark.parametrize("new,old", [([1], [0]), ([1, 1, 1, 1], [0, 5, 15, 16]), ([3, 0, 70, 17], [14, 9, 63, 0]), ([300], [130])])
+@pytest.mark.parametrize("new,old", [([1], [0]), ([1, 1, 1, 1], [0, 5, 15, 16]), ([4, 3, 0, 2], [15, 62, 9, 254]), ([3, 0, 70, 17], [14, 9, 63, 0]),
+                                     ([300], [130]), ([5, 600, 1, 33], [0, 1, 2, 300])])
 def test_append(page, new, old, eight):
     _append_case(page, new, old, 3, 5, BF16, eight, True, 128, False, False)
 
@@ -148,7 +152,9 @@ def test_append_into_pages_that_do_not_exist(eight):
         table[0, 1], table[1, 0], table[2, 1] = -5, 1000, 2 ** 31 - 1
 
     _append_case(16, [40, 3, 20], [3, 2, 9], 2, 2, BF16, eight, True, 128, False, False, spoil=spoil)
-    _append_case(16, [40], [-13], 2, 2, BF16, eight, True, 128, False, True)  # the length counts fewer tokens than come
+    for n in (40, 3):  # the length counts fewer tokens than come, or none
+        _append_case(16, [n], [-2], 2, 2, BF16, eight, True, 128, False, True)
+        _append_case(16, [n, 5], [-n, 7], 2, 2, BF16, eight, True, 128, False, True)
 
 
 def test_append_without_rotation_and_twice():
