@@ -105,6 +105,10 @@ class QPre(ctypes.Structure):
 # ``chitu_b200_kv_cache`` as bytes: a call packs it afresh, which takes a tenth of filling a ctypes structure field by field
 KV_CACHE = struct.Struct("4P" "3q3q2q2q" "3P" "q" "6i")
 CACHE_16BIT, CACHE_E4M3 = 0, 1
+# arrays of n pointers / 64-bit / 32-bit integers as bytes
+PTRS = tuple(struct.Struct(f"{n}P").pack for n in range(4))
+I64S = tuple(struct.Struct(f"{n}q").pack for n in range(7))
+INTS = tuple(struct.Struct(f"{n}i").pack for n in range(4))
 
 SYNC_INTS = 64
 
@@ -250,21 +254,22 @@ def load() -> ctypes.CDLL:
         _vp, _vp,
     ]
     lib.chitu_b200_rotary.restype = ctypes.c_int
+    # (arrays as plain addresses: bytes and ctypes arrays alike)
     lib.chitu_b200_rotary.argtypes = [
-        _vpp, _vpp, _i64p, _i64p, ctypes.POINTER(ctypes.c_int), ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
-        ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, _vp,
+        _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp,
+        ctypes.c_int64, ctypes.c_int, _vp,
     ]
     lib.chitu_b200_kv_append.restype = ctypes.c_int
     lib.chitu_b200_kv_append.argtypes = [
-        ctypes.c_char_p, _vp, _vp, _vp, _i64p, _i64p, _i64p, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
-        _vp, ctypes.c_int, _vp, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp,
+        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp,
+        ctypes.c_int64, ctypes.c_int, ctypes.c_int, _vp,
     ]
     lib.chitu_b200_attn_cache_workspace_bytes.restype = ctypes.c_int64
     lib.chitu_b200_attn_cache_workspace_bytes.argtypes = [ctypes.c_int] * 3
     lib.chitu_b200_attn_fwd_cache.restype = ctypes.c_int
     lib.chitu_b200_attn_fwd_cache.argtypes = [
-        ctypes.c_char_p, _vp, _i64p, _vp, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_int,
-        ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int64, _vp, _vp,
+        _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp,
+        ctypes.c_int64, _vp, _vp,
     ]
     lib.chitu_b200_peer_wait_outputs.restype = ctypes.c_int
     lib.chitu_b200_peer_wait_outputs.argtypes = [ctypes.POINTER(PeerSyncDesc), _vp, _vp]

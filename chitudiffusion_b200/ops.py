@@ -886,6 +886,7 @@ def peer_wait_outputs(sync, device: torch.device) -> None:
 
 
 # ---------------------------------------------------------------------------------------------- paged key/value cache
+# Calls of a generation loop wait for the host: tensors are asked for each attribute once, arrays go down as packed bytes.
 _CACHE_HEAD_DIM = 128
 _CACHE_PAGES = (16, 32, 64, 128, 256)
 _POSITION_DTYPES = (torch.int32, torch.int64)
@@ -893,18 +894,18 @@ _POSITION_DTYPES = (torch.int32, torch.int64)
 
 def _token_rows(t: torch.Tensor) -> torch.Tensor:
     """``t [tokens, heads, D]`` as the kernels take it: channels contiguous, 16-byte aligned, otherwise of any strides."""
-    per = 16 // t.element_size()
     s0, s1, s2 = t.stride()
-    if s2 == 1 and s0 % per == 0 and s1 % per == 0 and s0 > 0 and s1 > 0 and t.data_ptr() % 16 == 0:
+    if s2 == 1 and s0 and s1 and not (s0 | s1) * t.element_size() & 15 and not t.data_ptr() & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_rope(rope_table: torch.Tensor, head_dim: int, what: str) -> int:
     """Rotated channels of a table of (cos, sin) pairs ``[rows, rot / 2, 2]``."""
-    if rope_table.dtype != torch.float32 or rope_table.dim() != 3 or rope_table.shape[2] != 2 or not rope_table.is_contiguous():
+    shape = rope_table.shape
+    if rope_table.dtype != torch.float32 or len(shape) != 3 or shape[2] != 2 or not rope_table.is_contiguous():
         raise ValueError(f"{what}: rope_table must be a contiguous fp32 [rows, rot / 2, 2] tensor")
-    rot = 2 * rope_table.shape[1]
+    rot = 2 * shape[1]
     if rot > head_dim:
         raise ValueError(f"{what}: rope_table turns {rot} channels, a head has {head_dim}")
     if rot % 16 or rot == 0:
@@ -915,7 +916,7 @@ def _check_rope(rope_table: torch.Tensor, head_dim: int, what: str) -> int:
 def _check_positions(positions: torch.Tensor, tokens: int, what: str) -> torch.Tensor:
     if positions.dtype not in _POSITION_DTYPES or positions.numel() != tokens:
         raise ValueError(f"{what}: positions must be int32 or int64, one per token ({tokens})")
-    return positions.contiguous()
+    return positions if positions.is_contiguous() else positions.contiguous()
 
 
 def rotary(x, positions: torch.Tensor, rope_table: torch.Tensor, interleaved: bool = True, out=None):
@@ -929,54 +930,61 @@ def rotary(x, positions: torch.Tensor, rope_table: torch.Tensor, interleaved: bo
     See ``chitu_b200_rotary``.
     """
     single = isinstance(x, torch.Tensor)
-    xs = [x] if single else list(x)
-    outs = [None] * len(xs) if out is None else [out] if single else list(out)
-    if not 1 <= len(xs) <= 3 or len(outs) != len(xs):
+    xs = (x,) if single else tuple(x)
+    n = len(xs)
+    outs = (None,) * n if out is None else (out,) if single else tuple(out)
+    if not 1 <= n <= 3 or len(outs) != n:
         raise ValueError("rotary: one to three tensors, and as many outputs")
     first = xs[0]
-    if first.dim() not in (3, 4) or first.dtype not in _DTYPES:
+    shape, dtype = first.shape, first.dtype
+    dim = len(shape)
+    if dim not in (3, 4) or dtype not in _DTYPES:
         raise ValueError("rotary: x must be [T, H, D] or [B, S, H, D], bf16, fp16 or fp32")
-    lead, D, dtype, device = first.shape[:-2], first.shape[-1], first.dtype, first.device
-    n_tokens = first.shape[0] if first.dim() == 3 else first.shape[0] * first.shape[1]
+    lead, D, on = shape[:-2], shape[-1], first.get_device()
+    n_tokens = shape[0] if dim == 3 else shape[0] * shape[1]
     if D % 16 or D > 512:
         raise NotImplementedError(f"rotary: head_dim must be a multiple of 16 up to 512 (got {D})")
     rot = _check_rope(rope_table, D, "rotary")
     positions = _check_positions(positions, n_tokens, "rotary")
-    n = len(xs)
     ptrs, out_ptrs, strides, out_strides, heads, keep, results = [], [], [], [], [], [], []
     for t, o in zip(xs, outs):
-        if t.shape[:-2] != lead or t.shape[-1] != D or t.dtype != dtype or t.device != device:
+        s = t.shape
+        if s[:-2] != lead or s[-1] != D or t.dtype != dtype or t.get_device() != on:
             raise ValueError("rotary: tensors of one call share tokens, head_dim, dtype and device")
-        if t.shape[-2] == 0:
+        if s[-2] == 0:
             raise ValueError("rotary: a tensor has no heads")
-        rows = _token_rows(t if t.dim() == 3 else t.flatten(0, 1))
+        rows = _token_rows(t if dim == 3 else t.flatten(0, 1))
         if o is None:
-            o = torch.empty(t.shape, dtype=dtype, device=device)
-            o_rows = o if o.dim() == 3 else o.flatten(0, 1)
+            o = torch.empty_like(t, memory_format=torch.contiguous_format)
+            out_ptrs.append(o.data_ptr())
+            out_strides += (s[-2] * D, D)
         else:
-            if o.shape != t.shape or o.dtype != dtype or o.device != device:
+            if o.shape != s or o.dtype != dtype or o.get_device() != on:
                 raise ValueError("rotary: out must have x's shape, dtype and device")
-            o_rows = o if o.dim() == 3 else o.flatten(0, 1)
+            o_rows = o if dim == 3 else o.flatten(0, 1)
             if o_rows.data_ptr() != o.data_ptr() or _token_rows(o_rows) is not o_rows:
                 raise ValueError("rotary: out must have contiguous channels and 16-byte aligned rows")
+            out_ptrs.append(o.data_ptr())
+            out_strides += o_rows.stride()[:2]
         ptrs.append(rows.data_ptr())
-        out_ptrs.append(o_rows.data_ptr())
         strides += rows.stride()[:2]
-        out_strides += o_rows.stride()[:2]
-        heads.append(t.shape[-2])
+        heads.append(s[-2])
         keep.append(rows)
         results.append(o)
-    _require_cuda(*xs, *results, positions, rope_table)
-    if positions.device != device or rope_table.device != device:
+    if on < 0:
+        _require_cuda(first)
+    if positions.get_device() != on or rope_table.get_device() != on:
         raise ValueError("rotary: positions and rope_table must be on x's device")
     if n_tokens == 0:
         return results[0] if single else results
-    with _on(device):
-        rc = _lib.load().chitu_b200_rotary(
-            _lib.ptr_array(ptrs), _lib.ptr_array(out_ptrs), _lib.i64_array(strides), _lib.i64_array(out_strides),
-            (ctypes.c_int * n)(*heads), n, n_tokens, D, rot, _DTYPES[dtype], positions.data_ptr(),
-            1 if positions.dtype == torch.int64 else 0, rope_table.data_ptr(), rope_table.shape[0], 1 if interleaved else 0,
-            _stream_ptr(device))
+    args = (_lib.PTRS[n](*ptrs), _lib.PTRS[n](*out_ptrs), _lib.I64S[2 * n](*strides), _lib.I64S[2 * n](*out_strides), _lib.INTS[n](*heads),
+            n, n_tokens, D, rot, _DTYPES[dtype], positions.data_ptr(), positions.dtype == torch.int64, rope_table.data_ptr(),
+            rope_table.shape[0], bool(interleaved), torch._C._cuda_getCurrentRawStream(on))
+    if torch._C._cuda_getDevice() == on:
+        rc = _lib.load().chitu_b200_rotary(*args)
+    else:
+        with torch.cuda.device(on):
+            rc = _lib.load().chitu_b200_rotary(*args)
     if rc:
         _lib.check(rc, "rotary")
     _launched()
@@ -984,55 +992,59 @@ def rotary(x, positions: torch.Tensor, rope_table: torch.Tensor, interleaved: bo
 
 
 def _pack_cache(k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale, v_scale, dtype, what):
-    """``chitu_b200_kv_cache`` of a call as bytes, after the checks that need no GPU: ``(bytes, pages, page_size, heads, is_8bit)``."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+    """``chitu_b200_kv_cache`` of a call as bytes, after the checks that need no GPU: ``(bytes, batch, table width, page_size, heads)``."""
+    shape, cache_dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != cache_dtype:
         raise ValueError(f"{what}: k_cache and v_cache must be [pages, page_size, H, 128] of one shape and dtype")
-    n_pages, page, heads, D = k_cache.shape
+    n_pages, page, heads, D = shape
     if D != _CACHE_HEAD_DIM:
         raise NotImplementedError(f"{what}: head_dim must be {_CACHE_HEAD_DIM} (got {D})")
     if page not in _CACHE_PAGES:
         raise NotImplementedError(f"{what}: page_size must be one of {_CACHE_PAGES} (got {page})")
     if n_pages == 0 or heads == 0:
         raise ValueError(f"{what}: the cache has no pages or no heads")
-    eight = k_cache.dtype == torch.float8_e4m3fn
-    if not eight and k_cache.dtype != dtype:
-        raise NotImplementedError(f"{what}: pages hold float8_e4m3fn or the inputs' type {dtype} (got {k_cache.dtype})")
-    device = k_cache.device
-    per = 16 if eight else 8
-    ks, vs = k_cache.stride(), v_cache.stride()
-    if ks[3] != 1 or vs[3] != 1 or any(s % per or s <= 0 for s in ks[:3] + vs[:3]) or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    eight = cache_dtype == torch.float8_e4m3fn
+    if not eight and cache_dtype != dtype:
+        raise NotImplementedError(f"{what}: pages hold float8_e4m3fn or the inputs' type {dtype} (got {cache_dtype})")
+    on = k_cache.get_device()
+    kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
+    k0, k1, k2, k3 = k_cache.stride()
+    v0, v1, v2, v3 = v_cache.stride()
+    if k3 != 1 or v3 != 1 or not (k0 and k1 and k2 and v0 and v1 and v2) or (k0 | k1 | k2 | v0 | v1 | v2) & (15 if eight else 7) or (kp | vp) & 15:
         raise ValueError(f"{what}: cache channels must be contiguous, rows and pages 16-byte aligned")
     if eight:
         for s in (k_scale, v_scale):
-            if s is None or s.dtype != torch.float32 or s.shape != (n_pages, heads) or s.device != device:
+            if s is None or s.dtype != torch.float32 or s.shape != (n_pages, heads) or s.get_device() != on:
                 raise ValueError(f"{what}: 8-bit pages need fp32 k_scale and v_scale [pages, H] = ({n_pages}, {heads})")
-        kss, vss, ksp, vsp = k_scale.stride(), v_scale.stride(), k_scale.data_ptr(), v_scale.data_ptr()
+        (ks0, ks1), (vs0, vs1), ksp, vsp = k_scale.stride(), v_scale.stride(), k_scale.data_ptr(), v_scale.data_ptr()
     else:
         if k_scale is not None or v_scale is not None:
             raise ValueError(f"{what}: 16-bit pages have no scales")
-        kss = vss = (0, 0)
-        ksp = vsp = 0
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[1] == 0 or block_table.stride(1) != 1:
+        ks0 = ks1 = vs0 = vs1 = ksp = vsp = 0
+    shape = block_table.shape
+    if len(shape) != 2 or block_table.dtype != torch.int32 or shape[1] == 0 or block_table.stride(1) != 1:
         raise ValueError(f"{what}: block_table must be an int32 [B, pages] tensor with contiguous rows")
-    B, width = block_table.shape
+    B, width = shape
     if kv_lens.dtype != torch.int32 or kv_lens.shape != (B,) or not kv_lens.is_contiguous():
         raise ValueError(f"{what}: kv_lens must be a contiguous int32 [B] tensor (B = {B})")
     if cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (B + 1,) or not cu_seqlens.is_contiguous():
         raise ValueError(f"{what}: cu_seqlens must be a contiguous int32 [B + 1] tensor (B = {B})")
-    if v_cache.device != device or block_table.device != device or kv_lens.device != device or cu_seqlens.device != device:
+    if v_cache.get_device() != on or block_table.get_device() != on or kv_lens.get_device() != on or cu_seqlens.get_device() != on:
         raise ValueError(f"{what}: the cache, its table and its lengths must be on one device")
-    packed = _lib.KV_CACHE.pack(
-        k_cache.data_ptr(), v_cache.data_ptr(), ksp, vsp, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kss[0], kss[1], vss[0], vss[1],
-        block_table.data_ptr(), kv_lens.data_ptr(), cu_seqlens.data_ptr(), block_table.stride(0), B, width, n_pages, page, heads,
-        _lib.CACHE_E4M3 if eight else _lib.CACHE_16BIT)
-    return packed, B, width, page, heads, eight
+    packed = _lib.KV_CACHE.pack(kp, vp, ksp, vsp, k0, k1, k2, v0, v1, v2, ks0, ks1, vs0, vs1, block_table.data_ptr(), kv_lens.data_ptr(),
+                                cu_seqlens.data_ptr(), block_table.stride(0), B, width, n_pages, page, heads,
+                                _lib.CACHE_E4M3 if eight else _lib.CACHE_16BIT)
+    return packed, B, width, page, heads
 
 
-def _check_tokens(t: torch.Tensor, name: str, what: str) -> None:
-    if t.dim() != 3 or t.shape[2] != _CACHE_HEAD_DIM:
+def _check_tokens(t: torch.Tensor, name: str, what: str):
+    """Shape and type of packed tokens."""
+    shape, dtype = t.shape, t.dtype
+    if len(shape) != 3 or shape[2] != _CACHE_HEAD_DIM:
         raise ValueError(f"{what}: {name} must be packed tokens [T, H, {_CACHE_HEAD_DIM}]")
-    if t.dtype not in (torch.bfloat16, torch.float16):
+    if dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f"{what}: {name} must be bf16 or fp16")
+    return shape, dtype
 
 
 def kv_cache_append(
@@ -1064,49 +1076,54 @@ def kv_cache_append(
     brings (default: the average); it sizes the launch, results do not depend on it.
     """
     what = "kv_cache_append"
-    _check_tokens(k, "k", what)
-    if v.shape != k.shape or v.dtype != k.dtype:
+    shape, dtype = _check_tokens(k, "k", what)
+    if v.shape != shape or v.dtype != dtype:
         raise ValueError(f"{what}: shape mismatch: k {tuple(k.shape)}, v {tuple(v.shape)}")
-    packed, B, width, page, heads, eight = _pack_cache(k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale, v_scale, k.dtype, what)
-    T = k.shape[0]
-    if k.shape[1] != heads:
-        raise ValueError(f"{what}: k has {k.shape[1]} heads, the cache {heads}")
-    device = k.device
+    packed, B, _, _, heads = _pack_cache(k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale, v_scale, dtype, what)
+    T = shape[0]
+    if shape[1] != heads:
+        raise ValueError(f"{what}: k has {shape[1]} heads, the cache {heads}")
+    on = k.get_device()
+    q_heads = 0
     if q is not None:
-        _check_tokens(q, "q", what)
-        if q.shape[0] != T or q.dtype != k.dtype or q.shape[1] == 0:
+        q_shape, q_dtype = _check_tokens(q, "q", what)
+        q_heads = q_shape[1]
+        if q_shape[0] != T or q_dtype != dtype or q_heads == 0:
             raise ValueError(f"{what}: q must be [T, Hq, 128] of k's tokens and dtype")
         if rope_table is None:
             raise ValueError(f"{what}: q is taken to be rotated, which needs a rope_table")
-    rot = 0
+    rot = rows = table_ptr = 0
     if rope_table is not None:
-        rot = _check_rope(rope_table, _CACHE_HEAD_DIM, what)
+        rot, rows, table_ptr = _check_rope(rope_table, _CACHE_HEAD_DIM, what), rope_table.shape[0], rope_table.data_ptr()
     elif positions is not None:
         raise ValueError(f"{what}: positions without a rope_table")
     if positions is not None:
         positions = _check_positions(positions, T, what)
-    _require_cuda(k, v, k_cache, q, positions, rope_table)
+    if on < 0:
+        _require_cuda(k)
     for t in (v, k_cache, q, positions, rope_table):
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != on:
             raise ValueError(f"{what}: all tensors must be on one device")
     k, v = _token_rows(k), _token_rows(v)
-    q_out = None
+    i64x2 = _lib.I64S[2]
+    q_out = q_ptr = q_strides = q_out_ptr = None
     if q is not None:
         q = _token_rows(q)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_ptr, q_strides, q_out_ptr = q.data_ptr(), i64x2(*q.stride()[:2]), q_out.data_ptr()
     if T == 0 or B == 0:
         return q_out
     if max_new is None:
         max_new = -(-T // B)
-    i64x2 = _lib._I64x2
-    with _on(device):
-        rc = _lib.load().chitu_b200_kv_append(
-            packed, k.data_ptr(), v.data_ptr(), q.data_ptr() if q is not None else None, i64x2(*k.stride()[:2]), i64x2(*v.stride()[:2]),
-            i64x2(*q.stride()[:2]) if q is not None else None, q_out.data_ptr() if q is not None else None,
-            q.shape[1] if q is not None else 0, T, _DTYPES[k.dtype], int(max_new),
-            positions.data_ptr() if positions is not None else None, 1 if positions is not None and positions.dtype == torch.int64 else 0,
-            rope_table.data_ptr() if rope_table is not None else None, rope_table.shape[0] if rope_table is not None else 0, rot,
-            1 if interleaved else 0, _stream_ptr(device))
+    args = (packed, k.data_ptr(), v.data_ptr(), q_ptr, i64x2(*k.stride()[:2]), i64x2(*v.stride()[:2]), q_strides, q_out_ptr, q_heads, T,
+            _DTYPES[dtype], int(max_new), None if positions is None else positions.data_ptr(),
+            positions is not None and positions.dtype == torch.int64, table_ptr, rows, rot, bool(interleaved),
+            torch._C._cuda_getCurrentRawStream(on))
+    if torch._C._cuda_getDevice() == on:
+        rc = _lib.load().chitu_b200_kv_append(*args)
+    else:
+        with torch.cuda.device(on):
+            rc = _lib.load().chitu_b200_kv_append(*args)
     if rc:
         _lib.check(rc, what)
     _launched()
@@ -1120,6 +1137,11 @@ def _cache_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
         if ws is not None and ws.numel() >= nbytes:
             return ws
     return _split_scratch(device, nbytes)
+
+
+@functools.lru_cache(maxsize=256)
+def _cache_workspace_bytes(heads: int, q_heads: int, max_q: int) -> int:
+    return int(_lib.load().chitu_b200_attn_cache_workspace_bytes(heads, q_heads, max_q))
 
 
 def attn_fwd_cache(
@@ -1150,36 +1172,39 @@ def attn_fwd_cache(
     what the table can hold); they choose the kernel and its grid, results are right whatever they are.
     """
     what = "attn_fwd_cache"
-    _check_tokens(q, "q", what)
-    packed, B, width, page, heads, eight = _pack_cache(k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale, v_scale, q.dtype, what)
-    T, Hq, D = q.shape
+    shape, dtype = _check_tokens(q, "q", what)
+    packed, B, width, page, heads = _pack_cache(k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale, v_scale, dtype, what)
+    T, Hq, D = shape
     if Hq == 0 or Hq % heads:
         raise ValueError(f"{what}: {Hq} query heads over {heads} key heads")
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"{what}: softmax_scale must be positive and finite (got {scale})")
-    device = q.device
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != device):
+    device, on = q.device, q.get_device()
+    if out is not None and (out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.get_device() != on):
         raise ValueError(f"{what}: out must be a contiguous tensor of q's shape, dtype and device")
-    _require_cuda(q, k_cache)
-    if k_cache.device != device:
+    if on < 0:
+        _require_cuda(q)
+    if k_cache.get_device() != on:
         raise ValueError(f"{what}: q and the cache must be on one device")
     q = _token_rows(q)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((Hq, T), dtype=torch.float32, device=device) if return_lse else None
     if T == 0 or B == 0:
         return out, lse
     max_q = -(-T // B) if max_q is None else max(1, int(max_q))
     max_kv = width * page if max_kv is None else max(1, min(int(max_kv), width * page))
-    lib = _lib.load()
-    with _on(device):
-        need = lib.chitu_b200_attn_cache_workspace_bytes(heads, Hq, max_q)
-        ws = _cache_scratch(device, need) if need else None
-        rc = lib.chitu_b200_attn_fwd_cache(
-            packed, q.data_ptr(), _lib._I64x2(*q.stride()[:2]), out.data_ptr(), lse.data_ptr() if lse is not None else None, Hq, T,
-            scale, 1 if causal else 0, _DTYPES[q.dtype], max_q, max_kv, ws.data_ptr() if need else None, ws.numel() if need else 0,
-            status_word(device).data_ptr(), _stream_ptr(device))
+    need = _cache_workspace_bytes(heads, Hq, max_q)
+    ws = _cache_scratch(device, need)
+    args = (packed, q.data_ptr(), _lib.I64S[2](*q.stride()[:2]), out.data_ptr(), None if lse is None else lse.data_ptr(), Hq, T, scale,
+            bool(causal), _DTYPES[dtype], max_q, max_kv, ws.data_ptr(), ws.numel(), status_word(device).data_ptr(),
+            torch._C._cuda_getCurrentRawStream(on))
+    if torch._C._cuda_getDevice() == on:
+        rc = _lib.load().chitu_b200_attn_fwd_cache(*args)
+    else:
+        with torch.cuda.device(on):
+            rc = _lib.load().chitu_b200_attn_fwd_cache(*args)
     if rc:
         _lib.check(rc, what)
     _launched()
