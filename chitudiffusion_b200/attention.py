@@ -80,6 +80,19 @@ class B200AttnBackend:
         ops.poll_status(q.device)
         return out, lse, None
 
+    def attend_cache(self, q: torch.Tensor, cache, *, causal: bool = False, softmax_scale: Optional[float] = None,
+                     return_attn_probs: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """Attention of ``q`` over a :class:`kv_cache.PagedKVCache` (frames made earlier, a prompt, tokens), with the call's own
+        tokens appended before; returns what a call of the backend returns.  Here rows may be causal, lengths may differ and
+        query heads may share key heads, which dense calls refuse."""
+        if self.impl != BACKEND_NAME:
+            raise NotImplementedError(f"attend_cache belongs to the {BACKEND_NAME} backend (this is {self.impl})")
+        ev = self._event_start()
+        out, lse = cache.attend(q, causal=causal, softmax_scale=softmax_scale, return_lse=return_attn_probs)
+        self._event_stop(ev)
+        ops.poll_status(q.device)
+        return out, lse, None
+
     def _event_start(self):
         if self.event_log is None:
             return None

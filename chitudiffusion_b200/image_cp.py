@@ -25,6 +25,11 @@ variables (:131-157), are mirrored for the ``agkv`` mode (they change the result
                           multiple of CHITU_CP_KV_CACHE_INTERVAL (4) - nothing is gathered: the cached tensors
                           are reused with this rank's fresh shard spliced in (:167-205)
 
+A switch of this library's own holds that cache in 8 bits: with ``CHITU_B200_KV_CACHE_FP8=1`` a fresh step stores the OTHER ranks'
+keys and values in a ``kv_cache.PagedKVCache`` (half the memory; 75600 tokens x 40 heads: 0.77 GB a layer), and a stale step attends
+to the pages and to this rank's fresh shard and the text, which stay exact, and merges the two by their log-sum-exps - nothing
+is concatenated.
+
 The producer-callback entries (``attention_fused``, ``cp_attn_with_full_txt_fused``,
 ``attention_fused_packed``, :508-635) run the producers and take the same paths: the overlap they buy
 in the reference comes here from the exchange kernels themselves.
@@ -39,7 +44,9 @@ from typing import Dict, Optional, Tuple
 import torch
 import torch.distributed as dist
 
+from . import ops
 from .context_parallel import B200ContextParallel
+from .kv_cache import PagedKVCache
 
 _VALID_MODES = {"agkv", "ulysses", "ring", "ring_graph", "unified"}
 _FP8_MAX = 448.0  # largest e4m3 magnitude
@@ -78,7 +85,8 @@ class B200ImageContextParallel:
         self._kvcache_warmup = int(os.environ.get("CHITU_CP_KV_CACHE_WARMUP", "8"))
         self._kvcache_interval = max(1, int(os.environ.get("CHITU_CP_KV_CACHE_INTERVAL", "4")))
         self._kvcache_tail = int(os.environ.get("CHITU_CP_KV_CACHE_TAIL", "3"))
-        self._kvcache: Dict[tuple, tuple] = {}
+        self._kvcache_fp8 = os.environ.get("CHITU_B200_KV_CACHE_FP8", "0") == "1"
+        self._kvcache: Dict[tuple, object] = {}
         self._cur_step: Optional[int] = None
         self._cur_total: Optional[int] = None
         self._cur_tag = "cond"
@@ -145,7 +153,7 @@ class B200ImageContextParallel:
         key = (self._cur_tag, layer)
         if self._kvcache_is_fresh() or key not in self._kvcache:
             full_k, full_v = self.all_gather_seq(img_k), self.all_gather_seq(img_v)
-            self._kvcache[key] = (full_k.detach(), full_v.detach())
+            self._kvcache[key] = self._paged_others(key, full_k, full_v) if self._kvcache_fp8 else (full_k.detach(), full_v.detach())
             return full_k, full_v
         cached_k, cached_v = self._kvcache[key]
         n = img_k.shape[1]
@@ -154,6 +162,36 @@ class B200ImageContextParallel:
         full_v = torch.cat([cached_v[:, :lo], img_v, cached_v[:, lo + n:]], dim=1)
         return full_k, full_v
 
+    def _paged_others(self, key: tuple, full_k: torch.Tensor, full_v: torch.Tensor) -> PagedKVCache:
+        """The other ranks' rows of a gathered layer in 8-bit pages; a layer's cache is used again from step to step."""
+        B, S, H, _ = full_k.shape
+        n = S // self._group.group_size
+        cache = self._kvcache.get(key)
+        if cache is None or (cache.batch, cache.num_heads, cache.max_tokens) != (B, H, S - n):
+            cache = PagedKVCache(B, H, S - n, page_size=128, device=full_k.device)
+        for b in range(B):
+            cache.truncate(b)
+        lo = self._group.rank_in_group * n
+        for rows in (slice(0, lo), slice(lo + n, S)):
+            if rows.start < rows.stop:
+                cache.append(full_k[:, rows], full_v[:, rows])
+        return cache
+
+    def _attn_agkv_stale_fp8(self, cache: PagedKVCache, txt_q, txt_k, txt_v, img_q, img_k, img_v):
+        """A stale step over 8-bit pages: other ranks' keys from the pages, this rank's shard and the text as they are."""
+        n = img_q.shape[1]
+        q = torch.cat([img_q, txt_q], dim=1).contiguous()
+        own_out, own_lse, _ = self.attn_backend(q, torch.cat([img_k, txt_k], dim=1), torch.cat([img_v, txt_v], dim=1), causal=False,
+                                                return_attn_probs=True)
+        far_out, far_lse = cache.attend(q, return_lse=True)
+        B, S, H, D = q.shape
+        acc = torch.empty((B, S, H, D), dtype=torch.float32, device=q.device)
+        acc_lse = torch.empty((B, S, H, 1), dtype=torch.float32, device=q.device)
+        out = torch.empty_like(q)
+        ops.lse_combine(acc, acc_lse, own_out, own_lse, first=True)
+        ops.lse_combine(acc, acc_lse, far_out, far_lse, first=False, final_out=out)
+        return out[:, n:], out[:, :n]
+
     def _attn_agkv_approx(self, txt_q, txt_k, txt_v, img_q, img_k, img_v):
         """All-gather mode with the cache or the FP8 transfer switched on (:637-653): local queries
         ``[image shard, text]`` against ``[all image keys, text keys]`` on the raw kernel."""
@@ -161,6 +199,8 @@ class B200ImageContextParallel:
         if self._kvcache_enabled and self._cur_step is not None:
             layer = self._layer_idx
             self._layer_idx += 1
+            if self._kvcache_fp8 and not self._kvcache_is_fresh() and (self._cur_tag, layer) in self._kvcache:
+                return self._attn_agkv_stale_fp8(self._kvcache[(self._cur_tag, layer)], txt_q, txt_k, txt_v, img_q, img_k, img_v)
             full_k, full_v = self._agkv_gather_cached(layer, img_k, img_v)
         else:
             full_k, full_v = self.all_gather_seq_fp8(img_k), self.all_gather_seq_fp8(img_v)

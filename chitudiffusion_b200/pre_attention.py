@@ -15,6 +15,7 @@ kernel reads them through L2.
 
 from __future__ import annotations
 
+import math
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
@@ -64,6 +65,48 @@ def axis_rope_table(ids: torch.Tensor, axes_dims: Sequence[int], theta: float = 
         cols.append(torch.outer(ids[:, a].to(torch.float64), inv))
     ang = torch.cat(cols, dim=1)
     table = torch.stack([torch.cos(ang), torch.sin(ang)], dim=-1).to(torch.float32).contiguous()
+    return table.to(device) if device is not None else table
+
+
+def scaled_rope_table(rot_dim: int, max_len: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                      original_len: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                      device: Optional[torch.device] = None) -> torch.Tensor:
+    """``[max_len, rot_dim / 2, 2]`` fp32 (cos, sin) of one axis of positions, for :func:`ops.rotary` and the cache's append.
+
+    ``scaling`` makes a model trained on ``original_len`` positions reach ``factor`` times as far:
+
+    * ``"none"``      angle ``p * theta^(-2j / rot_dim)``;
+    * ``"linear"``    ``p / factor`` in the place of ``p``;
+    * ``"base"``      ``theta * factor^(rot_dim / (rot_dim - 2))`` in the place of ``theta``: the slowest pair turns as with
+      ``"linear"``, the fastest as with ``"none"``;
+    * ``"by_parts"``  pairs that make more than ``beta_fast`` turns within ``original_len`` keep their angle, those with fewer than
+      ``beta_slow`` get the linear one, the others a blend by their index; cos and sin times ``0.1 ln(factor) + 1`` (Peng et
+      al., "YaRN: Efficient Context Window Extension of Large Language Models", 2023).
+
+    Built in float64 on the host, like the other tables.
+    """
+    if rot_dim % 2 or rot_dim < 4 or max_len < 1 or factor < 1.0:
+        raise ValueError("scaled_rope_table: rot_dim must be even and at least 4, max_len positive, factor at least 1")
+    j = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    gain = 1.0
+    if scaling == "base":
+        theta = theta * factor ** (rot_dim / (rot_dim - 2))
+    inv = torch.pow(torch.tensor(theta, dtype=torch.float64), -j / rot_dim)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "by_parts":
+        def index_of(turns: float) -> float:  # the pair that makes so many turns within original_len
+            return rot_dim * math.log(original_len / (2.0 * math.pi * turns)) / (2.0 * math.log(theta))
+
+        low = max(math.floor(index_of(beta_fast)), 0)
+        high = min(math.ceil(index_of(beta_slow)), rot_dim - 1)
+        keep = 1.0 - ((j / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        inv = inv / factor * (1.0 - keep) + inv * keep
+        gain = 0.1 * math.log(factor) + 1.0
+    elif scaling not in ("none", "base"):
+        raise ValueError(f"scaled_rope_table: unknown scaling '{scaling}'")
+    ang = torch.outer(torch.arange(max_len, dtype=torch.float64), inv)
+    table = (torch.stack([torch.cos(ang), torch.sin(ang)], dim=-1) * gain).to(torch.float32).contiguous()
     return table.to(device) if device is not None else table
 
 

@@ -501,3 +501,103 @@ def test_an_empty_call_and_a_table_wider_than_the_sequences():
     ref = model.attend(q, kc, vc, ks, vs, wide[:, :2], lens, cu, 128 ** -0.5, False)
     out, lse = ops.attn_fwd_cache(q.cuda(), dev[0], dev[1], view, lens.cuda(), cu.cuda(), k_scale=dev[2], v_scale=dev[3], return_lse=True)
     _attention_close(out, lse, ref, BF16, True)
+
+
+# ------------------------------------------------------------------------------------------------ the class and its users
+def _held(cache, sequence):
+    """fp64 keys and values [length, H, 128] that a PagedKVCache holds of a sequence."""
+    t = {k: None if v is None else v.cpu() for k, v in cache.tensors.items()}
+    n = cache.lens[sequence]
+    return tuple(model.gathered(t[x + "_cache"], t[x + "_scale"], t["block_table"][sequence], n)[0] for x in "kv")
+
+
+def _dense(q, k, v, causal_from=None):
+    """fp64 attention of q [S, Hq, 128] over k, v [n, H, 128]: (out, lse [Hq, S], softmax |v|)."""
+    group = q.shape[1] // k.shape[1]
+    k, v = (t.double().repeat_interleave(group, 1) for t in (k, v))
+    s = torch.einsum("qhd,khd->hqk", q.double(), k) * 128 ** -0.5
+    if causal_from is not None:
+        s = s.masked_fill(torch.arange(k.shape[0]) > (causal_from + torch.arange(q.shape[0]))[:, None], -math.inf)
+    w = torch.softmax(s, -1)
+    return torch.einsum("hqk,khd->qhd", w, v), torch.logsumexp(s, -1), torch.einsum("hqk,khd->qhd", w, v.abs())
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+def test_paged_cache_and_backend_frame_by_frame(dtype):
+    """Frames of a clip one after the other, two samples, then single tokens of one of them: as the class is used."""
+    from chitudiffusion_b200 import B200AttnBackend, PagedKVCache
+
+    gen = torch.Generator().manual_seed(12)
+    heads, group, frame = 2, 2, 90
+    rope = model.rope_table(128, 400)
+    cache = PagedKVCache(2, heads, 400, page_size=32, dtype=dtype, device="cuda")
+    backend = B200AttnBackend("b200")
+    for step in range(3):
+        k, v = (torch.randn(2, frame, heads, 128, generator=gen).to(BF16) for _ in range(2))
+        q = torch.randn(2, frame, heads * group, 128, generator=gen).to(BF16)
+        turned = cache.append(k.cuda(), v.cuda(), q=q.cuda(), rope_table=rope.cuda())
+        pos = torch.arange(step * frame, (step + 1) * frame).repeat(2)
+        _equal(turned, model.rotate(q.flatten(0, 1), pos, rope, True).to(BF16).view(q.shape))
+        out, lse, none = backend.attend_cache(turned, cache, return_attn_probs=True)
+        assert none is None and out.shape == q.shape and lse.shape == (2, heads * group, frame)
+        for b in range(2):
+            want = _dense(turned[b].cpu(), *_held(cache, b))
+            _attention_close(out[b], lse[b], want, BF16, dtype == E4M3)
+    cache.truncate(1, 75)
+    k, v = (torch.randn(3, heads, 128, generator=gen).to(BF16) for _ in range(2))
+    q = torch.randn(3, heads * group, 128, generator=gen).to(BF16)
+    cache.append(k.cuda(), v.cuda(), [0, 3])
+    out, lse = cache.attend(q.cuda(), causal=True, return_lse=True)
+    assert cache.lens == [270, 78]
+    _attention_close(out, lse, _dense(q, *_held(cache, 1), causal_from=75), BF16, dtype == E4M3)
+    with pytest.raises(NotImplementedError):
+        B200AttnBackend("b200_q8").attend_cache(q.cuda(), cache)
+
+
+def test_image_cache_of_other_ranks_in_8_bits(monkeypatch):
+    """The cross-step K/V cache in 8-bit pages, one rank of two: fresh steps as without it, stale ones attend to the kept pages and to
+    this rank's fresh shard.
+
+    Tolerance: the two partial results are rounded to bf16 (2^-8 of softmax |v| at most), their probabilities too (2^-8),
+    the merged result once more (2^-8 of itself); scores as everywhere."""
+    from chitudiffusion_b200 import B200AttnBackend
+    from chitudiffusion_b200.image_cp import B200ImageContextParallel
+
+    for name, value in (("CHITU_CP_KV_CACHE", "1"), ("CHITU_CP_KV_CACHE_WARMUP", "0"), ("CHITU_CP_KV_CACHE_INTERVAL", "2"),
+                        ("CHITU_CP_KV_CACHE_TAIL", "0"), ("CHITU_B200_KV_CACHE_FP8", "1")):
+        monkeypatch.setenv(name, value)
+    gen = torch.Generator().manual_seed(3)
+    B, n, text, H = 2, 150, 20, 2
+
+    def draw(rows):
+        return torch.randn(B, rows, H, 128, generator=gen).to(BF16)
+
+    class Group:
+        group_size, rank_in_group = 2, 1
+
+        def all_gather_sequence(self, t):
+            return torch.cat([others.pop(0), t], 1)
+
+    cp = B200ImageContextParallel(B200AttnBackend("b200"), mode="agkv")
+    cp.enable(Group())
+    far = None
+    for step in range(4):
+        cp.begin_forward(step, 100)
+        others = [draw(n).cuda() for _ in range(2)]
+        if step % 2 == 0:
+            far = [t.cpu().double() for t in others]
+        tq, tk, tv, iq, ik, iv = draw(text), draw(text), draw(text), draw(n), draw(n), draw(n)
+        txt, img = cp.attention(*[t.cuda() for t in (tq, tk, tv, iq, ik, iv)])
+        assert len(others) == (0 if step % 2 == 0 else 2)  # a stale step gathers nothing
+        for b in range(B):
+            keys = far
+            if step % 2:  # the kept rows as their codes say
+                cache = cp._kvcache[("cond", 0)]
+                keys = [t[None].expand(B, -1, -1, -1) for t in _held(cache, b)]
+                for exact, kept in zip(far, keys):
+                    assert ((kept[b] - exact[b]).abs() <= 2 ** -4 * exact[b].abs() + 2 ** -9 * 2.0 ** -6).all()
+            k, v = (torch.cat([far_rows[b], own[b].double(), t[b].double()]) for far_rows, own, t in zip(keys, (ik, iv), (tk, tv)))
+            want, _, mag = _dense(torch.cat([iq[b], tq[b]]), k, v)
+            got = torch.cat([img[b], txt[b]]).double().cpu()
+            tol = 2 ** -8 * want.abs() + 1.02 * (2 ** -7 + 2 * SCORE) * mag + 1e-6
+            assert ((got - want).abs() <= tol).all(), (step, ((got - want).abs() / tol).max().item())

@@ -196,3 +196,93 @@ def test_the_c_entries_check_what_comes_with_it(lib):
     assert rotary(one, one, st, st, heads, 1, 5, 64, 128, 0, p, 0, p, 8, 0, None) == -1
     assert rotary(one, one, odd, st, heads, 1, 5, 128, 128, 0, p, 0, p, 8, 0, None) == -1
     assert rotary(one, one, st, st, heads, 1, 5, 128, 128, 3, p, 0, p, 8, 0, None) == -2
+
+
+# ------------------------------------------------------------------------------------------------ tables, bookkeeping
+@pytest.mark.parametrize("rot", [16, 64, 128])
+def test_scaled_rope_tables(rot):
+    from chitudiffusion_b200.pre_attention import axis_rope_table, scaled_rope_table
+
+    plain = scaled_rope_table(rot, 300)
+    assert torch.equal(plain, axis_rope_table(torch.arange(300)[:, None], [rot]))
+    assert torch.equal(scaled_rope_table(rot, 300, scaling="linear", factor=4.0)[::4], plain[:75])
+    # "base": the fastest pair as without, the slowest as with "linear"
+    base, linear = (scaled_rope_table(rot, 300, scaling=s, factor=4.0) for s in ("base", "linear"))
+    assert torch.equal(base[:, 0], plain[:, 0])
+    assert (base[:, -1] - linear[:, -1]).abs().max() <= 1e-6
+    # "by_parts": turns within 4096 positions decide, cos and sin share the gain
+    parts = scaled_rope_table(rot, 300, scaling="by_parts", factor=4.0, original_len=4096).double()
+    gain = 0.1 * torch.log(torch.tensor(4.0, dtype=torch.float64)) + 1.0
+    assert (parts.square().sum(-1).sqrt() - gain).abs().max() <= 1e-6
+    turns = 4096 / (2 * torch.pi) * 10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    fast, slow = turns > 32 * 10000.0 ** (2 / rot), turns < 10000.0 ** (-2 / rot)  # (the blend begins and ends at whole pairs)
+    assert (parts[:, fast] / gain - plain[:, fast]).abs().max() <= 1e-6
+    if slow.any():
+        assert (parts[:, slow] / gain - linear[:, slow]).abs().max() <= 1e-6
+    for bad in (dict(scaling="cubic"), dict(factor=0.5)):
+        with pytest.raises(ValueError):
+            scaled_rope_table(rot, 300, **bad)
+
+
+class _Calls:
+    """The operators' calls, in the place of the operators."""
+
+    def __init__(self, monkeypatch):
+        self.seen = []
+        monkeypatch.setattr(ops, "kv_cache_append", lambda k, v, **a: self._note("append", k, a, a.get("q")))
+        monkeypatch.setattr(ops, "attn_fwd_cache", lambda q, **a: self._note("attend", q, a, (q, torch.zeros(q.shape[1], q.shape[0]) if a["return_lse"] else None)))
+
+    def _note(self, what, x, a, result):
+        self.seen.append((what, tuple(x.shape), a["kv_lens"].tolist(), a["cu_seqlens"].tolist(), a["block_table"].clone(), a))
+        return result
+
+
+def test_paged_cache_bookkeeping(monkeypatch):
+    from chitudiffusion_b200 import PagedKVCache
+
+    calls = _Calls(monkeypatch)
+    cache = PagedKVCache(2, 3, 100, page_size=16, num_pages=8, device="cpu")
+    assert cache.tensors["k_cache"].shape == (8, 16, 3, 128) and cache.tensors["k_cache"].dtype == E4M3 and cache.free_pages == 8
+
+    def tokens(*shape):
+        return torch.zeros(*shape, 3, 128, dtype=BF16)
+
+    q = torch.zeros(2, 5, 6, 128, dtype=BF16)
+    assert cache.append(tokens(2, 5), tokens(2, 5), q=q, rope_table=TABLE).shape == q.shape
+    assert calls.seen[-1][2:4] == ([5, 5], [0, 5, 10]) and calls.seen[-1][5]["max_new"] == 5 and cache.free_pages == 6
+    out, lse = cache.attend(q, causal=True, return_lse=True)
+    assert out.shape == q.shape and lse.shape == (2, 6, 5) and calls.seen[-1][1] == (10, 6, 128)
+    cache.append(tokens(40), tokens(40), [33, 2])
+    assert cache.lens == [38, 7] and calls.seen[-1][2:4] == ([38, 7], [0, 33, 35]) and cache.free_pages == 4
+    used = calls.seen[-1][4]
+    assert (used >= 0).sum().item() == 4 and used[used >= 0].unique().numel() == 4
+    cache.attend(torch.zeros(3, 3, 128, dtype=BF16), q_lens=[1, 2])
+    assert calls.seen[-1][3] == [0, 1, 3] and calls.seen[-1][5]["max_kv"] == 38
+    # no page left: refused, nothing changes
+    with pytest.raises(RuntimeError, match="free"):
+        cache.append(tokens(90), tokens(90), [0, 90])
+    with pytest.raises(ValueError, match="at most"):
+        cache.append(tokens(63), tokens(63), [63, 0])
+    assert cache.lens == [38, 7] and cache.free_pages == 4
+    # what is forgotten is free again
+    cache.truncate(0, 17)
+    assert cache.lens == [17, 7] and cache.free_pages == 5 and cache.tensors["kv_lens"].tolist() == [17, 7]
+    cache.truncate(1)
+    assert cache.free_pages == 6
+    # a call that the operator refuses appends nothing
+    def refuse(*a, **k):
+        raise ValueError("no")
+
+    monkeypatch.setattr(ops, "kv_cache_append", refuse)
+    with pytest.raises(ValueError, match="no"):
+        cache.append(tokens(2, 30), tokens(2, 30))
+    assert cache.lens == [17, 0] and cache.free_pages == 6 and cache.tensors["kv_lens"].tolist() == [17, 0]
+    for bad in (lambda: cache.append(tokens(3, 1), tokens(3, 1)), lambda: cache.append(tokens(5), tokens(5)),
+                lambda: cache.append(tokens(5), tokens(5), [3, 3]), lambda: cache.attend(q[:1]), lambda: cache.truncate(2),
+                lambda: cache.truncate(0, 18), lambda: PagedKVCache(0, 1, 1, device="cpu")):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        PagedKVCache(1, 1, 1, page_size=48, device="cpu")
+    with pytest.raises(NotImplementedError):
+        PagedKVCache(1, 1, 1, dtype=torch.float32, device="cpu")
