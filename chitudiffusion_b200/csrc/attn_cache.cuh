@@ -151,10 +151,11 @@ struct RowsCursor {
   }
 };
 template <int kTile>
-__device__ __forceinline__ long long rows_steps(const CacheAttnParams& p, int b) {
+__device__ __forceinline__ long long rows_steps(const CacheAttnParams& p, int b, int& tiles) {
   const SeqInfo s = seq_info(p, b);
   const long long n_rb = (static_cast<long long>(s.n_new) * p.group + 15) >> 4;
-  return n_rb * p.heads_kv * max((s.len + kTile - 1) / kTile, 1);
+  tiles = max((s.len + kTile - 1) / kTile, 1);
+  return n_rb * p.heads_kv * tiles;
 }
 
 // Query rows g and g + 8 as matrix fragments: for 8-bit pages piece j (64 channels), step k (16 of them) is channels
@@ -225,6 +226,8 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   volatile int* last_flag = reinterpret_cast<volatile int*>(smem + Shape::bar_at + kRowsWarps * kStages * 8);
   volatile int* abort_flag = last_flag + 1;
   if (lane == 0) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
     *abort_flag = 0;
     // a step's copies, and four lanes' of the scales
     for (int s = 0; s < kStages; ++s) mbar_init(bars + 8 * s, kEightBit ? 5 : 1);
@@ -235,18 +238,29 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 
   // all steps, and where this CTA's run begins (each warp finds out by itself)
   long long total = 0;
-  for (int b = lane; b < p.batch; b += 32) total += rows_steps<kTile>(p, b);
+  int longest = 1;  // tiles of an item
+  for (int b = lane; b < p.batch; b += 32) {
+    int tiles;
+    total += rows_steps<kTile>(p, b, tiles);
+    longest = max(longest, tiles);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const long long per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(p.min_tiles));
-  const long long lo = blockIdx.x * per;
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  // A run costs about a microsecond a step, a piece of an item that is merged a fifth of one: n tiles are best cut into runs of
+  // sqrt(n / 5), where the grid does not ask for longer ones (32 tiles, 8 heads: runs of one 18.7 us, of two 12.8).
+  const int per = static_cast<int>(max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(max(1.f, sqrtf(0.2f * longest)))));
+  const long long lo = static_cast<long long>(blockIdx.x) * per;
   if (lo >= total) return;
-  const int n_steps = static_cast<int>(min(per, total - lo));
+  const int n_steps = static_cast<int>(min(static_cast<long long>(per), total - lo));
   RowsCursor cur;
   long long at = 0;  // steps before sequence cur.b
   for (cur.b = 0;; cur.b += 32) {
     const int b = cur.b + lane;
-    const long long mine = b < p.batch ? rows_steps<kTile>(p, b) : 0;
+    int tiles;
+    const long long mine = b < p.batch ? rows_steps<kTile>(p, b, tiles) : 0;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -263,13 +277,11 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     at += __shfl_sync(0xffffffffu, upto, 31);
   }
   cur.measure<kTile>(p);
-  long long item_start;  // first step of the item under the cursor
   {
     const long long item = (lo - at) / cur.n_tiles;
     cur.rb = static_cast<int>(item / p.heads_kv);
     cur.h = static_cast<int>(item - static_cast<long long>(cur.rb) * p.heads_kv);
-    item_start = at + item * cur.n_tiles;
-    cur.tile = static_cast<int>(lo - item_start);
+    cur.tile = static_cast<int>(lo - at - item * cur.n_tiles);
   }
   RowsCursor ahead = cur;  // what is copied next
   int copied = 0;
@@ -560,16 +572,18 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         }
       }
       fence_proxy_async_smem();  // (before the next copies into these stages)
-      const long long item_end = item_start + cur.n_tiles;
-      const long long c_first = item_start / per, c_last = (item_end - 1) / per;
+      // CTAs that have a share of this item, which began at step `begun` of this one's run (or before it)
+      const int begun = step - cur.tile, last_step = begun + cur.n_tiles - 1;
+      const int cta = blockIdx.x;
+      const int c_first = begun >= 0 ? cta : cta - (per - 1 - begun) / per, c_last = cta + last_step / per;
       bool write = true;
       if (c_first == c_last) {
         __syncthreads();
       } else {
-        auto piece = [&](long long cta) {  // an item starts a CTA's run, or is the last of it
-          return p.part + (2 * cta + (item_start > cta * per ? 1 : 0)) * kRowsPieceFloats;
+        auto piece = [&](int c) {  // an item starts a CTA's run, or is the last of it
+          return p.part + static_cast<long long>(2 * c + (c == c_first && begun - (c - cta) * per > 0 ? 1 : 0)) * kRowsPieceFloats;
         };
-        float* out_piece = piece(blockIdx.x);
+        float* out_piece = piece(cta);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (i >= n_halves) break;
@@ -577,41 +591,68 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           for (int t = 0; t < 4; ++t) reinterpret_cast<float2*>(out_piece)[(i * 16 + 4 * warp + t) * 32 + lane] = r[i][t];
           if (warp == 0 && c == 0) reinterpret_cast<float2*>(out_piece + 2048)[g + 8 * i] = make_float2(m_row[i], l_row[i]);
         }
-        __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {
-          const int before = atomicAdd(p.count + c_first, 1);
+          // (the barrier has ordered the CTA's stores before this release, and orders its loads behind the acquire)
+          int before;
+          asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.count + c_first) : "memory");
           const int last = before == c_last - c_first;
           if (last) p.count[c_first] = 0;
-          __threadfence();
           *last_flag = last;
         }
         __syncthreads();
         write = *last_flag != 0;
         if (write) {
-          const int n_pieces = static_cast<int>(c_last - c_first) + 1;
+          // Pieces in their order, three or seven at a time through the warp's stage (in registers they cost the main loop its own:
+          // spills, half the speed): this warp's accumulators of a piece, then its 16 rows' statistics.
+          const int n_pieces = c_last - c_first + 1;
+          const int region = n_halves * 1024 + 128, at_once = n_halves == 1 ? 7 : 3;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (i >= n_halves) break;
             m_row[i] = -INFINITY;
             l_row[i] = 0.f;
-            for (int k = 0; k < n_pieces; ++k) m_row[i] = fmaxf(m_row[i], __ldcg(reinterpret_cast<const float2*>(piece(c_first + k) + 2048) + g + 8 * i).x);
 #pragma unroll
             for (int t = 0; t < 4; ++t) r[i][t] = make_float2(0.f, 0.f);
-#pragma unroll 4
-            for (int k = 0; k < n_pieces; ++k) {
-              const float2* from = reinterpret_cast<const float2*>(piece(c_first + k));
-              const float2 st = __ldcg(from + 1024 + g + 8 * i);
-              const float f = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m_row[i]);
-              l_row[i] = fmaf(st.y, f, l_row[i]);
+          }
+#pragma unroll 1
+          for (int k0 = 0; k0 < n_pieces; k0 += at_once) {
+            const int n = min(at_once, n_pieces - k0);
+#pragma unroll 1
+            for (int k = 0; k < n; ++k) {
+              const float* from = piece(c_first + k0 + k);
+              const uint32_t to = src + k * region;
+#pragma unroll 1
+              for (int part = lane; part < n_halves * 64; part += 32)  // 16 bytes: two lanes' pairs of one accumulator
+                cp_async16(to + part * 16, from + (part >> 6) * 1024 + warp * 256 + (part & 63) * 4);
+              if (lane < 8) cp_async16(to + region - 128 + lane * 16, from + 2048 + lane * 4);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            __syncwarp();
 #pragma unroll
-              for (int t = 0; t < 4; ++t) {
-                const float2 v = __ldcg(from + (i * 16 + 4 * warp + t) * 32 + lane);
-                r[i][t].x = fmaf(v.x, f, r[i][t].x);
-                r[i][t].y = fmaf(v.y, f, r[i][t].y);
+            for (int i = 0; i < 2; ++i) {
+              if (i >= n_halves) break;
+#pragma unroll 1
+              for (int k = 0; k < n; ++k) {
+                const uint32_t at = src + k * region;
+                float2 st;
+                asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(st.x), "=f"(st.y) : "r"(at + region - 128 + (g + 8 * i) * 8) : "memory");
+                const float top = fmaxf(m_row[i], st.x);
+                const float mine = m_row[i] == -INFINITY ? 0.f : fast_exp2(m_row[i] - top), theirs = st.x == -INFINITY ? 0.f : fast_exp2(st.x - top);
+                m_row[i] = top;
+                l_row[i] = fmaf(st.y, theirs, l_row[i] * mine);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                  float x, y;
+                  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x), "=f"(y) : "r"(at + (i * 4 + t) * 256 + lane * 8) : "memory");
+                  r[i][t] = make_float2(fmaf(x, theirs, r[i][t].x * mine), fmaf(y, theirs, r[i][t].y * mine));
+                }
               }
             }
+            __syncwarp();
           }
+          fence_proxy_async_smem();  // (before the next copy into the stage)
+          __syncwarp();
         }
       }
       if (write) {
@@ -632,7 +673,6 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         }
       }
       if (step + 1 < n_steps) {
-        item_start = item_end;
         cur.next_item<kTile>(p);
         fresh = true;
       }

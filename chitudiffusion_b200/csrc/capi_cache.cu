@@ -96,9 +96,8 @@ int make_cache_map(CUtensorMap* map, const chitu_b200_kv_cache* c, const void* b
   return CHITU_OK;
 }
 
-// Grid of the rows kernel: all CTAs resident at once, or as many as there can be runs of kRowsMinTiles tiles.
+// Grid of the rows kernel: all CTAs resident at once, or as many as there can be runs of a tile.
 constexpr int kRowsGrid = kSms * 3;
-constexpr int kRowsMinTiles = 2;
 int64_t rows_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kRowsGrid) * 2 * chitu::kRowsPieceFloats * 4; }
 
 template <bool kFp16, bool kEightBit>
@@ -108,7 +107,7 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const chit
   cudaError_t e = allow_smem(chitu::attn_cache_rows_kernel<kFp16, kEightBit>, smem, done);
   if (e != cudaSuccess) return e;
   const int64_t items = static_cast<int64_t>(p.batch) * p.heads_kv * ((static_cast<int64_t>(max_q) * p.group + 15) / 16);
-  const int64_t runs = (items * ((max_kv + chitu::RowsShape<kEightBit>::tile - 1) / chitu::RowsShape<kEightBit>::tile) + kRowsMinTiles - 1) / kRowsMinTiles;
+  const int64_t runs = items * ((max_kv + chitu::RowsShape<kEightBit>::tile - 1) / chitu::RowsShape<kEightBit>::tile);
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kSms * chitu::RowsShape<kEightBit>::ctas_per_sm, runs)));
   chitu::attn_cache_rows_kernel<kFp16, kEightBit><<<grid, chitu::kRowsThreads, smem, st>>>(tk, tv, p);
   return cudaGetLastError();
@@ -407,7 +406,6 @@ int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, c
              : (eight ? launch_tile<false, true>(tk, tv, p, st) : launch_tile<false, false>(tk, tv, p, st));
     return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "attn_fwd_cache: launch");
   }
-  p.min_tiles = kRowsMinTiles;
   e = fp16 ? (eight ? launch_rows<true, true>(tk, tv, p, max_q, max_kv, st) : launch_rows<true, false>(tk, tv, p, max_q, max_kv, st))
            : (eight ? launch_rows<false, true>(tk, tv, p, max_q, max_kv, st) : launch_rows<false, false>(tk, tv, p, max_q, max_kv, st));
   return e == cudaSuccess ? CHITU_OK : cuda_fail(e, "attn_fwd_cache: launch");
