@@ -51,7 +51,7 @@ __device__ __forceinline__ SeqInfo seq_info(const CacheAttnParams& p, int b) {
   SeqInfo s;
   s.tok0 = min(max(__ldg(p.cu + b), 0), p.tokens);
   s.n_new = min(max(__ldg(p.cu + b + 1), s.tok0), p.tokens) - s.tok0;
-  const int raw = __ldg(p.lens + b);
+  const int raw = max(__ldg(p.lens + b), -(1 << 30));
   s.len = static_cast<int>(min(static_cast<long long>(max(raw, 0)), static_cast<long long>(p.width) << p.page_shift));
   s.first = raw - s.n_new;
   return s;
@@ -661,14 +661,14 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           const int row_i = cur.rb * 16 + g + 8 * i;
           const int tok = row_i / p.group, hq = cur.h * p.group + row_i - tok * p.group;
           if (i < n_halves && tok < cur.seq.n_new) {
-            const float inv = l_row[i] > 0.f ? 1.f / l_row[i] : 0.f;
+            const float inv = l_row[i] == 0.f ? 0.f : 1.f / l_row[i];
             const size_t row = static_cast<size_t>(cur.seq.tok0 + tok);
             uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128 + 4 * warp;
             // (accumulator t, column 2 c + e: channel 16 (2 c + e) + t)
             *reinterpret_cast<uint2*>(dst + 32 * c) = make_uint2(pack2<kFp16>(r[i][0].x * inv, r[i][1].x * inv), pack2<kFp16>(r[i][2].x * inv, r[i][3].x * inv));
             *reinterpret_cast<uint2*>(dst + 32 * c + 16) = make_uint2(pack2<kFp16>(r[i][0].y * inv, r[i][1].y * inv), pack2<kFp16>(r[i][2].y * inv, r[i][3].y * inv));
             if (p.lse != nullptr && warp == 0 && c == 0)
-              p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_row[i] > 0.f ? (m_row[i] - kProbShift + log2f(l_row[i])) * 0.6931471805599453f : -INFINITY;
+              p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_row[i] == 0.f ? -INFINITY : (m_row[i] - kProbShift + log2f(l_row[i])) * 0.6931471805599453f;
           }
         }
       }

@@ -750,7 +750,7 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         __syncwarp();
         tc_fence_after_sync();
         if (piece < 0) {
-          const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+          const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
           uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
@@ -775,7 +775,7 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             __syncwarp();
           }
           if (live && p.lse != nullptr)
-            p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_sum > 0.f ? (m - kProbShift + log2f(l_sum)) * 0.6931471805599453f : -INFINITY;
+            p.lse[static_cast<size_t>(hq) * p.tokens + row] = l_sum == 0.f ? -INFINITY : (m - kProbShift + log2f(l_sum)) * 0.6931471805599453f;
         } else {
           // a piece: rows as they are, the maximum and the sum with them
           float* to = p.part + static_cast<long long>(piece) * kTilePieceFloats + t * (kTilePieceFloats / 2);
@@ -867,7 +867,7 @@ attn_cache_join_kernel(const __grid_constant__ CacheAttnParams p, int ctas) {
     }
   }
   if (!live) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const size_t row = static_cast<size_t>(join.row + in_blk);
   uint16_t* dst = static_cast<uint16_t*>(p.out) + (row * (static_cast<size_t>(p.heads_kv) * p.group) + hq) * 128 + warp * 16;
   uint32_t v[8];
@@ -877,7 +877,7 @@ attn_cache_join_kernel(const __grid_constant__ CacheAttnParams p, int ctas) {
   d[0] = make_uint4(v[0], v[1], v[2], v[3]);
   d[1] = make_uint4(v[4], v[5], v[6], v[7]);
   if (warp == 0 && p.lse != nullptr)
-    p.lse[static_cast<size_t>(hq) * p.tokens + row] = l > 0.f ? (m - kProbShift + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    p.lse[static_cast<size_t>(hq) * p.tokens + row] = l == 0.f ? -INFINITY : (m - kProbShift + log2f(l)) * 0.6931471805599453f;
 }
 
 }  // namespace chitu

@@ -37,6 +37,8 @@ int check_cache(const chitu_b200_kv_cache* c, const char* what) {
   if (page_shift_of(c->page_size) < 0) return fail(CHITU_E_UNSUPPORTED, "%s: page_size must be 16, 32, 64, 128 or 256 (got %d)", what, c->page_size);
   if (c->batch < 0 || c->table_width < 1 || c->n_pages < 1 || c->heads < 1 || c->table_stride < 0)
     return fail(CHITU_E_INVALID, "%s: bad batch, table or page count", what);
+  if (static_cast<int64_t>(c->table_width) * c->page_size > (1 << 30))
+    return fail(CHITU_E_UNSUPPORTED, "%s: a table may name at most 2^30 tokens per sequence", what);
   const int es = c->format == CHITU_CACHE_E4M3 ? 1 : 2;
   if (!aligned16(c->k) || !aligned16(c->v)) return fail(CHITU_E_INVALID, "%s: pages must be 16-byte aligned", what);
   for (const int64_t* st : {c->k_strides, c->v_strides}) {

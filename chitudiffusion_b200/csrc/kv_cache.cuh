@@ -261,7 +261,7 @@ kv_append_kernel(const __grid_constant__ AppendParams p) {
   const int c0 = min(max(__ldg(p.cu + b), 0), p.tokens), c1 = min(max(__ldg(p.cu + b + 1), c0), p.tokens);
   const int n_new = c1 - c0;
   if (n_new == 0) return;
-  const int first = __ldg(p.lens + b) - n_new;  // position of the first new token
+  const int first = max(__ldg(p.lens + b), -(1 << 30)) - n_new;  // position of the first new token
   const int kind = static_cast<int>(blockIdx.y) < p.kv_blocks ? 0 : static_cast<int>(blockIdx.y) < 2 * p.kv_blocks ? 1 : 2;  // (kv_blocks 0: queries only)
   if (kind != 2 && first + n_new <= 0) return;  // (no token has a place)
   const int shift = kEightBit && kind != 2 ? p.page_shift : min(p.page_shift, 6);  // rows of a run
@@ -425,7 +425,7 @@ kv_append_few_kernel(const __grid_constant__ AppendParams p) {
   const int c0 = min(max(__ldg(p.cu + b), 0), p.tokens), c1 = min(max(__ldg(p.cu + b + 1), c0), p.tokens);
   const int n_new = c1 - c0;
   if (n_new == 0) return;
-  const int first = __ldg(p.lens + b) - n_new;
+  const int first = max(__ldg(p.lens + b), -(1 << 30)) - n_new;
   const int rot16 = p.rope != nullptr ? p.rot >> 4 : 0;
   int v0, v1;
   piece_vectors(u, rot16, 8, v0, v1);

@@ -1132,7 +1132,7 @@ def kv_cache_append(
 
 def _cache_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
     """:func:`_split_scratch` with the eager buffer looked up first."""
-    if not torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_getDevice() == _device_key(device) and not torch.cuda.is_current_stream_capturing():
         ws = _workspaces.get((_device_key(device), _stream_ptr(device)))
         if ws is not None and ws.numel() >= nbytes:
             return ws

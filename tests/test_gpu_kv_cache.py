@@ -309,6 +309,31 @@ def test_scores_far_apart(new, eight):
         assert ((lse.double().cpu() - want_lse).abs() <= score + 1e-6 * want_lse.abs()).all()
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 9]])
+@pytest.mark.parametrize("eight", [True, False])
+def test_a_query_that_is_not_a_number_and_lengths_below_zero(new, eight):
+    """NaN in one query stays in its row; a negative length holds no keys, for neither operator."""
+    lens, T = [200, -5, 77], sum(new)
+    args, dev, ref = _attend_case(32, new, lens, 2, 4, BF16, eight, False)
+    q = args[0].clone()
+    q[0, 3, 7] = math.nan
+    out, lse = _ops().attn_fwd_cache(q, *args[1:], **dev, return_lse=True)
+    assert out[0, 3].isnan().all() and lse[3, 0].isnan()
+    keep = torch.ones(T, 8, dtype=torch.bool)
+    keep[0, 3] = False
+    plain, plain_lse = _ops().attn_fwd_cache(*args, **dev, return_lse=True)
+    assert torch.equal(out[:T].cpu()[keep], plain[:T].cpu()[keep]) and torch.equal(lse[:, :T].cpu()[keep.T], plain_lse[:, :T].cpu()[keep.T])
+    k = torch.randn(T, 2, 128).to(BF16).cuda()
+    caches = [args[1].clone(), args[2].clone()]
+    scales = [None if s is None else s.clone() for s in (dev["k_scale"], dev["v_scale"])]
+    for length in (0, -2 ** 31):
+        _ops().kv_cache_append(k, k, *caches, args[3], torch.full((3,), length, dtype=torch.int32).cuda(), args[5], k_scale=scales[0], v_scale=scales[1])
+    for got, was in zip(caches + scales, (args[1], args[2], dev["k_scale"], dev["v_scale"])):
+        if was is not None:
+            raw = torch.uint8 if got.element_size() == 1 else torch.int16 if got.element_size() == 2 else torch.int32
+            assert torch.equal(got.contiguous().view(raw), was.contiguous().view(raw))
+
+
 @pytest.mark.parametrize("eight", [True, False])
 @pytest.mark.parametrize("new,lens,causal", [([1, 1], [70001, 33333], True), ([64], [20000], True), ([300, 5], [9000, 4000], False)])
 def test_long_caches(new, lens, causal, eight):

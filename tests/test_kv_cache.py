@@ -156,7 +156,7 @@ def _descriptor(**change):
 
 @pytest.mark.parametrize("change,code,text", [
     (dict(k=0), -1, b"null"), (dict(lens=0), -1, b"null"), (dict(vs=0), -1, b"scale"), (dict(format=7), -2, b"e4m3"),
-    (dict(page=20), -2, b"page_size"), (dict(pages=0), -1, b"page count"), (dict(width=0), -1, b"table"), (dict(batch=-1), -1, b"batch"),
+    (dict(page=20), -2, b"page_size"), (dict(width=(1 << 26) + 1), -2, b"2^30"), (dict(pages=0), -1, b"page count"), (dict(width=0), -1, b"table"), (dict(batch=-1), -1, b"batch"),
     (dict(kst=(4096, 256, 8)), -1, b"stride"), (dict(vst=(0, 256, 128)), -1, b"stride"), (dict(vst=(4096, -256, 128)), -1, b"stride"),
 ])
 def test_the_c_entries_check_the_descriptor_before_any_cuda_call(lib, change, code, text):
