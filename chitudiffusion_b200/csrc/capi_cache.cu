@@ -115,9 +115,11 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const chit
   return cudaGetLastError();
 }
 
-// Which kernel a call takes.  Up to 16 query rows of a key head (tokens x heads that share it) are one tile of the rows kernel;
-// more would have it read the cache once per 16 rows.
-bool takes_tile_kernel(int max_q, int group) { return static_cast<int64_t>(max_q) * group > 16 && group <= 128; }
+// Which kernel a call takes.  16 query rows of a key head (tokens x heads that share it) are one tile of the rows kernel, which
+// reads the cache once per 16 rows (from the L2 cache where two tiles of rows are in step).  Rows against tile kernel, 8-bit
+// pages, 8 key heads: 32 rows, 64 sequences of 500 keys 40 : 65 us, of 16000 keys 655 : 778, 8 of 4000 36 : 40, one of 16000 35 : 33;
+// 48 rows, 64 of 500 69 : 79 but of 16000 970 : 816; 64 rows, 8 of 4000 56 : 40, 64 of 16000 1291 : 823.
+bool takes_tile_kernel(int max_q, int group) { return static_cast<int64_t>(max_q) * group > 32 && group <= 128; }
 constexpr int kTileMinTiles = 2;
 int64_t tile_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kSms) * (2 * chitu::kTilePieceFloats * 4 + sizeof(chitu::TileJoin)); }
 
