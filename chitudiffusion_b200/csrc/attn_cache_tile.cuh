@@ -13,13 +13,19 @@
 //                    page, or 128 rows of one; page numbers are the outermost coordinate, and one outside the pool reads
 //                    zeros) and the scales of a tile's sixteen-key groups
 //
+// Measured: 4680 queries over 32760 keys, 12 heads, 8-bit pages of 128: 759 us, 1241 TFLOP/s (attn_persist_kernel on the same keys
+// in 16 bits: 706); four causal chunks of 389 to 512 tokens over up to 8100 keys, 32 query heads over 8, pages of 64: 148 us,
+// 980 TFLOP/s.  A block of one tile's rows has one chain of scores, exponentials and products, and the SM waits for it: split
+// over both halves of the CTA (every second key tile each) 64 such blocks of 16000 keys took 746 us instead of 823, but the
+// code that it needs cost the cases above 0.5 %, and a form of its own with more copies in flight (673) cost shorter ones 3 to 7 %.
+//
 // Widening costs the SM sub-partitions' issue slots (about 100 instructions per warp and tile) rather than a pass over
 // memory: read back from a 16-bit copy of the cache, three frames over 21 would move 200 MB more.
 //
 // Work.  A block's share of the work is the keys it sees, K = the last row's, and kBlockKeys for what a block costs besides (its
-// queries, the first scores, its result).  All blocks in the order (sequence,
-// key head, block) are a line of such keys; CTA c takes the c-th of gridDim.x equal runs of it, and of a block those
-// 128-key tiles whose first key (behind the block's kBlockKeys) lies in its run.  So ragged lengths, causal blocks and few long blocks alike finish together.
+// queries, the first scores, its result).  All blocks in the order (sequence, key head, block) are a line of such keys; CTA c
+// takes the c-th of gridDim.x equal runs of it, and of a block those 128-key tiles whose first key (behind the block's
+// kBlockKeys) lies in its run.  So ragged lengths, causal blocks and few long blocks alike finish together.
 // (Dealing out whole blocks first, so that CTAs walk the same keys at the same time, gained nothing: 790 us against 770 for
 // three frames over 21.)  A block that a run's border cuts leaves fp32 pieces in scratch; attn_cache_join_kernel, launched
 // behind, merges them with all SMs (the CTA that comes last would have up to 148 pieces of 128 KB to itself).
@@ -48,7 +54,7 @@ struct TileJoin {
   int n_pieces;          // 0: there is no such block
   int first;             // where the first piece is; the others are 2 (CTA + 1), 2 (CTA + 2), ...
   int row, n_rows;       // first packed token, query rows
-  int h, unused[3];
+  int h, pad[3];
 };
 // scratch of one piece: per tile [32 column groups][128 rows] float4, then (maximum, sum) of 128 rows
 constexpr int kTilePieceFloats = 2 * (32 * kTileM * 4 + 2 * kTileM);
@@ -70,7 +76,7 @@ struct TileSeg {
   int tok0, n_new, len, first;  // of the sequence
   int h, blk, rows;             // key head, block, query rows
   int piece;                    // where its fp32 piece goes, -1: the result itself
-  int unused[2];
+  int pad[2];
 };
 static_assert(sizeof(TileSeg) == 48, "control block");
 struct TileLine {
@@ -208,9 +214,6 @@ __device__ __forceinline__ void st_global32(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// One softmax step (thread = one row, 128 scores): scores in, probabilities out.  As persist_softmax_step, with a factor and an
-// addend for each sixteen keys (coef: key scale, log2 of the value scale, its inverse) and, in a form of its own that keeps the
-// other one short, `valid` keys visible to this row.  m is the largest (score factor + addend) so far in log2 units, moved only when it has grown by more than 2^8.
 // mbar_wait with its loop in a few instructions: the roles' hot loops share the instruction cache.  As there, a wait ends when
 // the barrier's phase is complete, when another role has given up, or after about a second (2^24 polls of at least 100 cycles).
 __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
@@ -231,6 +234,10 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
   return ok != 0;
 }
 
+// One softmax step (thread = one row, 128 scores): scores in, probabilities out.  As persist_softmax_step, with a factor and an
+// addend for each sixteen keys (coef: key scale, log2 of the value scale, its inverse) and, in a form of its own that keeps the
+// other one short, `valid` keys visible to this row.  m is the largest (score factor + addend) so far in log2 units, moved only
+// when it has grown by more than 2^8.
 template <bool kHalf, bool kMasked>
 __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, bool first, int valid, float row_factor, const float4* coef,
                                                   float& m, float& l_sum, volatile int* abort_flag, int* status) {

@@ -544,8 +544,8 @@ int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const 
  * behind a sequence's length are never read; those within it have to be finite.  softmax_scale must be positive.
  *
  * max_q and max_kv are how many queries and keys the longest sequence is expected to have: they choose the kernel and its grid,
- * and results are right whatever the lengths turn out to be (the work is shared out on the device).  workspace: chitu_b200_attn_cache_workspace_bytes(...) bytes,
- * 16-byte aligned, its first CHITU_SPLITKV_HEADER_BYTES zero before the first call and left zero by each (rules as for
+ * and results are right whatever the lengths turn out to be (the work is shared out on the device).
+ * workspace: chitu_b200_attn_cache_workspace_bytes(...) bytes, 16-byte aligned, its first CHITU_SPLITKV_HEADER_BYTES zero before the first call and left zero by each (rules as for
  * chitu_b200_attn_fwd_splitkv, with which it may be shared).
  */
 int64_t chitu_b200_attn_cache_workspace_bytes(int heads, int q_heads, int max_q);
