@@ -926,7 +926,8 @@ def rotary(x, positions: torch.Tensor, rope_table: torch.Tensor, interleaved: bo
     (cos, sin) pairs ``[rows, rot / 2, 2]``; see ``pre_attention.scaled_rope_table``); the others pass, and so do tokens whose
     position is outside the table.  Pairs are adjacent channels, as everywhere in this library, or with
     ``interleaved=False`` channels ``(j, j + rot / 2)``.  bf16, fp16 or fp32 in and out; ``D`` and ``rot`` multiples of 16.
-    ``out`` (a tensor, or one per tensor of the list) may be ``x`` itself.  ``[B, S, H, D]`` tensors are taken as ``B * S`` tokens.
+    ``out`` (a tensor, or one per tensor of the list) may be ``x`` itself, each in its own place; other overlaps are refused as
+    far as they begin at one address.  ``[B, S, H, D]`` tensors are taken as ``B * S`` tokens.
     See ``chitu_b200_rotary``.
     """
     single = isinstance(x, torch.Tensor)
@@ -971,6 +972,10 @@ def rotary(x, positions: torch.Tensor, rope_table: torch.Tensor, interleaved: bo
         heads.append(s[-2])
         keep.append(rows)
         results.append(o)
+    if out is not None and n_tokens:
+        for i, at in enumerate(out_ptrs):
+            if at in out_ptrs[:i] or any(at == p and (i != j or strides[2 * i:2 * i + 2] != out_strides[2 * i:2 * i + 2]) for j, p in enumerate(ptrs)):
+                raise ValueError("rotary: an output may only take the place of its own input, with its strides")
     if on < 0:
         _require_cuda(first)
     if positions.get_device() != on or rope_table.get_device() != on:
@@ -1072,7 +1077,7 @@ def kv_cache_append(
     the last sequence are left alone.
 
     With ``rope_table`` keys turn by the row of their position, or of ``positions [T]`` where given (a clip's per-token rows), and
-    ``q [T, Hq, 128]``, if given, is rotated by the same launch and returned.  ``max_new`` is how many tokens the longest sequence
+    ``q [T, Hq, 128]``, if given, is rotated by the same launch and returned (rows behind the last sequence are not written).  ``max_new`` is how many tokens the longest sequence
     brings (default: the average); it sizes the launch, results do not depend on it.
     """
     what = "kv_cache_append"

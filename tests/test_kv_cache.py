@@ -43,6 +43,7 @@ def _attend(**change):
 
 
 TABLE = torch.zeros(64, 64, 2)
+X, Y = torch.zeros(5, 2, 128), torch.zeros(5, 2, 128)
 
 CACHE_REFUSALS = [
     (dict(k_cache=torch.zeros(4, 16, 2, 64, dtype=E4M3), v_cache=torch.zeros(4, 16, 2, 64, dtype=E4M3)), NotImplementedError, "head_dim"),
@@ -135,6 +136,11 @@ def test_attention_refusals(change, error, text):
     ([torch.zeros(5, 2, 128)] * 2, dict(out=[torch.zeros(5, 2, 128)]), ValueError, "as many outputs"),
     (torch.zeros(5, 2, 128), dict(out=torch.zeros(5, 2, 128, dtype=BF16)), ValueError, "out must"),
     (torch.zeros(5, 2, 128), dict(out=torch.zeros(5, 2, 130)[..., :128]), ValueError, "16-byte aligned"),
+    ([X, torch.zeros(5, 2, 128)], dict(out=[Y, Y]), ValueError, "its own input"),
+    ([X, Y], dict(out=[Y, X]), ValueError, "its own input"),
+    ([X, X], dict(out=[X, X]), ValueError, "its own input"),
+    (X, dict(out=X.view(2, 5, 128).transpose(0, 1)), ValueError, "its own input"),
+    ([X, Y], dict(out=[X, Y]), RuntimeError, "CUDA tensors only"),
     (torch.zeros(5, 2, 128), dict(), RuntimeError, "CUDA tensors only"),
 ])
 def test_rotary_refusals(x, change, error, text):
