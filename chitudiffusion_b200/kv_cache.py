@@ -157,6 +157,8 @@ class PagedKVCache:
             lens = self._new if q_lens is None else [int(n) for n in q_lens]
             if len(lens) != self.batch or min(lens) < 0 or sum(lens) > q.shape[0]:
                 raise ValueError("PagedKVCache: packed queries need q_lens, one per sequence, of no more tokens than there are")
+        if out is not None and (out.shape != q.shape or not out.is_contiguous()):
+            raise ValueError(f"PagedKVCache: out must be contiguous, of q's shape {tuple(q.shape)}")
         args = self.tensors
         if lens != self._new:
             ends = [0]

@@ -264,6 +264,12 @@ def test_paged_cache_bookkeeping(monkeypatch):
     assert (used >= 0).sum().item() == 4 and used[used >= 0].unique().numel() == 4
     cache.attend(torch.zeros(3, 3, 128, dtype=BF16), q_lens=[1, 2])
     assert calls.seen[-1][3] == [0, 1, 3] and calls.seen[-1][5]["max_kv"] == 38
+    # an output that would be copied to be written is refused
+    cache.attend(q, out=torch.zeros_like(q))
+    assert calls.seen[-1][5]["out"].shape == (10, 6, 128)
+    for wrong in (torch.zeros(5, 2, 6, 128, dtype=BF16).transpose(0, 1), torch.zeros(10, 6, 128, dtype=BF16)):
+        with pytest.raises(ValueError, match="contiguous"):
+            cache.attend(q, out=wrong)
     # no page left: refused, nothing changes
     with pytest.raises(RuntimeError, match="free"):
         cache.append(tokens(90), tokens(90), [0, 90])
