@@ -103,7 +103,8 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
 // item's count merges its pieces in order; nobody waits.
 //
 // 64 sequences of 3 to 16300 keys, one token each, 32 query heads over 8, 8-bit pages of 64: 190 us, 5.7 TB/s of keys and values (four
-// times as long: 6.5 TB/s, the rate of a copy); two of 125000 in pages of 16: 101 us; 16-bit pages of 32, 16 sequences of 500 to 8191: 105 us,
+// times as long: 6.5 TB/s, the rate of a copy); two of 125000 in pages of 16: 96 us (101 with a merge of 28 pieces in four
+// turns rather than two); 16-bit pages of 32, 16 sequences of 500 to 8191: 105 us,
 // 5.4 TB/s.  The first version, a block per 256 keys and loads through registers, took 329, 183 and 178.
 //
 // A warp takes 32 (16-bit pages: 16) of a tile's keys and keeps its own softmax.  The matrix instructions' sum over channels and the
@@ -607,10 +608,12 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
         __syncthreads();
         write = *last_flag != 0;
         if (write) {
-          // Pieces in their order, three or seven at a time through the warp's stage (in registers they cost the main loop its own:
-          // spills, half the speed): this warp's accumulators of a piece, then its 16 rows' statistics.
+          // Pieces in their order through the warp's stage (in registers they cost the main loop its own: spills, half the speed),
+          // or all of its stages where the run is over: this warp's accumulators of a piece, then its 16 rows' statistics.
           const int n_pieces = c_last - c_first + 1;
-          const int region = n_halves * 1024 + 128, at_once = n_halves == 1 ? 7 : 3;
+          const int region = n_halves * 1024 + 128;
+          const uint32_t room = step + 1 == n_steps ? ring : src;
+          const int at_once = (step + 1 == n_steps ? kStages : 1) * Shape::step_bytes / region;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             m_row[i] = -INFINITY;
@@ -624,7 +627,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 #pragma unroll 1
             for (int k = 0; k < n; ++k) {
               const float* from = piece(c_first + k0 + k);
-              const uint32_t to = src + k * region;
+              const uint32_t to = room + k * region;
 #pragma unroll 1
               for (int part = lane; part < n_halves * 64; part += 32)  // 16 bytes: two lanes' pairs of one accumulator
                 cp_async16(to + part * 16, from + (part >> 6) * 1024 + warp * 256 + (part & 63) * 4);
@@ -638,7 +641,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
               if (i >= n_halves) break;
 #pragma unroll 1
               for (int k = 0; k < n; ++k) {
-                const uint32_t at = src + k * region;
+                const uint32_t at = room + k * region;
                 float2 st;
                 asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(st.x), "=f"(st.y) : "r"(at + region - 128 + (g + 8 * i) * 8) : "memory");
                 const float top = fmaxf(m_row[i], st.x);
