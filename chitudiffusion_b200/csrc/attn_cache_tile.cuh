@@ -31,6 +31,8 @@
 // behind, merges them with all SMs (the CTA that comes last would have up to 148 pieces of 128 KB to itself).
 #pragma once
 
+#include <cfloat>
+
 #include "attn_cache.cuh"
 
 namespace chitu {
@@ -237,7 +239,8 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
 // One softmax step (thread = one row, 128 scores): scores in, probabilities out.  As persist_softmax_step, with a factor and an
 // addend for each sixteen keys (coef: key scale, log2 of the value scale, its inverse) and, in a form of its own that keeps the
 // other one short, `valid` keys visible to this row.  m is the largest (score factor + addend) so far in log2 units, moved only
-// when it has grown by more than 2^8.
+// when it has grown by more than 2^8.  Hidden scores are -inf before they meet their factor, which therefore is not allowed
+// to vanish there: a row of zeros has 2^-126 of its own, and a small key scale would take it to 0 and the score to NaN.
 template <bool kHalf, bool kMasked>
 __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, bool first, int valid, float row_factor, const float4* coef,
                                                   float& m, float& l_sum, volatile int* abort_flag, int* status) {
@@ -253,6 +256,10 @@ __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, b
     for (int i = 0; i < 128; ++i)
       if (i >= valid) s[i >> 5][i & 31] = 0xff800000u;  // -inf
   }
+  auto factor = [&](const float4& k) {
+    const float f = row_factor * k.x;
+    return kMasked ? fmaxf(f, FLT_MIN) : f;
+  };
   float mx = -INFINITY;
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
@@ -265,7 +272,7 @@ __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, b
     b = max3(b, __uint_as_float(x[12]), __uint_as_float(x[13]));
     a = max3(a, __uint_as_float(x[14]), __uint_as_float(x[15]));
     const float4 k = coef[c];
-    mx = fmaxf(mx, fmaf(fmaxf(a, b), row_factor * k.x, k.y));
+    mx = fmaxf(mx, fmaf(fmaxf(a, b), factor(k), k.y));
   }
   if (first) {
     m = mx;
@@ -299,7 +306,7 @@ __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, b
     for (int q = 0; q < 4; ++q) {
       const int c = half * 4 + q;
       const float4 k = coef[c];
-      const float f = row_factor * k.x, add = k.y + shift;
+      const float f = factor(k), add = k.y + shift;
       const float2 f2 = make_float2(f, f), add2 = make_float2(add, add);
       const uint32_t* x = &s[c >> 1][(c & 1) * 16];
       float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);

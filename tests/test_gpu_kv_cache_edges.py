@@ -1,0 +1,76 @@
+"""Paged key/value cache on the GPU: rows and scales at the ends of their range, strides other than the plain ones, the class
+without waits, what a call counts.
+
+Tolerances as in test_gpu_kv_cache.py unless a test says otherwise.
+"""
+
+import math
+
+import pytest
+import torch
+
+import _kv_cache_model as model
+from test_gpu_kv_cache import _attention_close, _equal
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def _ops():
+    from chitudiffusion_b200 import ops
+
+    return ops
+
+
+# ------------------------------------------------------------------------------------------------ queries of nothing
+@pytest.mark.parametrize("key_scale", [0.0, 2.0 ** -126, 2.0 ** -22, 2.0 ** -7])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("n", [3, 40, 300])  # few rows; one tile of a block; blocks of two, and the diagonal in several
+@pytest.mark.parametrize("causal", [True, False])
+def test_zero_and_tiny_query_rows(n, dtype, key_scale, causal):
+    """A zero query weighs all visible keys alike, whatever the keys' scale is: the mean of the values, and log(their number)."""
+    gen = torch.Generator().manual_seed(n)
+    heads, group, page, lens = 2, 2, 32, [430, n]
+    (kc, ks), (vc, vs) = (model.make_cache(gen, 26, page, heads, dtype, True) for _ in range(2))
+    table = model.make_tables(gen, lens, page, 26)
+    ks[table[0, 3:].long()] = key_scale  # of some pages only: others have ordinary ones
+    ks[table[1].clamp(min=0).long()] = key_scale
+    q = torch.randn(2 * n, heads * group, 128, generator=gen).to(dtype)
+    q[::2] = 0.0
+    q[1, 0], q[1, 1] = torch.finfo(dtype).tiny, -torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    lens_t, cu = torch.tensor(lens, dtype=torch.int32), torch.tensor([0, n, 2 * n], dtype=torch.int32)
+    ref = model.attend(q, kc, vc, ks, vs, table, lens_t, cu, 128 ** -0.5, causal)
+    out, lse = _ops().attn_fwd_cache(*[t.cuda() for t in (q, kc, vc, table, lens_t, cu)], k_scale=ks.cuda(), v_scale=vs.cuda(), causal=causal,
+                                     return_lse=True, max_q=n)
+    _attention_close(out, lse, ref, dtype, True)
+    seen = torch.cat([torch.arange(length - n, length) + 1 if causal else torch.full((n,), length) for length in lens])
+    assert (lse.cpu().double()[:, ::2] - seen[::2].double().log()).abs().max() <= 1.4e-4
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("n", [7, 40, 300])
+def test_tokens_of_nothing_appended_and_attended_to(n, dtype):
+    """Zeros through append and attention, as padding or a first run on empty inputs gives them; values are ordinary in between."""
+    ops, heads, group, page = _ops(), 2, 2, 64
+    gen = torch.Generator().manual_seed(n)
+    (kc, ks), (vc, vs) = (model.make_cache(gen, 12, page, heads, dtype, True) for _ in range(2))
+    dev = [t.cuda() for t in (kc, vc, ks, vs)]
+    table, rope = torch.randperm(12, generator=gen).int()[None], model.rope_table(128, 700)
+    zeros = torch.zeros(n, heads, 128, dtype=dtype)
+    v = torch.randn(n, heads, 128, generator=gen).to(dtype)
+    v[: n // 2] = 0.0
+    q, cu = torch.zeros(n, heads * group, 128, dtype=dtype), torch.tensor([0, n], dtype=torch.int32)
+    for step in (1, 2):
+        lens = torch.tensor([step * n], dtype=torch.int32)
+        turned = ops.kv_cache_append(zeros.cuda(), v.cuda(), dev[0], dev[1], table.cuda(), lens.cuda(), cu.cuda(), k_scale=dev[2], v_scale=dev[3],
+                                     rope_table=rope.cuda(), q=q.cuda())
+        for x, c, s in ((zeros.float(), kc, ks), (v.float(), vc, vs)):
+            model.append(x, c, s, table, lens, cu)
+        for got, want in zip(dev, (kc, vc, ks, vs)):
+            assert torch.equal(got.float().cpu(), want.float())  # (values: a rotated zero may have either sign)
+        for causal in (True, False):
+            ref = model.attend(q, kc, vc, ks, vs, table, lens, cu, 128 ** -0.5, causal)
+            out, lse = ops.attn_fwd_cache(turned, dev[0], dev[1], table.cuda(), lens.cuda(), cu.cuda(), k_scale=dev[2], v_scale=dev[3],
+                                          causal=causal, return_lse=True)
+            _attention_close(out, lse, ref, dtype, True)
