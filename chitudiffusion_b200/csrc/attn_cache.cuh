@@ -14,6 +14,8 @@
 // 2^-24 of its largest before fp16 drops any of their bits), which goes into the score's factor.
 #pragma once
 
+#include <cfloat>
+
 #include "attn_persist.cuh"
 #include "kv_cache.cuh"
 
@@ -60,7 +62,12 @@ __device__ __forceinline__ SeqInfo seq_info(const CacheAttnParams& p, int b) {
 // probabilities are kept at up to 2^(kProbShift + kRescaleThreshold) in fp16, whose range would otherwise end 2^-24 below
 // the row's maximum
 constexpr float kProbShift = 7.f;
-constexpr float kMinValueScale = 1e-30f;  // (a value scale of zero has no logarithm; its codes are zero)
+// A value scale of zero has no logarithm: it counts as the smallest normal number.  l = sum p / vs has to stay finite, so the
+// running maximum takes scales below 2^-82 for 2^-82: a weight p / vs is then at most 2^(15 + 82), and a sequence has at most
+// 2^30 keys.  Probabilities keep the true scale, so where all scales of a row are below 2^-82 by 2^x, its largest ones come to
+// 2^(7 - x) and end in fp16's last steps of 2^-24: values of 2^-100 still have most of their bits, those near 2^-117 are zeros.
+constexpr float kMinValueScale = FLT_MIN;
+constexpr float kLowValueLog2 = -82.f;
 
 __device__ __forceinline__ void mma_16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -434,7 +441,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int half = 0; half < kHalves; ++half) {
-      float k_scale = 1.f, v_log2 = 0.f;
+      float k_scale = 1.f, v_log2 = 0.f, lift = 0.f;
       v_inv[half] = 1.f;
       if constexpr (kEightBit) {
         k_scale = __uint_as_float(half ? scales.z : scales.x);
@@ -445,6 +452,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           k_scale = v_inv[half] = 1.f;
           v_log2 = 0.f;
         }
+        lift = fmaxf(kLowValueLog2 - v_log2, 0.f);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -461,7 +469,7 @@ attn_cache_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
             for (int e = 0; e < 2; ++e)
               if ((half ? there.y : there.x) == 0 || key0 + 8 * n + 2 * c + e >= limit[i]) s[n][2 * i + e] = -INFINITY;
         }
-        top[i] = max3(top[i], max3(s[2 * half][2 * i], s[2 * half][2 * i + 1], s[2 * half + 1][2 * i]), s[2 * half + 1][2 * i + 1]);
+        top[i] = fmaxf(top[i], fmaxf(max3(s[2 * half][2 * i], s[2 * half][2 * i + 1], s[2 * half + 1][2 * i]), s[2 * half + 1][2 * i + 1]) + lift);
       }
     }
     if (__any_sync(0xffffffffu, top[0] > ceiling[0] || top[1] > ceiling[1])) {

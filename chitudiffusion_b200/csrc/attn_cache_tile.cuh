@@ -31,8 +31,6 @@
 // behind, merges them with all SMs (the CTA that comes last would have up to 148 pieces of 128 KB to itself).
 #pragma once
 
-#include <cfloat>
-
 #include "attn_cache.cuh"
 
 namespace chitu {
@@ -237,9 +235,9 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 // One softmax step (thread = one row, 128 scores): scores in, probabilities out.  As persist_softmax_step, with a factor and an
-// addend for each sixteen keys (coef: key scale, log2 of the value scale, its inverse) and, in a form of its own that keeps the
-// other one short, `valid` keys visible to this row.  m is the largest (score factor + addend) so far in log2 units, moved only
-// when it has grown by more than 2^8.  Hidden scores are -inf before they meet their factor, which therefore is not allowed
+// addend for each sixteen keys (coef: key scale, log2 of the value scale, the scale's inverse, the logarithm as the maximum takes
+// it) and, in a form of its own that keeps the other one short, `valid` keys visible to this row.  m is the largest (score factor +
+// addend) so far in log2 units, moved only when it has grown by more than 2^8.  Hidden scores are -inf before they meet their factor, which therefore is not allowed
 // to vanish there: a row of zeros has 2^-126 of its own, and a small key scale would take it to 0 and the score to NaN.
 template <bool kHalf, bool kMasked>
 __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, bool first, int valid, float row_factor, const float4* coef,
@@ -272,7 +270,7 @@ __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, b
     b = max3(b, __uint_as_float(x[12]), __uint_as_float(x[13]));
     a = max3(a, __uint_as_float(x[14]), __uint_as_float(x[15]));
     const float4 k = coef[c];
-    mx = fmaxf(mx, fmaf(fmaxf(a, b), factor(k), k.y));
+    mx = fmaxf(mx, fmaf(fmaxf(a, b), factor(k), k.w));
   }
   if (first) {
     m = mx;
@@ -476,11 +474,13 @@ attn_cache_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
           {
             const int from = __shfl_sync(0xffffffffu, page, (lane * 16 >> box_shift) & 31);
             if (lane < 8) {
-              float4 k = make_float4(1.f, from < 0 ? -INFINITY : 0.f, 1.f, 0.f);
+              const float hidden = from < 0 ? -INFINITY : 0.f;
+              float4 k = make_float4(1.f, hidden, 1.f, hidden);
               if (kEightBit && from >= 0) {
                 const float ks = __ldg(p.scale[0] + from * p.s_page[0] + walk.w.h * p.s_head[0]);
                 const float vs = fmaxf(__ldg(p.scale[1] + from * p.s_page[1] + walk.w.h * p.s_head[1]), kMinValueScale);
-                k = make_float4(fmaxf(ks, 1e-30f), __log2f(vs), __fdividef(1.f, vs), 0.f);
+                const float log2_vs = __log2f(vs);
+                k = make_float4(ks, log2_vs, __fdividef(1.f, vs), fmaxf(log2_vs, kLowValueLog2));
               }
               coef_ring[(tiles % kCoefStages) * 8 + lane] = k;
             }

@@ -74,3 +74,54 @@ def test_tokens_of_nothing_appended_and_attended_to(n, dtype):
             out, lse = ops.attn_fwd_cache(turned, dev[0], dev[1], table.cuda(), lens.cuda(), cu.cuda(), k_scale=dev[2], v_scale=dev[3],
                                           causal=causal, return_lse=True)
             _attention_close(out, lse, ref, dtype, True)
+
+
+# ------------------------------------------------------------------------------------------------ scales of values
+@pytest.mark.parametrize("exponents", [(-126,), (-104,), (-100, -96), (-99, -126, -80), (-60, -30), (-8, 90), (110,)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_value_scales_of_any_exponent(n, exponents):
+    """Values as small as a bf16 can be, and as large: scales that the append gives them.
+
+    A probability is held in fp16 with the value's scale in its exponent; scales below 2^-82 are below the largest by as much as they
+    are smaller, and fp16 ends in steps of 2^-24, half of which is a probability's error, against a largest one of at
+    least 2^(7 - x) for scales of 2^(-82 - x): 2^(x - 32) of the largest weight for every key, or all of it where that is more than 1."""
+    gen = torch.Generator().manual_seed(n)
+    heads, group, page, length = 2, 4, 32, 300
+    (kc, ks), (vc, vs) = (model.make_cache(gen, 10, page, heads, BF16, True) for _ in range(2))
+    for p in range(10):
+        vs[p] = 2.0 ** exponents[p % len(exponents)]
+    table, lens = torch.randperm(10, generator=gen).int()[None], torch.tensor([length], dtype=torch.int32)
+    q, cu = torch.randn(n, heads * group, 128, generator=gen).to(BF16), torch.tensor([0, n], dtype=torch.int32)
+    out, lse = _ops().attn_fwd_cache(*[t.cuda() for t in (q, kc, vc, table, lens, cu)], k_scale=ks.cuda(), v_scale=vs.cuda(), return_lse=True,
+                                     max_q=n)
+    want, want_lse, mag = model.attend(q, kc, vc, ks, vs, table, lens, cu, 128 ** -0.5, False)
+    assert ((lse.double().cpu() - want_lse).abs() <= 1.4e-4 + 1e-6 * want_lse.abs()).all()
+    below = max(0, -82 - max(exponents))
+    v, _ = model.gathered(vc, vs, table[0], length)
+    steps = min(1.0, 2.0 ** (below - 32)) * v.abs().sum(0).repeat_interleave(group, 0)[None]
+    # (a bf16 ends in steps of 2^-133)
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2 * 1.4e-4) * 1.01 * mag + steps + 2.0 ** -133
+    got = out.double().cpu()
+    assert torch.isfinite(got).all() and ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_many_keys_without_values(n):
+    """Values of zero have the smallest scale: their weights' sum stays finite over long sequences, and so does the log-sum-exp.
+
+    All keys after a sequence's first page score the same, 5 above the first page's (below the 2^8 at which a running maximum moves)."""
+    heads, page, batch, length = 8, 256, 40, 30000
+    pages = 1 + -(-length // page)
+    kc = torch.zeros(pages, page, heads, 128)
+    q = torch.zeros(n * batch, heads, 128, dtype=FP16)
+    q[..., 0] = 1.0
+    kc[1:, :, :, 0] = 5.0
+    kc, vc = kc.to(E4M3).cuda(), torch.zeros(pages, page, heads, 128, dtype=E4M3, device="cuda")
+    ks, vs = torch.ones(pages, heads, device="cuda"), torch.full((pages, heads), 2.0 ** -126, device="cuda")
+    table = torch.arange(pages - 1, dtype=torch.int32).clamp(min=0)[None].repeat(batch, 1)
+    lens, cu = torch.full((batch,), length, dtype=torch.int32), n * torch.arange(batch + 1, dtype=torch.int32)
+    out, lse = _ops().attn_fwd_cache(q.cuda(), kc, vc, table.cuda(), lens.cuda(), cu.cuda(), k_scale=ks, v_scale=vs, softmax_scale=1.0,
+                                     return_lse=True, max_q=n)
+    want = math.log(page + (length - page) * math.exp(5.0))
+    assert (out == 0).all()
+    assert ((lse - want).abs() <= 1.4e-4).all(), lse.min().item()
