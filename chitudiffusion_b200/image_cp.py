@@ -153,7 +153,10 @@ class B200ImageContextParallel:
         key = (self._cur_tag, layer)
         if self._kvcache_is_fresh() or key not in self._kvcache:
             full_k, full_v = self.all_gather_seq(img_k), self.all_gather_seq(img_v)
-            self._kvcache[key] = self._paged_others(key, full_k, full_v) if self._kvcache_fp8 else (full_k.detach(), full_v.detach())
+            if self._kvcache_fp8 and self._group.group_size > 1:
+                self._kvcache[key] = self._paged_others(key, full_k, full_v)
+            else:  # (a group of one has no other ranks' rows to keep in pages)
+                self._kvcache[key] = (full_k.detach(), full_v.detach())
             return full_k, full_v
         cached_k, cached_v = self._kvcache[key]
         n = img_k.shape[1]
@@ -167,7 +170,7 @@ class B200ImageContextParallel:
         B, S, H, _ = full_k.shape
         n = S // self._group.group_size
         cache = self._kvcache.get(key)
-        if cache is None or (cache.batch, cache.num_heads, cache.max_tokens) != (B, H, S - n):
+        if not isinstance(cache, PagedKVCache) or (cache.batch, cache.num_heads, cache.max_tokens) != (B, H, S - n):
             cache = PagedKVCache(B, H, S - n, page_size=128, device=full_k.device)
         for b in range(B):
             cache.truncate(b)
@@ -199,8 +202,9 @@ class B200ImageContextParallel:
         if self._kvcache_enabled and self._cur_step is not None:
             layer = self._layer_idx
             self._layer_idx += 1
-            if self._kvcache_fp8 and not self._kvcache_is_fresh() and (self._cur_tag, layer) in self._kvcache:
-                return self._attn_agkv_stale_fp8(self._kvcache[(self._cur_tag, layer)], txt_q, txt_k, txt_v, img_q, img_k, img_v)
+            kept = self._kvcache.get((self._cur_tag, layer))
+            if isinstance(kept, PagedKVCache) and not self._kvcache_is_fresh():
+                return self._attn_agkv_stale_fp8(kept, txt_q, txt_k, txt_v, img_q, img_k, img_v)
             full_k, full_v = self._agkv_gather_cached(layer, img_k, img_v)
         else:
             full_k, full_v = self.all_gather_seq_fp8(img_k), self.all_gather_seq_fp8(img_v)

@@ -125,3 +125,60 @@ def test_many_keys_without_values(n):
     want = math.log(page + (length - page) * math.exp(5.0))
     assert (out == 0).all()
     assert ((lse - want).abs() <= 1.4e-4).all(), lse.min().item()
+
+
+# ------------------------------------------------------------------------------------------------ the cross-step cache's ranks
+def _image_cp(monkeypatch, cp, world, rank, n, B=2, H=2):
+    """`cp` as rank `rank` of `world` with shards of `n` rows and 8-bit pages, every second step stale, and what draws its inputs; the other
+    ranks' rows of a step are drawn when they are gathered and kept in `cp.far`."""
+    gen = torch.Generator(device="cuda").manual_seed(10 * world + rank)
+
+    def draw(rows):
+        return torch.randn(B, rows, H, 128, generator=gen, device="cuda").to(BF16)
+
+    class Group:
+        group_size, rank_in_group = world, rank
+
+        def all_gather_sequence(self, t):
+            others = [draw(n) for _ in range(world - 1)]
+            cp.far = (cp.far + [others])[-2:]
+            return torch.cat(others[:rank] + [t] + others[rank:], 1)
+
+    cp.far = []
+    cp._kvcache_enabled = cp._kvcache_fp8 = True
+    cp._kvcache_warmup, cp._kvcache_interval, cp._kvcache_tail = 0, 2, 0
+    cp.enable(Group())
+    return cp, draw
+
+
+@pytest.mark.parametrize("n", [150, 128, 37])
+@pytest.mark.parametrize("world,rank", [(1, 0), (2, 0), (2, 1), (3, 0), (3, 1), (3, 2)])
+def test_image_cache_in_8_bits_on_every_rank(monkeypatch, world, rank, n):
+    """Fresh and stale steps of a rank that has others on one side of it, on both sides (pages that two appends share), or none.
+
+    Tolerance as in test_image_cache_of_other_ranks_in_8_bits, against attention over the kept rows as their codes say; those
+    are the gathered rows to half a step of e4m3 (2^-4), twice where a page's earlier codes move to a larger scale."""
+    from chitudiffusion_b200 import B200AttnBackend
+    from chitudiffusion_b200.image_cp import B200ImageContextParallel
+    from test_gpu_kv_cache import SCORE, _dense, _held
+
+    cp, draw = _image_cp(monkeypatch, B200ImageContextParallel(B200AttnBackend("b200"), mode="agkv"), world, rank, n)
+    for step in range(4):
+        cp.begin_forward(step, 100)
+        tq, tk, tv, iq, ik, iv = (draw(rows) for rows in (20, 20, 20, n, n, n))
+        gathered = len(cp.far)
+        txt, img = cp.attention(tq, tk, tv, iq, ik, iv)
+        for b in range(2):
+            keys = [torch.cat([t[b] for t in others] + [ik[b][:0]]).cpu() for others in cp.far]
+            if step % 2 and world > 1:
+                kept = _held(cp._kvcache[("cond", 0)], b)
+                for exact, got in zip(keys, kept):
+                    exact = exact.double()
+                    assert ((got - exact).abs() <= 2 * 2 ** -4 * exact.abs() + 2 ** -9 * 2.0 ** -6).all()
+                keys = kept
+            k, v = (torch.cat([x.double(), own[b].cpu().double(), t[b].cpu().double()]) for x, own, t in zip(keys, (ik, iv), (tk, tv)))
+            want, _, mag = _dense(torch.cat([iq[b], tq[b]]).cpu(), k, v)
+            got = torch.cat([img[b], txt[b]]).double().cpu()
+            tol = 2 ** -8 * want.abs() + 1.02 * (2 ** -7 + 2 * SCORE) * mag + 1e-6
+            assert ((got - want).abs() <= tol).all(), (step, ((got - want).abs() / tol).max().item())
+        assert world == 1 or step % 2 == 0 or len(cp.far) == gathered  # a stale step gathers nothing

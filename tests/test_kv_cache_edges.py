@@ -1,0 +1,58 @@
+"""Paged key/value cache without a GPU: bookkeeping of calls that fail, ranks of the cross-step cache, tables, launch hints."""
+
+import math
+
+import pytest
+import torch
+
+import oracle
+from chitudiffusion_b200 import PagedKVCache, ops
+from chitudiffusion_b200.image_cp import B200ImageContextParallel
+
+BF16, FP16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+# ------------------------------------------------------------------------------------------------ the cross-step cache
+class _Backend:
+    impl = "torch_sdpa"
+
+    def __call__(self, q, k, v, *_, softmax_scale=None, return_attn_probs=False, **__):
+        out, lse = oracle.sdpa_fp32(q, k, v, softmax_scale, return_lse=True)
+        return out.to(q.dtype), (lse if return_attn_probs else None), None
+
+
+class _Group:
+    """A rank of a group whose other ranks' rows are drawn."""
+
+    def __init__(self, world, rank, others=None):
+        self.group_size, self.rank_in_group, self.others = world, rank, others
+
+    def all_gather_sequence(self, t):
+        rows = [] if self.others is None else self.others(t)
+        return torch.cat(rows[:self.rank_in_group] + [t] + rows[self.rank_in_group:], 1)
+
+
+def _schedule(monkeypatch, group, eight):
+    for name, value in (("CHITU_CP_KV_CACHE", "1"), ("CHITU_CP_KV_CACHE_WARMUP", "0"), ("CHITU_CP_KV_CACHE_INTERVAL", "2"),
+                        ("CHITU_CP_KV_CACHE_TAIL", "0"), ("CHITU_B200_KV_CACHE_FP8", "1" if eight else "0")):
+        monkeypatch.setenv(name, value)
+    cp = B200ImageContextParallel(_Backend(), mode="agkv")
+    cp.enable(group)
+    return cp
+
+
+def test_image_cache_of_a_group_of_one(monkeypatch):
+    """A group without other ranks has nothing to keep in pages: fresh and stale steps are those of the 16-bit cache."""
+    gen = torch.Generator().manual_seed(1)
+    calls = [[torch.randn(2, rows, 2, 128, generator=gen) for rows in (3, 3, 3, 10, 10, 10)] for _ in range(4)]
+    outs = []
+    for eight in (False, True):
+        cp = _schedule(monkeypatch, _Group(1, 0), eight)
+        outs.append([])
+        for step, args in enumerate(calls):
+            cp.begin_forward(step, 100)
+            outs[-1] += cp.attention(*args)
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and len(outs[1]) == 8
+    txt_q, txt_k, txt_v, img_q, img_k, img_v = calls[1]  # a stale step: the fresh shard is all there is
+    want = oracle.sdpa_fp32(torch.cat([txt_q, img_q], 1), torch.cat([txt_k, img_k], 1), torch.cat([txt_v, img_v], 1))
+    assert (torch.cat(outs[1][2:4], 1) - want).abs().max() < 2e-6
