@@ -166,10 +166,11 @@ class B200ImageContextParallel:
         return full_k, full_v
 
     def _paged_others(self, key: tuple, full_k: torch.Tensor, full_v: torch.Tensor) -> PagedKVCache:
-        """The other ranks' rows of a gathered layer in 8-bit pages; a layer's cache is used again from step to step."""
+        """The other ranks' rows of a gathered layer in 8-bit pages; a layer's cache is used again from step to step (and is nobody's
+        while it is filled: should that fail, the next step gathers)."""
         B, S, H, _ = full_k.shape
         n = S // self._group.group_size
-        cache = self._kvcache.get(key)
+        cache = self._kvcache.pop(key, None)
         if not isinstance(cache, PagedKVCache) or (cache.batch, cache.num_heads, cache.max_tokens) != (B, H, S - n):
             cache = PagedKVCache(B, H, S - n, page_size=128, device=full_k.device)
         for b in range(B):

@@ -56,3 +56,37 @@ def test_image_cache_of_a_group_of_one(monkeypatch):
     txt_q, txt_k, txt_v, img_q, img_k, img_v = calls[1]  # a stale step: the fresh shard is all there is
     want = oracle.sdpa_fp32(torch.cat([txt_q, img_q], 1), torch.cat([txt_k, img_k], 1), torch.cat([txt_v, img_v], 1))
     assert (torch.cat(outs[1][2:4], 1) - want).abs().max() < 2e-6
+
+
+def test_a_layer_whose_refill_fails_is_not_attended_to(monkeypatch):
+    """The pages of a layer are filled again in place: where that ends half way the layer has no cache, and the next step gathers."""
+    appended = []
+
+    def append(k, v, **_):
+        appended.append(k.shape[0])
+        if len(appended) == 4:
+            raise RuntimeError("no memory left")
+
+    monkeypatch.setattr(ops, "kv_cache_append", append)
+    gen = torch.Generator().manual_seed(1)
+    gathered = []
+
+    def others(t):
+        gathered.append([torch.randn(t.shape, generator=gen) for _ in range(2)])
+        return gathered[-1]
+
+    group = _Group(3, 1, others)
+    cp = _schedule(monkeypatch, group, True)
+    cp._attn_agkv_stale_fp8 = lambda *a: pytest.fail("stale pages were attended to")
+    args = [torch.randn(1, rows, 2, 128, generator=gen) for rows in (3, 3, 3, 10, 10, 10)]
+    cp.begin_forward(0, 100)
+    cp.attention(*args)
+    cp.begin_forward(2, 100)
+    with pytest.raises(RuntimeError, match="memory"):
+        cp.attention(*args)
+    cp.begin_forward(3, 100)  # stale by its number
+    _, got = cp.attention(*args)
+    assert appended == [10] * 6 and len(gathered) == 6
+    (k0, k2), (v0, v2) = gathered[-2:]
+    k, v = (torch.cat([a, own, b, text], 1) for a, own, b, text in ((k0, args[4], k2, args[1]), (v0, args[5], v2, args[2])))
+    assert (got - oracle.sdpa_fp32(args[3], k, v)).abs().max() < 2e-6
