@@ -107,8 +107,11 @@ class PagedKVCache:
         """Forget what ``sequence`` holds behind its first ``tokens`` tokens; its pages behind them are free again."""
         if not 0 <= sequence < self.batch or not 0 <= tokens <= self._host_lens[sequence]:
             raise ValueError("PagedKVCache: no such sequence, or it holds fewer tokens")
-        pages = self._pages[sequence]
-        while len(pages) > -(-tokens // self.page_size):
+        pages, keep = self._pages[sequence], -(-tokens // self.page_size)
+        if len(pages) > keep:
+            # (they may soon be another sequence's: a caller that advances kv_lens by itself finds no page here)
+            self._table[sequence, keep:len(pages)] = -1
+        while len(pages) > keep:
             self._free.append(pages.pop())
         self._host_lens[sequence] = tokens
         self._lens[sequence] = tokens

@@ -90,3 +90,18 @@ def test_a_layer_whose_refill_fails_is_not_attended_to(monkeypatch):
     (k0, k2), (v0, v2) = gathered[-2:]
     k, v = (torch.cat([a, own, b, text], 1) for a, own, b, text in ((k0, args[4], k2, args[1]), (v0, args[5], v2, args[2])))
     assert (got - oracle.sdpa_fp32(args[3], k, v)).abs().max() < 2e-6
+
+
+# ------------------------------------------------------------------------------------------------ the class's bookkeeping
+def test_a_table_names_no_page_behind_what_a_sequence_holds(monkeypatch):
+    """Pages given back may be another sequence's: a length that the caller advances itself past its pages finds none there."""
+    monkeypatch.setattr(ops, "kv_cache_append", lambda k, v, **a: None)
+    cache = PagedKVCache(2, 1, 100, page_size=16, num_pages=6, device="cpu")
+    tokens = torch.zeros(80, 1, 128, dtype=BF16)
+    cache.append(tokens, tokens, [60, 5])
+    cache.truncate(0, 16)
+    cache.append(tokens, tokens, [0, 60])
+    table = cache.tensors["block_table"]
+    assert table.ge(0).sum(1).tolist() == [1, 5] and table[table >= 0].unique().numel() == 6
+    cache.truncate(1)
+    assert table.ge(0).sum(1).tolist() == [1, 0]
