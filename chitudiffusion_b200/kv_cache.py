@@ -26,7 +26,8 @@ class PagedKVCache:
     """Keys and values of ``batch`` sequences in pages of ``page_size`` tokens.
 
     ``max_tokens`` bounds each sequence; ``num_pages`` (default: enough for all of them at that length) the pool they share.
-    ``dtype`` is ``torch.float8_e4m3fn``, bf16 or fp16.  Appending without a free page raises and leaves the cache as it was.
+    ``dtype`` is ``torch.float8_e4m3fn``, bf16 or fp16.  An append that raises, for want of a free page or anything else, leaves the cache
+    holding what it held.
     Calls that are to be captured into a graph use the operators directly, on :attr:`tensors` (allotting pages is host work).
     """
 
@@ -91,17 +92,25 @@ class PagedKVCache:
         if ids:
             at = torch.tensor([rows, cols], device=device)
             self._table[at[0], at[1]] = torch.tensor(ids, dtype=torch.int32, device=device)
-        if list(new) != self._new:
-            ends = [0]
-            for n in new:
-                ends.append(ends[-1] + n)
-            self._cu.copy_(torch.tensor(ends, dtype=torch.int32))
-            self._new = list(new)
+        self._set_new(list(new))
         if len(set(new)) == 1:
             self._lens += new[0]
         else:
             self._lens.copy_(torch.tensor(after, dtype=torch.int32))
         self._host_lens = after
+
+    def _set_new(self, new: List[int]) -> None:
+        if new != self._new:
+            self._new = []  # (nothing that another call could match, should the copy fail)
+            self._cu.copy_(torch.tensor(self._ends(new), dtype=torch.int32))
+            self._new = new
+
+    @staticmethod
+    def _ends(lens: Sequence[int]) -> List[int]:
+        ends = [0]
+        for n in lens:
+            ends.append(ends[-1] + n)
+        return ends
 
     def truncate(self, sequence: int, tokens: int = 0) -> None:
         """Forget what ``sequence`` holds behind its first ``tokens`` tokens; its pages behind them are free again."""
@@ -134,15 +143,14 @@ class PagedKVCache:
             if len(new) != self.batch or sum(new) > k.shape[0]:
                 raise ValueError("PagedKVCache: packed tokens need new_lens, one per sequence, of no more tokens than there are")
         before, before_new = list(self._host_lens), list(self._new)
-        self._allot(new)
         try:
+            self._allot(new)
             turned = ops.kv_cache_append(self._packed(k), self._packed(v), **self.tensors, positions=positions, rope_table=rope_table,
                                          interleaved=interleaved, q=None if q is None else self._packed(q), max_new=max(new))
-        except (ValueError, NotImplementedError, RuntimeError):
-            for b, n in enumerate(before):  # a refused call appends nothing
+        except BaseException:  # (an interrupt or a wrong argument's TypeError leaves no tokens behind either)
+            for b, n in enumerate(before):
                 self.truncate(b, n)
-            if self._new != before_new:
-                self._new = [-1] * self.batch  # (the next call states its own)
+            self._set_new(before_new)
             raise
         return turned if turned is None or q.dim() == 3 else turned.view(q.shape)
 
@@ -164,10 +172,7 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: out must be contiguous, of q's shape {tuple(q.shape)}")
         args = self.tensors
         if lens != self._new:
-            ends = [0]
-            for n in lens:
-                ends.append(ends[-1] + n)
-            args["cu_seqlens"] = torch.tensor(ends, dtype=torch.int32, device=self._cu.device)
+            args["cu_seqlens"] = torch.tensor(self._ends(lens), dtype=torch.int32, device=self._cu.device)
         got, lse = ops.attn_fwd_cache(self._packed(q), **args, softmax_scale=softmax_scale, causal=causal, return_lse=return_lse,
                                       out=None if out is None else self._packed(out), max_q=max(lens), max_kv=max(self._host_lens))
         if q.dim() == 4:

@@ -105,3 +105,42 @@ def test_a_table_names_no_page_behind_what_a_sequence_holds(monkeypatch):
     assert table.ge(0).sum(1).tolist() == [1, 5] and table[table >= 0].unique().numel() == 6
     cache.truncate(1)
     assert table.ge(0).sum(1).tolist() == [1, 0]
+
+
+@pytest.mark.parametrize("error", [ValueError, TypeError, AttributeError, MemoryError, KeyboardInterrupt])
+def test_a_call_that_fails_appends_nothing(monkeypatch, error):
+    """Whatever ends an append: lengths, pages, table and offsets are those of before, for the next call and for the operators."""
+    held = []
+    monkeypatch.setattr(ops, "kv_cache_append", lambda k, v, **a: held.append(k.shape[0]))
+    monkeypatch.setattr(ops, "attn_fwd_cache", lambda q, **a: (a["cu_seqlens"].clone(), None))
+    cache = PagedKVCache(2, 1, 100, page_size=16, num_pages=9, device="cpu")
+    tokens = [torch.zeros(n, 1, 128, dtype=BF16) for n in (0, 9, 20, 40)]
+    cache.append(tokens[2], tokens[2], [17, 3])
+
+    def state():
+        return {n: None if t is None else t.clone() for n, t in cache.tensors.items() if not n.endswith("_cache")}, cache.lens, cache.free_pages
+
+    def same(a, b):
+        return a[1:] == b[1:] and all(torch.equal(a[0][n], b[0][n]) for n in a[0])
+
+    before = state()
+
+    def fail(*_, **__):
+        raise error("no")
+
+    with monkeypatch.context() as m:
+        m.setattr(ops, "kv_cache_append", fail)
+        for k, new in ((tokens[3], [8, 32]), (tokens[2].view(2, 10, 1, 128), None), (tokens[2], [17, 3]), (tokens[0], [0, 0])):
+            with pytest.raises(error):
+                cache.append(k, k, new)
+            assert same(state(), before)
+    # arguments that are no tensors fail on their own
+    for bad in (lambda: cache.append(tokens[3], None, [8, 32]), lambda: cache.append(tokens[3], tokens[3], [8, 32], q=[1.0])):
+        with pytest.raises((TypeError, AttributeError)):
+            bad()
+        assert same(state(), before)
+    # queries of the last append that went through, then one more of it
+    assert cache.attend(tokens[2])[0].tolist() == [0, 17, 20]
+    cache.append(tokens[1], tokens[1], [9, 0])
+    assert cache.lens == [26, 3] and cache.free_pages == 6 and cache.tensors["cu_seqlens"].tolist() == [0, 9, 9]
+    assert cache.tensors["block_table"].ge(0).sum(1).tolist() == [2, 1] and held == [20, 9]
