@@ -1,7 +1,7 @@
 """A paged key/value cache with its bookkeeping: pools, page tables and lengths of a batch of sequences.
 
 The arithmetic is in ``ops.kv_cache_append`` and ``ops.attn_fwd_cache``; this class allots pages, keeps the tables on the GPU up to
-date and hands both operators what they need.  Generation frame by frame (the frames made so far are the keys of the next
+date and hands both operators what they need; no call waits for the GPU.  Generation frame by frame (the frames made so far are the keys of the next
 chunk), a prompt taken in chunks and single tokens are the same two calls::
 
     cache = PagedKVCache(batch=2, num_heads=8, max_tokens=4096, device="cuda")
@@ -88,21 +88,27 @@ class PagedKVCache:
                 cols.append(len(self._pages[b]))
                 ids.append(self._free.pop())
                 self._pages[b].append(ids[-1])
-        device = self._table.device
         if ids:
-            at = torch.tensor([rows, cols], device=device)
-            self._table[at[0], at[1]] = torch.tensor(ids, dtype=torch.int32, device=device)
+            rows, cols, ids = self._on_device(rows + cols + ids).view(3, -1)
+            self._table[rows, cols] = ids
         self._set_new(list(new))
         if len(set(new)) == 1:
             self._lens += new[0]
         else:
-            self._lens.copy_(torch.tensor(after, dtype=torch.int32))
+            self._lens.copy_(self._on_device(after))
         self._host_lens = after
+
+    def _on_device(self, values: List[int]) -> torch.Tensor:
+        """``values`` where the cache is, without a wait for the GPU: from pinned memory, which torch uses again once the
+        copy is through."""
+        if self._table.device.type == "cpu":
+            return torch.tensor(values, dtype=torch.int32)
+        return torch.tensor(values, dtype=torch.int32, pin_memory=True).to(self._table.device, non_blocking=True)
 
     def _set_new(self, new: List[int]) -> None:
         if new != self._new:
             self._new = []  # (nothing that another call could match, should the copy fail)
-            self._cu.copy_(torch.tensor(self._ends(new), dtype=torch.int32))
+            self._cu.copy_(self._on_device(self._ends(new)))
             self._new = new
 
     @staticmethod
@@ -119,11 +125,11 @@ class PagedKVCache:
         pages, keep = self._pages[sequence], -(-tokens // self.page_size)
         if len(pages) > keep:
             # (they may soon be another sequence's: a caller that advances kv_lens by itself finds no page here)
-            self._table[sequence, keep:len(pages)] = -1
+            self._table[sequence, keep:len(pages)].fill_(-1)
         while len(pages) > keep:
             self._free.append(pages.pop())
         self._host_lens[sequence] = tokens
-        self._lens[sequence] = tokens
+        self._lens[sequence].fill_(tokens)  # (assigning a number copies it from the host, with a wait)
 
     # ------------------------------------------------------------------ the two calls
     def _packed(self, t: torch.Tensor) -> torch.Tensor:
@@ -172,7 +178,7 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: out must be contiguous, of q's shape {tuple(q.shape)}")
         args = self.tensors
         if lens != self._new:
-            args["cu_seqlens"] = torch.tensor(self._ends(lens), dtype=torch.int32, device=self._cu.device)
+            args["cu_seqlens"] = self._on_device(self._ends(lens))
         got, lse = ops.attn_fwd_cache(self._packed(q), **args, softmax_scale=softmax_scale, causal=causal, return_lse=return_lse,
                                       out=None if out is None else self._packed(out), max_q=max(lens), max_kv=max(self._host_lens))
         if q.dim() == 4:

@@ -182,3 +182,89 @@ def test_image_cache_in_8_bits_on_every_rank(monkeypatch, world, rank, n):
             tol = 2 ** -8 * want.abs() + 1.02 * (2 ** -7 + 2 * SCORE) * mag + 1e-6
             assert ((got - want).abs() <= tol).all(), (step, ((got - want).abs() / tol).max().item())
         assert world == 1 or step % 2 == 0 or len(cp.far) == gathered  # a stale step gathers nothing
+
+
+# ------------------------------------------------------------------------------------------------ the class's host path
+class _NoWaits:
+    """Operations that make the host wait for the GPU raise."""
+
+    def __enter__(self):
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+
+    def __exit__(self, *exc):
+        torch.cuda.set_sync_debug_mode("default")
+        return False
+
+
+@pytest.mark.parametrize("dtype", [E4M3, BF16])
+def test_the_class_does_not_wait_for_the_gpu(dtype):
+    """Appends that begin pages, of equal and differing lengths, queries of other lengths than the append's, truncation: the host runs
+    ahead of all of it, and every result is, bit for bit, that of the operators called one by one on tables of their own."""
+    from chitudiffusion_b200 import PagedKVCache
+
+    ops = _ops()
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    heads, group, B, page, width = 2, 2, 3, 16, 13
+    cache = PagedKVCache(B, heads, 200, page_size=page, dtype=dtype, device="cuda")
+    calls = [[40, 3, 17], [16, 16, 16], [1, 1, 1], [0, 30, 2], [1, 1, 1]]
+    draws = [[torch.randn(sum(new), h, 128, generator=gen, device="cuda").to(BF16) for h in (heads, heads, heads * group)] for new in calls]
+    other = torch.randn(B, 5, heads * group, 128, generator=gen, device="cuda").to(BF16)
+    busy = torch.randn(4096, 4096, generator=gen, device="cuda")
+    cache.append(*draws[0][:2], calls[0])  # (what the first call allocates is not at issue)
+    cache.attend(draws[0][2])
+    cache.attend(other)
+    busy = busy @ busy * 1e-4
+    for b in range(B):
+        cache.truncate(b)
+    outs = []
+    with _NoWaits():
+        for _ in range(40):
+            busy = busy @ busy * 1e-4
+        for new, (k, v, q) in zip(calls, draws):
+            if len(set(new)) == 1:
+                cache.append(*(t.view(B, new[0], heads, 128) for t in (k, v)))
+            else:
+                cache.append(k, v, new)
+            outs.append([cache.attend(q, causal=True)[0], cache.attend(other)[0], cache.attend(q, q_lens=new[::-1])[0]])
+        cache.truncate(1, 20)
+        outs.append([cache.attend(other)[0]])
+
+    table = torch.arange(B * width, dtype=torch.int32, device="cuda").view(B, width)
+    pools = [torch.empty(B * width, heads, page, 128, dtype=dtype, device="cuda").transpose(1, 2) for _ in range(2)]
+    scales = [torch.ones(B * width, heads, device="cuda") if dtype == E4M3 else None for _ in range(2)]
+    lens = [0] * B
+
+    def tensors(new):
+        cu = torch.tensor([sum(new[:b]) for b in range(B + 1)], dtype=torch.int32, device="cuda")
+        return dict(k_cache=pools[0], v_cache=pools[1], block_table=table, kv_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                    cu_seqlens=cu, k_scale=scales[0], v_scale=scales[1])
+
+    def attend(q, new, causal=False):
+        return ops.attn_fwd_cache(q, **tensors(new), causal=causal, max_q=max(new), max_kv=max(lens))[0]
+
+    for new, (k, v, q), got in zip(calls, draws, outs):
+        lens = [a + n for a, n in zip(lens, new)]
+        ops.kv_cache_append(k, v, **tensors(new), max_new=max(new))
+        want = [attend(q, new, True), attend(other.flatten(0, 1), [5] * B), attend(q, new[::-1])]
+        for x, y in zip(got, want):
+            assert torch.equal(x.flatten(0, -3), y)
+    lens[1] = 20
+    assert torch.equal(outs[-1][0].flatten(0, 1), attend(other.flatten(0, 1), [5] * B))
+    assert cache.lens == lens and cache.tensors["kv_lens"].tolist() == lens
+
+
+@pytest.mark.parametrize("rank", [0, 1])
+def test_a_stale_step_over_8_bit_pages_does_not_wait_for_the_gpu(monkeypatch, rank):
+    from chitudiffusion_b200 import B200AttnBackend
+    from chitudiffusion_b200.image_cp import B200ImageContextParallel
+
+    cp, draw = _image_cp(monkeypatch, B200ImageContextParallel(B200AttnBackend("b200"), mode="agkv"), 3, rank, 40)
+    inputs = [[draw(6)] * 3 + [draw(40) for _ in range(3)] for _ in range(6)]
+    for step in range(4):
+        cp.begin_forward(step, 100)
+        if step < 2:
+            cp.attention(*inputs[step])
+        else:  # (what the first fresh and the first stale call allocate is not at issue)
+            with _NoWaits():
+                cp.attention(*inputs[step])
