@@ -889,6 +889,7 @@ def peer_wait_outputs(sync, device: torch.device) -> None:
 # Calls of a generation loop wait for the host: tensors are asked for each attribute once, arrays go down as packed bytes.
 _CACHE_HEAD_DIM = 128
 _CACHE_PAGES = (16, 32, 64, 128, 256)
+_APPEND_FEW = 4  # appended tokens of the longest sequence up to which the library takes its form for single tokens
 _POSITION_DTYPES = (torch.int32, torch.int64)
 
 
@@ -1084,7 +1085,7 @@ def kv_cache_append(
     shape, dtype = _check_tokens(k, "k", what)
     if v.shape != shape or v.dtype != dtype:
         raise ValueError(f"{what}: shape mismatch: k {tuple(k.shape)}, v {tuple(v.shape)}")
-    packed, B, _, _, heads = _pack_cache(k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale, v_scale, dtype, what)
+    packed, B, _, page, heads = _pack_cache(k_cache, v_cache, block_table, kv_lens, cu_seqlens, k_scale, v_scale, dtype, what)
     T = shape[0]
     if shape[1] != heads:
         raise ValueError(f"{what}: k has {shape[1]} heads, the cache {heads}")
@@ -1131,7 +1132,8 @@ def kv_cache_append(
             rc = _lib.load().chitu_b200_kv_append(*args)
     if rc:
         _lib.check(rc, what)
-    _launched()
+    # (8-bit pages of 256 tokens: keys and values in one launch, queries in another)
+    _launched(2 if page == 256 and q is not None and k_scale is not None and min(int(max_new), T) > _APPEND_FEW else 1)
     return q_out
 
 
@@ -1212,5 +1214,6 @@ def attn_fwd_cache(
             rc = _lib.load().chitu_b200_attn_fwd_cache(*args)
     if rc:
         _lib.check(rc, what)
-    _launched()
+    # (chunks of queries: what the borders of the CTAs' runs have cut is joined by a kernel of its own)
+    _launched(2 if max_q * (Hq // heads) > 32 and Hq // heads <= 128 else 1)
     return out, lse

@@ -268,3 +268,51 @@ def test_a_stale_step_over_8_bit_pages_does_not_wait_for_the_gpu(monkeypatch, ra
         else:  # (what the first fresh and the first stale call allocate is not at issue)
             with _NoWaits():
                 cp.attention(*inputs[step])
+
+
+# ------------------------------------------------------------------------------------------------ what a call counts
+def _kernels(call):
+    """Kernels of this library that a captured `call` launches."""
+    from cuda.bindings import driver
+
+    def done(result):
+        assert result[0] == driver.CUresult.CUDA_SUCCESS
+        return result[1] if len(result) == 2 else result[1:]
+
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    raw = driver.CUgraph(graph.raw_cuda_graph())
+    names = []
+    for node in done(driver.cuGraphGetNodes(raw, done(driver.cuGraphGetNodes(raw))[1]))[0]:
+        if done(driver.cuGraphNodeGetType(node)) == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            params = done(driver.cuGraphKernelNodeGetParams(node))
+            names.append(done(driver.cuFuncGetName(params.func)) if int(params.func) else done(driver.cuKernelGetName(params.kern)))
+    return sum(b"chitu" in name for name in names)
+
+
+@pytest.mark.parametrize("n", [1, 5, 9, 40, 130])
+@pytest.mark.parametrize("group,page,eight", [(4, 64, True), (4, 256, True), (4, 256, False), (130, 32, True)])
+def test_launch_count_is_the_number_of_kernels(n, group, page, eight):
+    """The two attention kernels, the one that joins pieces, the append for few and for many tokens, and its form in two launches."""
+    ops = _ops()
+    gen = torch.Generator().manual_seed(1)
+    (kc, ks), (vc, vs) = (model.make_cache(gen, 4, page, 1, BF16, eight) for _ in range(2))
+    cache = [t.cuda() for t in (kc, vc, torch.arange(4, dtype=torch.int32)[None], torch.tensor([n + 3], dtype=torch.int32),
+                                torch.tensor([0, n], dtype=torch.int32))]
+    scales = dict(k_scale=ks.cuda(), v_scale=vs.cuda()) if eight else {}
+    k = torch.zeros(n, 1, 128, dtype=BF16, device="cuda")
+    q, rope = torch.zeros(n, group, 128, dtype=BF16, device="cuda"), model.rope_table(64, 200).cuda()
+    positions = torch.arange(n, device="cuda")
+    calls = (lambda: ops.kv_cache_append(k, k, *cache, **scales, rope_table=rope, q=q),
+             lambda: ops.kv_cache_append(k, k, *cache, **scales, max_new=n),
+             lambda: ops.kv_cache_append(k, k, *cache, **scales, rope_table=rope, q=q, max_new=1),
+             lambda: ops.attn_fwd_cache(q, *cache, **scales), lambda: ops.attn_fwd_cache(q, *cache, **scales, max_q=1),
+             lambda: ops.attn_fwd_cache(q, *cache, **scales, max_q=1000),
+             lambda: ops.rotary([q, k], positions, rope))
+    for call in calls:
+        call()
+        before = ops.launch_count
+        call()
+        counted = ops.launch_count - before
+        assert counted == _kernels(call), calls.index(call)
