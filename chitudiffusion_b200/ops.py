@@ -1053,6 +1053,14 @@ def _check_tokens(t: torch.Tensor, name: str, what: str):
     return shape, dtype
 
 
+def _expected_new(tokens: int, batch: int) -> int:
+    """``max_new`` of an append that does not say: with a token at least of every sequence the longest brings ``longest`` at most, and
+    up to ``_APPEND_FEW`` of them suit the form that walks them one after the other; a prompt may not go there unseen (one of
+    2000 tokens beside 699 single ones: 2415 us, in the other form sized for the average MIXED)."""
+    longest = tokens - batch + 1
+    return max(1, longest) if longest <= _APPEND_FEW else max(_APPEND_FEW + 1, -(-tokens // batch))
+
+
 def kv_cache_append(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -1078,8 +1086,11 @@ def kv_cache_append(
     the last sequence are left alone.
 
     With ``rope_table`` keys turn by the row of their position, or of ``positions [T]`` where given (a clip's per-token rows), and
-    ``q [T, Hq, 128]``, if given, is rotated by the same launch and returned (rows behind the last sequence are not written).  ``max_new`` is how many tokens the longest sequence
-    brings (default: the average); it sizes the launch, results do not depend on it.
+    ``q [T, Hq, 128]``, if given, is rotated by the same launch and returned (rows behind the last sequence are not written).
+
+    ``max_new`` is how many tokens the longest sequence brings; it chooses the kernel and sizes the launch, results do not depend on it.  By
+    default it is taken that every sequence brings a token.  State it where that is far off: a batch in which few sequences bring
+    anything takes a microsecond for each token of the longest one otherwise, one of two to four tokens each the form for prompts.
     """
     what = "kv_cache_append"
     shape, dtype = _check_tokens(k, "k", what)
@@ -1120,7 +1131,7 @@ def kv_cache_append(
     if T == 0 or B == 0:
         return q_out
     if max_new is None:
-        max_new = -(-T // B)
+        max_new = _expected_new(T, B)
     args = (packed, k.data_ptr(), v.data_ptr(), q_ptr, i64x2(*k.stride()[:2]), i64x2(*v.stride()[:2]), q_strides, q_out_ptr, q_heads, T,
             _DTYPES[dtype], int(max_new), None if positions is None else positions.data_ptr(),
             positions is not None and positions.dtype == torch.int64, table_ptr, rows, rot, bool(interleaved),

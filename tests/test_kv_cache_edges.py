@@ -144,3 +144,16 @@ def test_a_call_that_fails_appends_nothing(monkeypatch, error):
     cache.append(tokens[1], tokens[1], [9, 0])
     assert cache.lens == [26, 3] and cache.free_pages == 6 and cache.tensors["cu_seqlens"].tolist() == [0, 9, 9]
     assert cache.tensors["block_table"].ge(0).sum(1).tolist() == [2, 1] and held == [20, 9]
+
+
+# ------------------------------------------------------------------------------------------------ launch hints
+@pytest.mark.parametrize("tokens,batch,few", [
+    (64, 64, True), (1, 1, True), (4, 1, True), (5, 1, False), (66, 64, True), (67, 64, True), (68, 64, False), (40, 64, True),
+    (2699, 700, False),  # a prompt of 2000 tokens among 699 single ones
+    (128, 64, False), (256, 64, False), (19200, 64, False)])
+def test_an_append_without_a_hint_is_sized_for_the_longest_that_its_tokens_allow(tokens, batch, few):
+    """The form for single tokens walks a sequence's tokens one after the other: it is taken where, with a token at least of every sequence, none can
+    bring more than four.  Otherwise the other form, for no fewer tokens than the average."""
+    expected = ops._expected_new(tokens, batch)
+    assert (expected <= ops._APPEND_FEW) is few
+    assert expected >= 1 and (few or expected == max(ops._APPEND_FEW + 1, -(-tokens // batch)))
