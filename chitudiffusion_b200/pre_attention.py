@@ -80,8 +80,9 @@ def scaled_rope_table(rot_dim: int, max_len: int, theta: float = 10000.0, scalin
     * ``"base"``      ``theta * factor^(rot_dim / (rot_dim - 2))`` in the place of ``theta``: the slowest pair turns as with
       ``"linear"``, the fastest as with ``"none"``;
     * ``"by_parts"``  pairs that make more than ``beta_fast`` turns within ``original_len`` keep their angle, those with fewer than
-      ``beta_slow`` get the linear one, the others a blend by their index; cos and sin times ``0.1 ln(factor) + 1`` (Peng et
-      al., "YaRN: Efficient Context Window Extension of Large Language Models", 2023).
+      ``beta_slow`` get the linear one, the others a blend that is linear in the number of turns; cos and sin times
+      ``0.1 ln(factor) + 1`` (the definitions of Peng et al., "YaRN: Efficient Context Window Extension of Large Language Models",
+      2023; model code that blends by the pair's index gives other angles in between).
 
     Built in float64 on the host, like the other tables.
     """
@@ -95,12 +96,10 @@ def scaled_rope_table(rot_dim: int, max_len: int, theta: float = 10000.0, scalin
     if scaling == "linear":
         inv = inv / factor
     elif scaling == "by_parts":
-        def index_of(turns: float) -> float:  # the pair that makes so many turns within original_len
-            return rot_dim * math.log(original_len / (2.0 * math.pi * turns)) / (2.0 * math.log(theta))
-
-        low = max(math.floor(index_of(beta_fast)), 0)
-        high = min(math.ceil(index_of(beta_slow)), rot_dim - 1)
-        keep = 1.0 - ((j / 2 - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        if not beta_fast > beta_slow:
+            raise ValueError("scaled_rope_table: beta_fast must be greater than beta_slow")
+        turns = original_len / (2.0 * math.pi) * inv
+        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
         inv = inv / factor * (1.0 - keep) + inv * keep
         gain = 0.1 * math.log(factor) + 1.0
     elif scaling not in ("none", "base"):

@@ -157,3 +157,28 @@ def test_an_append_without_a_hint_is_sized_for_the_longest_that_its_tokens_allow
     expected = ops._expected_new(tokens, batch)
     assert (expected <= ops._APPEND_FEW) is few
     assert expected >= 1 and (few or expected == max(ops._APPEND_FEW + 1, -(-tokens // batch)))
+
+
+# ------------------------------------------------------------------------------------------------ tables
+@pytest.mark.parametrize("rot,factor,original_len,fast,slow", [(128, 4.0, 4096, 32.0, 1.0), (64, 8.0, 2048, 32.0, 1.0), (96, 1.0, 4096, 32.0, 1.0),
+                                                               (128, 16.0, 8192, 20.0, 0.5), (16, 2.0, 100, 8.0, 1.0)])
+def test_rope_table_by_parts_blends_by_turns(rot, factor, original_len, fast, slow):
+    """A pair that makes r turns within the original length keeps the share (r - slow) / (fast - slow) of its angle, none below, all above."""
+    from chitudiffusion_b200.pre_attention import scaled_rope_table
+
+    table = scaled_rope_table(rot, 50, theta=10000.0, scaling="by_parts", factor=factor, original_len=original_len, beta_fast=fast, beta_slow=slow)
+    gain = 0.1 * math.log(factor) + 1.0
+    blended = 0
+    for j in range(rot // 2):
+        angle = 10000.0 ** (-2 * j / rot)
+        turns = original_len * angle / (2 * math.pi)
+        keep = 0.0 if turns < slow else 1.0 if turns > fast else (turns - slow) / (fast - slow)
+        blended += 0.0 < keep < 1.0
+        angle = keep * angle + (1.0 - keep) * angle / factor
+        for p in (0, 1, 7, 49):
+            # (fp32 entries: half a step of a value of at most 2)
+            assert abs(table[p, j, 0].item() - gain * math.cos(p * angle)) <= 2.0 ** -23
+            assert abs(table[p, j, 1].item() - gain * math.sin(p * angle)) <= 2.0 ** -23
+    assert blended
+    with pytest.raises(ValueError, match="beta_fast"):
+        scaled_rope_table(rot, 50, scaling="by_parts", factor=factor, beta_fast=1.0, beta_slow=1.0)
