@@ -26,8 +26,6 @@ struct CacheAttnParams {
   long long q_token, q_head;
   void* out;      // [tokens, heads_q, 128] contiguous
   float* lse;     // [heads_q, tokens] fp32 natural log, or nullptr
-  const uint8_t* cache[2];                     // k, v
-  long long c_page[2], c_token[2], c_head[2];  // strides, bytes
   const float* scale[2];                       // 8-bit pages: one fp32 per page and head
   long long s_page[2], s_head[2];              // strides, elements
   const int* block_table;

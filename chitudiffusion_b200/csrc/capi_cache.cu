@@ -365,16 +365,10 @@ int chitu_b200_attn_fwd_cache(const chitu_b200_kv_cache* cache, const void* q, c
   p.q_head = q_strides[1];
   p.out = out;
   p.lse = lse;
-  p.cache[0] = static_cast<const uint8_t*>(cache->k);
-  p.cache[1] = static_cast<const uint8_t*>(cache->v);
   p.scale[0] = cache->k_scale;
   p.scale[1] = cache->v_scale;
   for (int i = 0; i < 2; ++i) {
-    const int64_t* cs = i == 0 ? cache->k_strides : cache->v_strides;
     const int64_t* ss = i == 0 ? cache->k_scale_strides : cache->v_scale_strides;
-    p.c_page[i] = cs[0] * es;
-    p.c_token[i] = cs[1] * es;
-    p.c_head[i] = cs[2] * es;
     p.s_page[i] = ss[0];
     p.s_head[i] = ss[1];
   }
