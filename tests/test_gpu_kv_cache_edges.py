@@ -316,3 +316,80 @@ def test_launch_count_is_the_number_of_kernels(n, group, page, eight):
         call()
         counted = ops.launch_count - before
         assert counted == _kernels(call), calls.index(call)
+
+
+# ------------------------------------------------------------------------------------------------ strides
+def _strided(t, kind):
+    """`t [pages, page, H, 128]` or `[pages, H]` with other strides: every second page of a larger pool, tokens or heads outermost."""
+    if t is None:
+        return None
+    if kind == "every other":
+        wide = torch.empty((2 * t.shape[0],) + t.shape[1:], dtype=t.dtype, device="cuda")
+        view = wide[::2]
+    elif kind == "padded rows":
+        wide = torch.empty(t.shape[:-1] + (t.shape[-1] + 32,), dtype=t.dtype, device="cuda")
+        view = wide[..., :t.shape[-1]]
+    elif kind == "transposed":
+        view = torch.empty([t.shape[i] for i in (range(t.dim() - 2, -1, -1) if t.dim() == 4 else (1, 0))] + ([t.shape[3]] if t.dim() == 4 else []),
+                           dtype=t.dtype, device="cuda")
+        view = view.permute(2, 1, 0, 3) if t.dim() == 4 else view.t()
+    else:
+        view = torch.empty(t.shape, dtype=t.dtype, device="cuda")
+    assert view.shape == t.shape
+    view.view(torch.uint8).copy_(t.contiguous().view(torch.uint8)) if t.dtype == E4M3 else view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("eight", [True, False])
+@pytest.mark.parametrize("n", [1, 3, 70, 300])
+@pytest.mark.parametrize("forms", [("plain", "every other"), ("padded rows", "transposed"), ("transposed", "plain"), ("every other", "padded rows")])
+def test_projections_pools_and_scales_of_any_strides(n, forms, eight):
+    """k, v and q as parts of one projection, key and value pools of two different layouts, scales that are not contiguous, through append and
+    attention."""
+    ops = _ops()
+    heads, group, page, old = 2, 4, 32, [5, 130]
+    gen = torch.Generator().manual_seed(n)
+    lens = [n + o for o in old]
+    pages = sum(-(-length // page) for length in lens) + 1
+    (kc, ks), (vc, vs) = (model.make_cache(gen, pages, page, heads, BF16, eight) for _ in range(2))
+    table = model.make_tables(gen, lens, page, pages)
+    lens, cu = torch.tensor(lens, dtype=torch.int32), torch.tensor([0, n, 2 * n], dtype=torch.int32)
+    rope = model.rope_table(128, 500)
+    packed = torch.randn(2 * n, heads * (group + 2), 128, generator=gen).to(BF16)
+    parts = packed.split([heads * group, heads, heads], 1)
+    q, k, v = packed.cuda().split([heads * group, heads, heads], 1)
+    dev = [_strided(t, forms[i]) for t, i in ((kc, 0), (vc, 1), (ks, 1), (vs, 0))]
+    turned = ops.kv_cache_append(k, v, dev[0], dev[1], table.cuda(), lens.cuda(), cu.cuda(), k_scale=dev[2], v_scale=dev[3], rope_table=rope.cuda(), q=q)
+    pos = torch.cat([torch.arange(length - n, length) for length in lens.tolist()])
+    for x, c, s in ((model.rotate(parts[1], pos, rope, True), kc, ks), (parts[2].float(), vc, vs)):
+        model.append(x, c, s, table, lens, cu)
+    for got, want in zip(dev, (kc, vc, ks, vs)):
+        if want is not None:
+            _equal(got, want)
+    _equal(turned, model.rotate(parts[0], pos, rope, True).to(BF16))
+    for causal in (True, False):
+        out, lse = ops.attn_fwd_cache(q, dev[0], dev[1], table.cuda(), lens.cuda(), cu.cuda(), k_scale=dev[2], v_scale=dev[3], causal=causal,
+                                      return_lse=True)
+        _attention_close(out, lse, model.attend(parts[0], kc, vc, ks, vs, table, lens, cu, 128 ** -0.5, causal), BF16, eight)
+
+
+@pytest.mark.parametrize("eight", [True, False])
+@pytest.mark.parametrize("n,group", [(1, 4), (40, 4), (300, 2), (1, 129), (3, 200), (40, 130)])
+def test_outputs_off_the_32_byte_grid_and_many_heads_of_a_key_head(n, group, eight):
+    ops = _ops()
+    heads, page, lens = 2, 64, [n + 200, n]
+    gen = torch.Generator().manual_seed(group)
+    (kc, ks), (vc, vs) = (model.make_cache(gen, 14, page, heads, BF16, eight) for _ in range(2))
+    table, lens = model.make_tables(gen, lens, page, 14), torch.tensor(lens, dtype=torch.int32)
+    cu = torch.tensor([0, n, 2 * n], dtype=torch.int32)
+    q = torch.randn(2 * n, heads * group, 128, generator=gen).to(BF16)
+    room = torch.full((q.numel() + 24,), 7.0, dtype=BF16, device="cuda")
+    out = room[8:-16].view(q.shape)
+    assert out.data_ptr() % 32 == 16
+    for causal in (True, False):
+        ref = model.attend(q, kc, vc, ks, vs, table, lens, cu, 128 ** -0.5, causal)
+        got, lse = ops.attn_fwd_cache(*[t.cuda() for t in (q, kc, vc, table, lens, cu)], k_scale=None if ks is None else ks.cuda(),
+                                      v_scale=None if vs is None else vs.cuda(), causal=causal, return_lse=True, out=out)
+        assert got is out
+        _attention_close(out, lse, ref, BF16, eight)
+        assert (room[:8] == 7.0).all() and (room[-16:] == 7.0).all()
