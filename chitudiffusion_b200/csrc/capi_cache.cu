@@ -74,7 +74,10 @@ cudaError_t allow_smem(Kernel kernel, int bytes, bool (&done)[kMaxDevices]) {
 
 constexpr int kSms = 148;
 
-// Appended tokens per sequence up to which eight threads take all of them (kv_append_few_kernel).
+// Appended tokens per sequence up to which eight threads take all of them (kv_append_few_kernel), about a microsecond each.  That
+// against the form for many, whose time hardly depends on their number up to a page: 1 sequence, 5 tokens 6.4 : 3.1 us, 8 sequences, 4 and
+// 5 tokens 5.6 : 4.9 and 6.6 : 5.0; 64 sequences, 4 and 12 tokens 5.7 : 13.0 and 13.5 : 13.9; 256 sequences, 4 and 16 tokens 8.3 : 38
+// and 34 : 44 (8-bit pages of 64, 48 heads).
 constexpr int kAppendFew = 4;
 
 // Tensor map over a pool: channels, heads, tokens of a page, pages; a box is 128 bytes of the channels by
@@ -120,6 +123,9 @@ cudaError_t launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const chit
 // pages, 8 key heads: 32 rows, 64 sequences of 500 keys 40 : 65 us, of 16000 keys 655 : 778, 8 of 4000 36 : 40, one of 16000 35 : 33;
 // 48 rows, 64 of 500 69 : 79 but of 16000 970 : 816; 64 rows, 8 of 4000 56 : 40, 64 of 16000 1291 : 823.
 bool takes_tile_kernel(int max_q, int group) { return static_cast<int64_t>(max_q) * group > 32 && group <= 128; }
+// Shortest run of a CTA, in tiles of 128 keys (a block's fixed cost is four): 1, 2, 4 and 8 of them take, 8-bit pages of 64, 40 queries over 4000
+// keys, 2 key heads of 4 query heads: 30.2, 24.7, 24.0, 28.6 us; 64 over 1000, 8 key heads: 20.0, 19.9, 22.0, 27.7; 4 x 64 over
+// 500, 4 key heads: 18.2, 19.9, 22.1, 19.8; 300 over 900, twice, 2 key heads of 2: 20.3, 19.9, 22.4, 28.1.
 constexpr int kTileMinTiles = 2;
 int64_t tile_workspace_bytes() { return kHeaderBytes + static_cast<int64_t>(kSms) * (2 * chitu::kTilePieceFloats * 4 + sizeof(chitu::TileJoin)); }
 
