@@ -1100,6 +1100,8 @@ def kv_cache_append(
     T = shape[0]
     if shape[1] != heads:
         raise ValueError(f"{what}: k has {shape[1]} heads, the cache {heads}")
+    if k_scale is not None and (0 in k_scale.stride() or 0 in v_scale.stride()):
+        raise ValueError(f"{what}: every page and head needs a scale of its own to write")
     on = k.get_device()
     q_heads = 0
     if q is not None:

@@ -182,3 +182,19 @@ def test_rope_table_by_parts_blends_by_turns(rot, factor, original_len, fast, sl
     assert blended
     with pytest.raises(ValueError, match="beta_fast"):
         scaled_rope_table(rot, 50, scaling="by_parts", factor=factor, beta_fast=1.0, beta_slow=1.0)
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("scale", [torch.ones(1, 2).expand(4, 2), torch.ones(4, 1).expand(4, 2), torch.ones(1).expand(4, 2)])
+def test_an_append_refuses_scales_that_share_memory(which, scale):
+    """One scale for several pages or heads can be read, but an append would write it for each of them."""
+    a = dict(k_cache=torch.zeros(4, 16, 2, 128, dtype=E4M3), v_cache=torch.zeros(4, 16, 2, 128, dtype=E4M3),
+             block_table=torch.zeros(1, 3, dtype=torch.int32), kv_lens=torch.tensor([5], dtype=torch.int32),
+             cu_seqlens=torch.tensor([0, 5], dtype=torch.int32), k_scale=torch.ones(4, 2), v_scale=torch.ones(4, 2))
+    a[which] = scale
+    k = torch.zeros(5, 2, 128, dtype=BF16)
+    with pytest.raises(ValueError, match="of its own"):
+        ops.kv_cache_append(k, k, **a)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):  # (which is looked at last)
+        ops.attn_fwd_cache(k, **a)
