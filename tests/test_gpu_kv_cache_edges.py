@@ -127,63 +127,6 @@ def test_many_keys_without_values(n):
     assert ((lse - want).abs() <= 1.4e-4).all(), lse.min().item()
 
 
-# ------------------------------------------------------------------------------------------------ the cross-step cache's ranks
-def _image_cp(monkeypatch, cp, world, rank, n, B=2, H=2):
-    """`cp` as rank `rank` of `world` with shards of `n` rows and 8-bit pages, every second step stale, and what draws its inputs; the other
-    ranks' rows of a step are drawn when they are gathered and kept in `cp.far`."""
-    gen = torch.Generator(device="cuda").manual_seed(10 * world + rank)
-
-    def draw(rows):
-        return torch.randn(B, rows, H, 128, generator=gen, device="cuda").to(BF16)
-
-    class Group:
-        group_size, rank_in_group = world, rank
-
-        def all_gather_sequence(self, t):
-            others = [draw(n) for _ in range(world - 1)]
-            cp.far = (cp.far + [others])[-2:]
-            return torch.cat(others[:rank] + [t] + others[rank:], 1)
-
-    cp.far = []
-    cp._kvcache_enabled = cp._kvcache_fp8 = True
-    cp._kvcache_warmup, cp._kvcache_interval, cp._kvcache_tail = 0, 2, 0
-    cp.enable(Group())
-    return cp, draw
-
-
-@pytest.mark.parametrize("n", [150, 128, 37])
-@pytest.mark.parametrize("world,rank", [(1, 0), (2, 0), (2, 1), (3, 0), (3, 1), (3, 2)])
-def test_image_cache_in_8_bits_on_every_rank(monkeypatch, world, rank, n):
-    """Fresh and stale steps of a rank that has others on one side of it, on both sides (pages that two appends share), or none.
-
-    Tolerance as in test_image_cache_of_other_ranks_in_8_bits, against attention over the kept rows as their codes say; those
-    are the gathered rows to half a step of e4m3 (2^-4), twice where a page's earlier codes move to a larger scale."""
-    from chitudiffusion_b200 import B200AttnBackend
-    from chitudiffusion_b200.image_cp import B200ImageContextParallel
-    from test_gpu_kv_cache import SCORE, _dense, _held
-
-    cp, draw = _image_cp(monkeypatch, B200ImageContextParallel(B200AttnBackend("b200"), mode="agkv"), world, rank, n)
-    for step in range(4):
-        cp.begin_forward(step, 100)
-        tq, tk, tv, iq, ik, iv = (draw(rows) for rows in (20, 20, 20, n, n, n))
-        gathered = len(cp.far)
-        txt, img = cp.attention(tq, tk, tv, iq, ik, iv)
-        for b in range(2):
-            keys = [torch.cat([t[b] for t in others] + [ik[b][:0]]).cpu() for others in cp.far]
-            if step % 2 and world > 1:
-                kept = _held(cp._kvcache[("cond", 0)], b)
-                for exact, got in zip(keys, kept):
-                    exact = exact.double()
-                    assert ((got - exact).abs() <= 2 * 2 ** -4 * exact.abs() + 2 ** -9 * 2.0 ** -6).all()
-                keys = kept
-            k, v = (torch.cat([x.double(), own[b].cpu().double(), t[b].cpu().double()]) for x, own, t in zip(keys, (ik, iv), (tk, tv)))
-            want, _, mag = _dense(torch.cat([iq[b], tq[b]]).cpu(), k, v)
-            got = torch.cat([img[b], txt[b]]).double().cpu()
-            tol = 2 ** -8 * want.abs() + 1.02 * (2 ** -7 + 2 * SCORE) * mag + 1e-6
-            assert ((got - want).abs() <= tol).all(), (step, ((got - want).abs() / tol).max().item())
-        assert world == 1 or step % 2 == 0 or len(cp.far) == gathered  # a stale step gathers nothing
-
-
 # ------------------------------------------------------------------------------------------------ the class's host path
 class _NoWaits:
     """Operations that make the host wait for the GPU raise."""
@@ -268,6 +211,63 @@ def test_a_stale_step_over_8_bit_pages_does_not_wait_for_the_gpu(monkeypatch, ra
         else:  # (what the first fresh and the first stale call allocate is not at issue)
             with _NoWaits():
                 cp.attention(*inputs[step])
+
+
+# ------------------------------------------------------------------------------------------------ the cross-step cache's ranks
+def _image_cp(monkeypatch, cp, world, rank, n, B=2, H=2):
+    """`cp` as rank `rank` of `world` with shards of `n` rows and 8-bit pages, every second step stale, and what draws its inputs; the other
+    ranks' rows of a step are drawn when they are gathered and kept in `cp.far`."""
+    gen = torch.Generator(device="cuda").manual_seed(10 * world + rank)
+
+    def draw(rows):
+        return torch.randn(B, rows, H, 128, generator=gen, device="cuda").to(BF16)
+
+    class Group:
+        group_size, rank_in_group = world, rank
+
+        def all_gather_sequence(self, t):
+            others = [draw(n) for _ in range(world - 1)]
+            cp.far = (cp.far + [others])[-2:]
+            return torch.cat(others[:rank] + [t] + others[rank:], 1)
+
+    cp.far = []
+    cp._kvcache_enabled = cp._kvcache_fp8 = True
+    cp._kvcache_warmup, cp._kvcache_interval, cp._kvcache_tail = 0, 2, 0
+    cp.enable(Group())
+    return cp, draw
+
+
+@pytest.mark.parametrize("n", [150, 128, 37])
+@pytest.mark.parametrize("world,rank", [(1, 0), (2, 0), (2, 1), (3, 0), (3, 1), (3, 2)])
+def test_image_cache_in_8_bits_on_every_rank(monkeypatch, world, rank, n):
+    """Fresh and stale steps of a rank that has others on one side of it, on both sides (pages that two appends share), or none.
+
+    Tolerance as in test_image_cache_of_other_ranks_in_8_bits, against attention over the kept rows as their codes say; those
+    are the gathered rows to half a step of e4m3 (2^-4), twice where a page's earlier codes move to a larger scale."""
+    from chitudiffusion_b200 import B200AttnBackend
+    from chitudiffusion_b200.image_cp import B200ImageContextParallel
+    from test_gpu_kv_cache import SCORE, _dense, _held
+
+    cp, draw = _image_cp(monkeypatch, B200ImageContextParallel(B200AttnBackend("b200"), mode="agkv"), world, rank, n)
+    for step in range(4):
+        cp.begin_forward(step, 100)
+        tq, tk, tv, iq, ik, iv = (draw(rows) for rows in (20, 20, 20, n, n, n))
+        gathered = len(cp.far)
+        txt, img = cp.attention(tq, tk, tv, iq, ik, iv)
+        for b in range(2):
+            keys = [torch.cat([t[b] for t in others] + [ik[b][:0]]).cpu() for others in cp.far]
+            if step % 2 and world > 1:
+                kept = _held(cp._kvcache[("cond", 0)], b)
+                for exact, got in zip(keys, kept):
+                    exact = exact.double()
+                    assert ((got - exact).abs() <= 2 * 2 ** -4 * exact.abs() + 2 ** -9 * 2.0 ** -6).all()
+                keys = kept
+            k, v = (torch.cat([x.double(), own[b].cpu().double(), t[b].cpu().double()]) for x, own, t in zip(keys, (ik, iv), (tk, tv)))
+            want, _, mag = _dense(torch.cat([iq[b], tq[b]]).cpu(), k, v)
+            got = torch.cat([img[b], txt[b]]).double().cpu()
+            tol = 2 ** -8 * want.abs() + 1.02 * (2 ** -7 + 2 * SCORE) * mag + 1e-6
+            assert ((got - want).abs() <= tol).all(), (step, ((got - want).abs() / tol).max().item())
+        assert world == 1 or step % 2 == 0 or len(cp.far) == gathered  # a stale step gathers nothing
 
 
 # ------------------------------------------------------------------------------------------------ what a call counts
@@ -393,3 +393,42 @@ def test_outputs_off_the_32_byte_grid_and_many_heads_of_a_key_head(n, group, eig
         assert got is out
         _attention_close(out, lse, ref, BF16, eight)
         assert (room[:8] == 7.0).all() and (room[-16:] == 7.0).all()
+
+
+# ------------------------------------------------------------------------------------------------ many sequences
+@pytest.mark.parametrize("eight", [True, False])
+def test_thousands_of_sequences(eight):
+    """A padded batch of 3000: some bring nothing, some hold nothing, pages of a common beginning are shared by all."""
+    ops, heads, group, page, B = _ops(), 1, 2, 16, 3000
+    gen = torch.Generator().manual_seed(5)
+    new = torch.randint(0, 4, (B,), generator=gen)
+    new[7], new[100:400] = 150, 0
+    lens = (new + torch.randint(0, 60, (B,), generator=gen)).int()
+    lens[::9] = new[::9].int()
+    lens[100:250] = 0
+    (kc, ks), (vc, vs) = (model.make_cache(gen, 2000, page, heads, BF16, eight) for _ in range(2))
+    table = torch.randint(0, 2000, (B, int(lens.max()) // page + 1), generator=gen).int()
+    table[:, :2] = torch.tensor([3, 1999], dtype=torch.int32)
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), new.cumsum(0)]).int()
+    q = torch.randn(int(cu[-1]), heads * group, 128, generator=gen).to(BF16)
+    ref = model.attend(q, kc, vc, ks, vs, table, lens, cu, 128 ** -0.5, True)
+    dev = [t.cuda() for t in (q, kc, vc, table, lens, cu)]
+    for hint in (1, 150, None):  # the kernel for few rows, the one for chunks
+        out, lse = ops.attn_fwd_cache(*dev, k_scale=None if ks is None else ks.cuda(), v_scale=None if vs is None else vs.cuda(), causal=True,
+                                      return_lse=True, max_q=hint)
+        _attention_close(out, lse, ref, BF16, eight)
+    # the same batch appended, a page for each of its own
+    table = torch.arange(B * table.shape[1], dtype=torch.int32).view(B, -1)
+    own = [model.make_cache(gen, table.numel(), page, heads, BF16, eight) for _ in range(2)]
+    k, v = (torch.randn(q.shape[0], heads, 128, generator=gen).to(BF16) for _ in range(2))
+    devs = [[t if t is None else t.cuda() for t in pair] for pair in own]
+    args = (k.cuda(), v.cuda(), devs[0][0], devs[1][0], table.cuda(), dev[4], dev[5])
+    for hint in (None, 1):  # (again: what a call leaves, the same call leaves again)
+        ops.kv_cache_append(*args, k_scale=devs[0][1], v_scale=devs[1][1], max_new=hint)
+        if hint is None:
+            for (c, s), x in zip(own, (k, v)):
+                model.append(x.float(), c, s, table, lens, cu)
+        for pair, got in zip(own, devs):
+            for a, b in zip(pair, got):
+                if a is not None:
+                    _equal(b, a)
