@@ -181,6 +181,8 @@ class PagedKVCache:
             args["cu_seqlens"] = self._on_device(self._ends(lens))
         got, lse = ops.attn_fwd_cache(self._packed(q), **args, softmax_scale=softmax_scale, causal=causal, return_lse=return_lse,
                                       out=None if out is None else self._packed(out), max_q=max(lens), max_kv=max(self._host_lens))
+        if q.is_cuda:
+            ops.poll_status(q.device)
         if q.dim() == 4:
             B, S, H, _ = q.shape
             got = got.view(q.shape)

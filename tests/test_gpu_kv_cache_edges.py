@@ -432,3 +432,24 @@ def test_thousands_of_sequences(eight):
             for a, b in zip(pair, got):
                 if a is not None:
                     _equal(b, a)
+
+
+def test_the_class_reports_a_wait_that_ran_out():
+    """A status that a kernel has left is raised by the next attend, as by the other entries of the product path; the scratch is replaced."""
+    from chitudiffusion_b200 import PagedKVCache, _lib
+
+    ops = _ops()
+    dev = torch.device("cuda", torch.cuda.current_device())
+    cache = PagedKVCache(1, 2, 200, device=dev)
+    k, q = torch.randn(1, 50, 2, 128, device=dev).to(BF16), torch.randn(1, 50, 4, 128, device=dev).to(BF16)
+    cache.append(k, k)
+    want = cache.attend(q)[0]
+    torch.cuda.synchronize()
+    try:
+        ops.status_word(dev).fill_(3)
+        with pytest.raises(_lib.ChituB200Error, match="softmax"):
+            cache.attend(q)
+        assert not any(used[0] == dev.index for used in ops._workspaces)
+        assert torch.equal(cache.attend(q)[0], want)
+    finally:
+        ops.status_word(dev).zero_()
