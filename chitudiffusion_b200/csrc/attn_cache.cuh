@@ -107,10 +107,10 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t a) {
 // run that ends inside an item (sequence, rows, head) leaves the item's fp32 piece in scratch, and the CTA that completes the
 // item's count merges its pieces in order; nobody waits.
 //
-// 64 sequences of 3 to 16300 keys, one token each, 32 query heads over 8, 8-bit pages of 64: 190 us, 5.7 TB/s of keys and values (four
-// times as long: 6.5 TB/s, the rate of a copy); two of 125000 in pages of 16: 96 us (101 with a merge of 28 pieces in four
-// turns rather than two); 16-bit pages of 32, 16 sequences of 500 to 8191: 105 us,
-// 5.4 TB/s.  The first version, a block per 256 keys and loads through registers, took 329, 183 and 178.
+// 64 sequences of 3 to 16300 keys, one token each, 32 query heads over 8, 8-bit pages of 64: 198 us, 5.4 TB/s of keys and values, one pass
+// behind the other, 215 us among other work (four times as long: 6.5 TB/s, the rate of a copy); two of 125000 in pages of 16: 99 and
+// 106 us (a merge of 28 pieces in four turns rather than two costs 5 more); 16-bit pages of 32, 16 sequences of 500 to 8191: 108 us,
+// 5.3 TB/s.  The first version, a block per 256 keys and loads through registers, took 329, 183 and 178.
 //
 // A warp takes 32 (16-bit pages: 16) of a tile's keys and keeps its own softmax.  The matrix instructions' sum over channels and the
 // output's channels may be numbered as is convenient, so a lane's fragments are whole 16-byte pieces of cache rows: for q k^T, of

@@ -13,9 +13,10 @@
 //                    page, or 128 rows of one; page numbers are the outermost coordinate, and one outside the pool reads
 //                    zeros) and the scales of a tile's sixteen-key groups
 //
-// Measured: 4680 queries over 32760 keys, 12 heads, 8-bit pages of 128: 759 us, 1241 TFLOP/s (attn_persist_kernel on the same keys
-// in 16 bits: 706); four causal chunks of 389 to 512 tokens over up to 8100 keys, 32 query heads over 8, pages of 64: 148 us,
-// 980 TFLOP/s.  A block of one tile's rows has one chain of scores, exponentials and products, and the SM waits for it: split
+// Measured: 4680 queries over 32760 keys, 12 heads, 8-bit pages of 128: 773 us, 1218 TFLOP/s on a cool card, 898 us and 1049 under the
+// power cap (attn_persist_kernel on the same keys in 16 bits: 706, 831); four causal chunks of 389 to 512 tokens over up to 8100
+// keys, 32 query heads over 8, pages of 64: 150 us, 969 TFLOP/s, among other work 162 us, 897.  16-bit pages, cool card: 904 us and,
+// for chunks of that kind, 140 us where 8-bit ones take 140 as well.  A block of one tile's rows has one chain of scores, exponentials and products, and the SM waits for it: split
 // over both halves of the CTA (every second key tile each) 64 such blocks of 16000 keys took 746 us instead of 823, but the
 // code that it needs cost the cases above 0.5 %, and a form of its own with more copies in flight (673) cost shorter ones 3 to 7 %.
 //

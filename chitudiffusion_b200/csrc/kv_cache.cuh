@@ -95,7 +95,7 @@ constexpr int kRotaryThreads = 256;
 
 // Memory bound.  A thread owns a piece of a token's heads: the factors are read once and stay in registers while it walks
 // heads_each heads of a tensor (blockIdx.y picks which), four of them in flight.  The first ones are asked for before the
-// position is known, whose factors are two loads away.  32760 tokens, 24 heads of 128: 69 us, 6.1 TB/s (one head in flight 78).
+// position is known, whose factors are two loads away.  32760 tokens, 24 heads of 128: 72 us, 5.9 TB/s (one head in flight 78).
 template <int kDtype, bool kInterleaved>
 __global__ void __launch_bounds__(kRotaryThreads)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
@@ -242,7 +242,7 @@ __device__ __forceinline__ void cp_async_wait() {
 // rows of a page or of the queries - of `turns` groups of heads one after the other, 4 threads per row and head, each with two rows'
 // pieces.  The rows' factors stay in registers; values come through a ring of copies, each thread reading what it copied, so
 // that a block has 48 KB on their way while it computes.  Memory bound: 12 prompts of 61 to 2603 tokens, 48 heads, 8-bit pages
-// of 64: 75 us, 5.1 TB/s; with a group of heads per block and loads to registers 122.  blockIdx.x is (sequence, run of rows), y
+// of 64: 76 us, 5.0 TB/s; with a group of heads per block and loads to registers 122.  blockIdx.x is (sequence, run of rows), y
 // the heads: k, v, q.
 template <int kThreads>
 struct AppendShape {

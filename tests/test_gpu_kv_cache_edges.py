@@ -374,7 +374,7 @@ def test_projections_pools_and_scales_of_any_strides(n, forms, eight):
 
 
 @pytest.mark.parametrize("eight", [True, False])
-@pytest.mark.parametrize("n,group", [(1, 4), (40, 4), (300, 2), (1, 129), (3, 200), (40, 130)])
+@pytest.mark.parametrize("n,group", [(1, 4), (40, 4), (300, 2), (1, 100), (5, 128), (7, 43), (1, 129), (3, 200), (40, 130)])
 def test_outputs_off_the_32_byte_grid_and_many_heads_of_a_key_head(n, group, eight):
     ops = _ops()
     heads, page, lens = 2, 64, [n + 200, n]
