@@ -63,7 +63,7 @@ constexpr float kProbShift = 7.f;
 // A value scale of zero has no logarithm: it counts as the smallest normal number.  l = sum p / vs has to stay finite, so the
 // running maximum takes scales below 2^-82 for 2^-82: a weight p / vs is then at most 2^(15 + 82), and a sequence has at most
 // 2^30 keys.  Probabilities keep the true scale, so where all scales of a row are below 2^-82 by 2^x, its largest ones come to
-// 2^(7 - x) and end in fp16's last steps of 2^-24: values of 2^-100 still have most of their bits, those near 2^-117 are zeros.
+// 2^(7 - x) and end in fp16's last steps of 2^-24: weights of values of 2^-92 have all their 11 bits, of 2^-105 none.
 constexpr float kMinValueScale = FLT_MIN;
 constexpr float kLowValueLog2 = -82.f;
 

@@ -16,9 +16,10 @@
 // Measured: 4680 queries over 32760 keys, 12 heads, 8-bit pages of 128: 773 us, 1218 TFLOP/s on a cool card, 898 us and 1049 under the
 // power cap (attn_persist_kernel on the same keys in 16 bits: 706, 831); four causal chunks of 389 to 512 tokens over up to 8100
 // keys, 32 query heads over 8, pages of 64: 150 us, 969 TFLOP/s, among other work 162 us, 897.  16-bit pages, cool card: 904 us and,
-// for chunks of that kind, 140 us where 8-bit ones take 140 as well.  A block of one tile's rows has one chain of scores, exponentials and products, and the SM waits for it: split
-// over both halves of the CTA (every second key tile each) 64 such blocks of 16000 keys took 746 us instead of 823, but the
-// code that it needs cost the cases above 0.5 %, and a form of its own with more copies in flight (673) cost shorter ones 3 to 7 %.
+// for chunks of like sizes, 140 us where 8-bit ones take 140 as well.  A block of one tile's rows has one chain of scores,
+// exponentials and products, and the SM waits for it: split over both halves of the CTA (every second key tile each) 64 such blocks of
+// 16000 keys took 746 us instead of 823, but the code that it needs cost the cases above 0.5 %, and a form of its own with more
+// copies in flight (673) cost shorter ones 3 to 7 %.
 //
 // Widening costs the SM sub-partitions' issue slots (about 100 instructions per warp and tile) rather than a pass over
 // memory: read back from a 16-bit copy of the cache, three frames over 21 would move 200 MB more.
@@ -238,8 +239,9 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
 // One softmax step (thread = one row, 128 scores): scores in, probabilities out.  As persist_softmax_step, with a factor and an
 // addend for each sixteen keys (coef: key scale, log2 of the value scale, the scale's inverse, the logarithm as the maximum takes
 // it) and, in a form of its own that keeps the other one short, `valid` keys visible to this row.  m is the largest (score factor +
-// addend) so far in log2 units, moved only when it has grown by more than 2^8.  Hidden scores are -inf before they meet their factor, which therefore is not allowed
-// to vanish there: a row of zeros has 2^-126 of its own, and a small key scale would take it to 0 and the score to NaN.
+// addend) so far in log2 units, moved only when it has grown by more than 2^8.  Hidden scores are -inf before they meet their
+// factor, which therefore may not vanish: a row of zeros has 2^-126 of its own, and a small key scale would take it to 0 and the
+// score to NaN.
 template <bool kHalf, bool kMasked>
 __device__ __forceinline__ void tile_softmax_step(const TileRefs& r, int step, bool first, int valid, float row_factor, const float4* coef,
                                                   float& m, float& l_sum, volatile int* abort_flag, int* status) {

@@ -1,16 +1,16 @@
 """A paged key/value cache with its bookkeeping: pools, page tables and lengths of a batch of sequences.
 
 The arithmetic is in ``ops.kv_cache_append`` and ``ops.attn_fwd_cache``; this class allots pages, keeps the tables on the GPU up to
-date and hands both operators what they need; no call waits for the GPU.  Generation frame by frame (the frames made so far are the keys of the next
-chunk), a prompt taken in chunks and single tokens are the same two calls::
+date and hands both operators what they need; no call waits for the GPU.  Generation frame by frame (the frames made so far are the
+keys of the next chunk), a prompt taken in chunks and single tokens are the same two calls::
 
     cache = PagedKVCache(batch=2, num_heads=8, max_tokens=4096, device="cuda")
     q = cache.append(k, v, q=q, rope_table=table)        # [B, S, H, 128], or packed tokens and new_lens=[...]
     out, lse = cache.attend(q, causal=True)
 
 Pages of 8 bits (the default) hold e4m3 codes with a power-of-two scale per page and head: half the memory of 16-bit ones and
-about half the time of a single-token step (64 sequences of up to 16300 keys, 8 key heads: 205 us against 368).  (The reference keeps the gathered keys of a layer as 16-bit tensors,
-modules/attention/image_cp_attention.py:131-205.)
+about half the time of a single-token step (64 sequences of up to 16300 keys, 8 key heads: 205 us against 368).  (The reference
+keeps the gathered keys of a layer as 16-bit tensors, modules/attention/image_cp_attention.py:131-205.)
 """
 
 from __future__ import annotations

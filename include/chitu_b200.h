@@ -485,8 +485,9 @@ int chitu_b200_stamp(unsigned long long* slot, void* stream);
  * and lens[b] counts the tokens that sequence b holds, those of the current call included.  A pool holds the inputs' 16-bit
  * type, or e4m3 codes (CHITU_CACHE_E4M3) with one fp32 scale per page and head: value = code * scale (scales are
  * finite and not below zero; attention takes value scales below 2^-126 for that).  Tokens of several sequences are packed:
- * sequence b's are rows cu_seqlens[b] ... cu_seqlens[b + 1] - 1.  Rows behind the last sequence are left as they are.  lens, cu_seqlens and block_table are device memory and are not looked at by the host: page numbers
- * outside [0, n_pages) are neither read nor written, lengths are cut to what the table can hold.
+ * sequence b's are rows cu_seqlens[b] ... cu_seqlens[b + 1] - 1.  Rows behind the last sequence are left as they are.  lens,
+ * cu_seqlens and block_table are device memory and are not looked at by the host: page numbers outside [0, n_pages) are
+ * neither read nor written, lengths are cut to what the table can hold.
  */
 #define CHITU_CACHE_16BIT 0
 #define CHITU_CACHE_E4M3 1
