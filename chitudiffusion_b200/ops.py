@@ -233,12 +233,12 @@ def _split_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
 
 
 def _cut_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Scratch for the cut query blocks of eager calls on the current stream of ``device``.
+    """Scratch for the cut query blocks of eager calls on the current stream of ``device``, and for attention over a cache.
 
     Never the buffer of :func:`splitkv_workspace`, whose address a caller's captured graph may hold.  A cut's need has a
-    bound, so the buffer is made once at that size (39 MB).  The buffers made last are kept; an older one goes back to
-    torch's allocator, which reuses it in its stream's order.  None is kept past a wait that ran out (see
-    :func:`check_status`).
+    bound, so the buffer is made once at that size (39 MB; cache attention's bound is 0.4 MB above it).  The buffers made
+    last are kept; an older one goes back to torch's allocator, which reuses it in its stream's order.  None is kept past a
+    wait that ran out (see :func:`check_status`).
     """
     key = (_device_key(device), _stream_ptr(device))
     ws = _cut_scratches.get(key)
@@ -1151,11 +1151,11 @@ def kv_cache_append(
 
 
 def _cache_scratch(device: torch.device, nbytes: int) -> torch.Tensor:
-    """:func:`_split_scratch` with the eager buffer looked up first."""
-    if torch._C._cuda_getDevice() == _device_key(device) and not torch.cuda.is_current_stream_capturing():
-        ws = _workspaces.get((_device_key(device), _stream_ptr(device)))
-        if ws is not None and ws.numel() >= nbytes:
-            return ws
+    """Scratch of one call: of an eager one that of the cuts (:func:`_cut_scratch`; a stream's calls follow one another, and both leave the
+    counters at its head zero), of a captured one its own (:func:`_split_scratch`)."""
+    with _on(device):
+        if not torch.cuda.is_current_stream_capturing():
+            return _cut_scratch(device, nbytes)
     return _split_scratch(device, nbytes)
 
 

@@ -449,7 +449,32 @@ def test_the_class_reports_a_wait_that_ran_out():
         ops.status_word(dev).fill_(3)
         with pytest.raises(_lib.ChituB200Error, match="softmax"):
             cache.attend(q)
-        assert not any(used[0] == dev.index for used in ops._workspaces)
+        assert not any(used[0] == dev.index for used in [*ops._workspaces, *ops._cut_scratches])
         assert torch.equal(cache.attend(q)[0], want)
     finally:
         ops.status_word(dev).zero_()
+
+
+def test_dense_and_cache_attention_in_turn_on_one_stream():
+    """Query blocks cut for an even end, blocks of a cache that runs' borders cut, and few rows share a stream's scratch."""
+    ops = _ops()
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    S, H, page = 2400, 16, 64
+    assert ops._balanced_workspace_bytes(torch.cuda.current_device(), 1, S, S, H) > 0  # (this call is cut)
+    q, k, v = (torch.randn(1, S, H, 128, generator=gen, device="cuda").to(BF16) for _ in range(3))
+    pools = [torch.randn(80, page, 2, 128, generator=gen, device="cuda").to(BF16) for _ in range(2)]
+    table = torch.randperm(80, generator=gen, device="cuda").int()[None]
+    lens = torch.tensor([5000], dtype=torch.int32, device="cuda")
+    calls = [lambda: ops.attn_fwd(q, k, v, return_lse=True)]
+    for n in (1, 700):
+        x, cu = torch.randn(n, 16, 128, generator=gen, device="cuda").to(BF16), torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        calls.append(lambda x=x, cu=cu, n=n: ops.attn_fwd_cache(x, *pools, table, lens, cu, causal=True, return_lse=True, max_q=n))
+    wants = []
+    for call in calls:  # each by itself, in scratch of its own
+        with torch.cuda.stream(torch.cuda.Stream()):
+            wants.append(call())
+            torch.cuda.synchronize()
+    for _ in range(5):
+        for i in (0, 1, 0, 2, 1, 2):
+            for got, want in zip(calls[i](), wants[i]):
+                assert torch.equal(got, want)

@@ -198,3 +198,27 @@ def test_an_append_refuses_scales_that_share_memory(which, scale):
         ops.kv_cache_append(k, k, **a)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):  # (which is looked at last)
         ops.attn_fwd_cache(k, **a)
+
+
+# ------------------------------------------------------------------------------------------------ scratch
+def test_cache_attention_never_uses_the_key_split_buffer(monkeypatch):
+    """That buffer's address may be part of a caller's captured graph, which is replayed on any stream beside eager calls."""
+    cpu = torch.device("cpu")
+    capturing = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: type("S", (), {"cuda_stream": 11})())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    for name, value in (("_stream_ptr", lambda dev: 11), ("_device_key", lambda dev: 0), ("_on", lambda dev: ops._NO_GUARD), ("_workspaces", {}),
+                        ("_retired_workspaces", []), ("_cut_scratches", {})):
+        monkeypatch.setattr(ops, name, value)
+    held = ops.splitkv_workspace(cpu, 50 << 20)  # as a captured call's workspace=
+    eager = ops._cache_scratch(cpu, 3 << 20)
+    assert eager.data_ptr() != held.data_ptr() and not eager[:ops.SPLIT_HEADER_BYTES].any()
+    assert ops._cache_scratch(cpu, 3 << 20) is eager
+    larger = ops._cache_scratch(cpu, 45 << 20)
+    assert larger.numel() >= 45 << 20 and larger.data_ptr() != held.data_ptr() and not larger[:ops.SPLIT_HEADER_BYTES].any()
+    assert ops._cache_scratch(cpu, 3 << 20) is larger
+    capturing.append(True)
+    own = [ops._cache_scratch(cpu, 3 << 20) for _ in range(2)]
+    assert len({t.data_ptr() for t in own + [held, larger]}) == 4 and not own[0][:ops.SPLIT_HEADER_BYTES].any()
